@@ -224,6 +224,88 @@ int spark_kv_store(const uint16_t* k, const uint16_t* v, const int64_t* slot_map
 int spark_slot_mapping(int64_t num_tokens, int64_t max_tokens, const int32_t* query_start, const int64_t* positions,
                        const int32_t* block_table, int64_t block_size, int64_t* out, void* stream);
 
+/* ======================================================================
+ * Batches of requests over the paged cache.
+ *
+ * The reference leaves these to vLLM's torch path (integration/model.py:50-62: query
+ * length > 1) and maps slots for one request at a time (integration/slot_mapping.py:8-22).
+ * `error` (int32 on the device, required) collects bits: 4 a negative length or
+ * descending starts, 8 the free list ran out, 16 a request longer than its block table
+ * row, 32 more tokens than output rows, 64 a block table entry outside the cache, 128 a
+ * position outside the rotation table, 256 a slot outside the cache; 1 and 2 as in
+ * spark_q4_gemm_tc.  What does not fit is skipped, never dereferenced.
+ * ====================================================================== */
+
+/* Block tables, token positions and slot maps from request lengths, in one launch.
+ * Request r has ctx_lens[r] cached and new_lens[r] new tokens (either may be 0):
+ *   query_start[r] = sum of new_lens below r (int32 [reqs + 1]), seq_lens[r] = ctx + new;
+ *   its pages ceil(ctx / bs) .. ceil((ctx + new) / bs) - 1 are written to
+ *   block_table[r * table_stride + page] from free_blocks[*free_head ...], in request
+ *   order, and *free_head_out = *free_head + pages taken (may be the same tensor);
+ *   row i (a token) gets its position and slot = page id * bs + offset, rows behind the
+ *   last token position 0 and slot -1 (int64 [rows] both).
+ * free_blocks NULL (then free_head and free_head_out too): the tables are complete
+ * already, nothing is taken.  A batch that does not fit (bits 4, 8, 16, 32) comes out
+ * empty -- all starts and lengths 0, all slots -1 -- and takes no page.  counter: int32,
+ * zero before the first call, left zero; calls that may overlap need one each.
+ * reqs <= 8192. */
+int spark_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int reqs, const int32_t* free_blocks,
+                     int num_free, const int32_t* free_head, int32_t* free_head_out, int32_t* block_table,
+                     int64_t table_stride, int table_width, int block_size, int rows, int32_t* query_start,
+                     int32_t* seq_lens, int64_t* positions, int64_t* slot_mapping, int* counter, int* error,
+                     void* stream);
+
+/* Per-head RMS norm of q and k (q_gamma, k_gamma bf16 [head_dim], both or neither NULL),
+ * neox rotation and the paged K / V store of `rows` rows of a fused qkv output (row r at
+ * qkv + r * row_stride: nq query heads, nkv key heads, nkv value heads; anything behind
+ * them is ignored) in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * gamma;  pairs (i, i + rotary_dim / 2) rotated by row
+ *   positions[r] of cos_sin (bf16 [max_pos][rotary_dim], cos | sin),
+ * in fp32 with one rounding to bf16 at the end.  q -> q_out bf16 [rows][nq][head_dim]; k
+ * and v -> the caches at slot_mapping[r] (negative: padding, not stored).  A row whose
+ * position is outside the table writes no q and no k (bit 128).  head_dim 128 or 256,
+ * rotary_dim % 16 == 0; row_stride % 8 == 0, 16-byte aligned tensors.  Replaces the
+ * rotation and store of FusedQkvStage (kernels/qkv.py:179-198) for many rows. */
+int spark_qk_norm_rope_store_rows(const uint16_t* qkv, int64_t row_stride, int rows, int nq, int nkv, int head_dim,
+                                  const uint16_t* q_gamma, const uint16_t* k_gamma, float eps,
+                                  const uint16_t* cos_sin, int64_t max_pos, int rotary_dim, const int64_t* positions,
+                                  const int64_t* slot_mapping, int block_size, int64_t num_blocks, uint16_t* k_cache,
+                                  uint16_t* v_cache, uint16_t* q_out, int* error, void* stream);
+
+/* Work list of spark_attn_paged, made on the device once per step and used by every layer
+ * of the same head layout and window.  query_start given: a packed batch, request r's
+ * query tokens are [query_start[r], query_start[r + 1]) and sit at the last positions of
+ * its seq_lens[r] keys; `window` > 0: each token attends to its last `window` positions,
+ * itself included.  prefix_len given (device int32, and query_start NULL): one query token
+ * per request, request r attends to all its seq_lens[r] keys, the first *prefix_len of
+ * which are the same for all and are read through the first request's table, once.
+ * plan: spark_attn_plan_bytes bytes for the same maxima, 16-byte aligned;
+ * reqs <= max_reqs.  Starts outside [0, max_tokens] or descending drop the request. */
+int64_t spark_attn_plan_bytes(int max_tokens, int max_reqs, int nq, int nkv, int head_dim);
+int64_t spark_attn_part_rows(int max_tokens, int max_reqs, int nq, int nkv, int head_dim);
+int spark_attn_plan(const int32_t* query_start, const int32_t* seq_lens, const int32_t* prefix_len, int reqs,
+                    int max_tokens, int max_reqs, int nq, int nkv, int head_dim, int window, void* plan, int* error,
+                    void* stream);
+
+/* Attention of the planned batch over the paged caches (bf16
+ * [num_blocks][nkv][block_size][head_dim], block_size a multiple of 16): for query token
+ * t (q + t * q_tok_stride + head * q_head_stride, bf16) out = softmax(scale * q.k) v over
+ * the keys its plan gives it, fp32 statistics; a token without keys is zero.  Rows of out
+ * behind the last planned token are left alone.  K and V of positions at or past a
+ * request's length may hold anything (NaN included).  head_dim 128 or 256, nq / nkv any
+ * integer up to 128, scale > 0; strides in elements, multiples of 8; the maxima and window
+ * are the plan's.  part_o fp32 [spark_attn_part_rows][nkv][head_dim] and part_ml fp32
+ * [spark_attn_part_rows][nkv][2] are workspace: calls that may overlap need a plan and
+ * workspace each.  wait_ns bounds each wait inside the kernel as in spark_q4_gemm_tc; bit
+ * 1 of *error: a wait ran out and out is not valid.  Replaces vLLM's torch attention of
+ * the reference's prefill (integration/model.py:50-62). */
+int spark_attn_paged(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int tokens,
+                     const uint16_t* k_cache, const uint16_t* v_cache, int64_t num_blocks, int block_size,
+                     const int32_t* block_table, int64_t table_stride, int table_width, int max_tokens, int max_reqs,
+                     int nq, int nkv, int head_dim, int window, float scale, const void* plan, float* part_o,
+                     float* part_ml, uint16_t* out, int64_t out_tok_stride, int64_t out_head_stride, int* error,
+                     int64_t wait_ns, void* stream);
+
 /* Enable / disable programmatic dependent launch on the kernels above (default on). */
 int spark_set_pdl(int enabled);
 

@@ -1,0 +1,149 @@
+// paged.cu -- C ABI entry points of the paged-batch operators (include/spark_b200.h).
+// Sizes, strides and alignments are checked here, before any launch.
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+
+#include "host.cuh"
+#include "paged.cuh"
+#include "spark_b200.h"
+
+using namespace spark;
+
+extern "C" {
+
+int spark_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int reqs, const int32_t* free_blocks,
+                     int num_free, const int32_t* free_head, int32_t* free_head_out, int32_t* block_table,
+                     int64_t table_stride, int table_width, int block_size, int rows, int32_t* query_start,
+                     int32_t* seq_lens, int64_t* positions, int64_t* slot_mapping, int* counter, int* error,
+                     void* stream) {
+  if (!ctx_lens || !new_lens || !block_table || !query_start || !seq_lens || !error || !counter)
+    return SPARK_ERR_INVALID_ARG;
+  if (rows > 0 && (!positions || !slot_mapping)) return SPARK_ERR_INVALID_ARG;
+  if (free_blocks ? (!free_head || !free_head_out) : (free_head || free_head_out)) return SPARK_ERR_INVALID_ARG;
+  if (reqs <= 0 || rows < 0 || num_free < 0 || block_size <= 0 || table_width <= 0 || table_stride < table_width)
+    return SPARK_ERR_UNSUPPORTED_SHAPE;
+  if (reqs > paged::kPlanMaxReqs) return SPARK_ERR_TOO_LARGE;
+  paged::PlanArgs p;
+  memset(&p, 0, sizeof(p));
+  p.ctx = ctx_lens, p.nw = new_lens, p.free_ids = free_blocks, p.free_head = free_head;
+  p.free_head_out = free_head_out, p.table = block_table, p.query_start = query_start, p.seq_lens = seq_lens;
+  p.positions = positions, p.slots = slot_mapping, p.table_stride = table_stride;
+  p.reqs = reqs, p.num_free = num_free, p.width = table_width, p.bs = block_size, p.rows = rows;
+  p.counter = counter, p.error = error;
+  const int64_t units = std::max<int64_t>(rows, reqs);
+  const int grid = (int)std::min<int64_t>((units + paged::kPlanThreads - 1) / paged::kPlanThreads, num_sms());
+  return launch(paged::paged_plan_kernel, dim3(grid), dim3(paged::kPlanThreads), 2 * ((size_t)reqs + 1) * 4,
+                as_stream(stream), p);
+}
+
+int spark_qk_norm_rope_store_rows(const uint16_t* qkv, int64_t row_stride, int rows, int nq, int nkv, int head_dim,
+                                  const uint16_t* q_gamma, const uint16_t* k_gamma, float eps,
+                                  const uint16_t* cos_sin, int64_t max_pos, int rotary_dim, const int64_t* positions,
+                                  const int64_t* slot_mapping, int block_size, int64_t num_blocks, uint16_t* k_cache,
+                                  uint16_t* v_cache, uint16_t* q_out, int* error, void* stream) {
+  if (!cos_sin || !positions || !slot_mapping || !k_cache || !v_cache || !error) return SPARK_ERR_INVALID_ARG;
+  if ((q_gamma == nullptr) != (k_gamma == nullptr)) return SPARK_ERR_INVALID_ARG;
+  if (rows < 0 || nq <= 0 || nkv <= 0 || (head_dim != 128 && head_dim != 256) || rotary_dim <= 0 ||
+      rotary_dim % 16 || rotary_dim > head_dim || max_pos <= 0 || block_size <= 0 || num_blocks <= 0)
+    return SPARK_ERR_UNSUPPORTED_SHAPE;
+  if (row_stride < (int64_t)(nq + 2 * nkv) * head_dim) return SPARK_ERR_UNSUPPORTED_SHAPE;
+  if (rows == 0) return SPARK_OK;
+  if (!qkv || !q_out) return SPARK_ERR_INVALID_ARG;
+  if (row_stride % 8 || !aligned(qkv, 16) || !aligned(cos_sin, 16) || !aligned(k_cache, 16) ||
+      !aligned(v_cache, 16) || !aligned(q_out, 16) || (q_gamma && (!aligned(q_gamma, 16) || !aligned(k_gamma, 16))))
+    return SPARK_ERR_ALIGNMENT;
+  paged::RopeArgs p;
+  memset(&p, 0, sizeof(p));
+  p.qkv = qkv, p.qg = q_gamma, p.kg = k_gamma, p.cos_sin = cos_sin, p.positions = positions, p.slots = slot_mapping;
+  p.k_cache = k_cache, p.v_cache = v_cache, p.q_out = q_out, p.row_stride = row_stride, p.max_pos = max_pos;
+  p.num_slots = num_blocks * block_size, p.eps = eps, p.rows = rows, p.nq = nq, p.nkv = nkv, p.rot = rotary_dim;
+  p.bs = block_size, p.error = error;
+  const int per_cta = 256 / (head_dim / 8);
+  const int64_t total = (int64_t)rows * (nq + 2 * nkv);
+  const int grid = (int)std::min<int64_t>((total + per_cta - 1) / per_cta, 8LL * num_sms());
+  if (head_dim == 128)
+    return launch(paged::rope_store_kernel<128>, dim3(grid), dim3(256), 0, as_stream(stream), p);
+  return launch(paged::rope_store_kernel<256>, dim3(grid), dim3(256), 0, as_stream(stream), p);
+}
+
+// ------------------------------------------------------------------ paged attention
+static int check_attn_shape(int max_tokens, int max_reqs, int nq, int nkv, int head_dim) {
+  if (max_tokens <= 0 || max_reqs <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || nq / nkv > 128 ||
+      (head_dim != 128 && head_dim != 256))
+    return SPARK_ERR_UNSUPPORTED_SHAPE;
+  // tile, item and partial-row counts are 32-bit
+  if (max_tokens > (1 << 22) || max_reqs > (1 << 16) || nkv > 4096) return SPARK_ERR_TOO_LARGE;
+  return SPARK_OK;
+}
+
+int64_t spark_attn_plan_bytes(int max_tokens, int max_reqs, int nq, int nkv, int head_dim) {
+  if (check_attn_shape(max_tokens, max_reqs, nq, nkv, head_dim)) return -1;
+  return paged::layout_of(max_tokens, max_reqs, nq, nkv, head_dim).bytes;
+}
+
+int64_t spark_attn_part_rows(int max_tokens, int max_reqs, int nq, int nkv, int head_dim) {
+  if (check_attn_shape(max_tokens, max_reqs, nq, nkv, head_dim)) return -1;
+  return paged::layout_of(max_tokens, max_reqs, nq, nkv, head_dim).part_rows;
+}
+
+int spark_attn_plan(const int32_t* query_start, const int32_t* seq_lens, const int32_t* prefix_len, int reqs,
+                    int max_tokens, int max_reqs, int nq, int nkv, int head_dim, int window, void* plan, int* error,
+                    void* stream) {
+  if (!seq_lens || !plan || !error || (query_start == nullptr) == (prefix_len == nullptr))
+    return SPARK_ERR_INVALID_ARG;
+  int st = check_attn_shape(max_tokens, max_reqs, nq, nkv, head_dim);
+  if (st) return st;
+  if (reqs < 0 || reqs > max_reqs || (prefix_len && reqs > max_tokens) || window < 0 || (prefix_len && window))
+    return SPARK_ERR_UNSUPPORTED_SHAPE;
+  if (!aligned(plan, 16)) return SPARK_ERR_ALIGNMENT;
+  paged::AttnPlanArgs p;
+  memset(&p, 0, sizeof(p));
+  p.query_start = query_start, p.seq_lens = seq_lens, p.prefix_len = prefix_len;
+  p.reqs = reqs, p.tokens = max_tokens, p.nq = nq, p.nkv = nkv, p.D = head_dim, p.window = window;
+  p.lay = paged::layout_of(max_tokens, max_reqs, nq, nkv, head_dim);
+  p.plan = static_cast<unsigned char*>(plan), p.error = error;
+  return launch(paged::attn_plan_kernel, dim3(1), dim3(paged::kAttnPlanThreads), 0, as_stream(stream), p);
+}
+
+int spark_attn_paged(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int tokens,
+                     const uint16_t* k_cache, const uint16_t* v_cache, int64_t num_blocks, int block_size,
+                     const int32_t* block_table, int64_t table_stride, int table_width, int max_tokens, int max_reqs,
+                     int nq, int nkv, int head_dim, int window, float scale, const void* plan, float* part_o,
+                     float* part_ml, uint16_t* out, int64_t out_tok_stride, int64_t out_head_stride, int* error,
+                     int64_t wait_ns, void* stream) {
+  if (!k_cache || !v_cache || !block_table || !plan || !part_o || !part_ml || !error) return SPARK_ERR_INVALID_ARG;
+  int st = check_attn_shape(max_tokens, max_reqs, nq, nkv, head_dim);
+  if (st) return st;
+  if (tokens < 0 || tokens > max_tokens || num_blocks <= 0 || block_size < 16 || block_size % 16 ||
+      table_width <= 0 || table_stride < 0 || window < 0 || !(scale > 0.0f) || scale > 1e30f)
+    return SPARK_ERR_UNSUPPORTED_SHAPE;
+  if (tokens == 0) return SPARK_OK;
+  if (!q || !out) return SPARK_ERR_INVALID_ARG;
+  // tensor-map coordinates are 32-bit rows of the caches
+  if (num_blocks * nkv * block_size > 0x7fffffffLL - 128) return SPARK_ERR_TOO_LARGE;
+  if (q_tok_stride % 8 || q_head_stride % 8 || out_tok_stride % 8 || out_head_stride % 8 || !aligned(q, 16) ||
+      !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(out, 16) || !aligned(plan, 16) ||
+      !aligned(part_o, 16) || !aligned(part_ml, 8))
+    return SPARK_ERR_ALIGNMENT;
+  paged::AttnArgs p;
+  memset(&p, 0, sizeof(p));
+  p.q = q, p.k_cache = k_cache, p.v_cache = v_cache, p.table = block_table, p.table_stride = table_stride;
+  p.q_tok = q_tok_stride, p.q_head = q_head_stride, p.o_tok = out_tok_stride, p.o_head = out_head_stride;
+  p.num_blocks = num_blocks, p.table_width = table_width, p.bs = block_size, p.tokens = tokens;
+  p.nq = nq, p.nkv = nkv, p.window = window, p.scale = scale;
+  p.plan = static_cast<const unsigned char*>(plan);
+  p.lay = paged::layout_of(max_tokens, max_reqs, nq, nkv, head_dim);
+  p.part_o = part_o, p.part_ml = reinterpret_cast<float2*>(part_ml), p.out = out, p.error = error;
+  (void)wait_ns;
+  const dim3 grid((unsigned)std::min<int64_t>((int64_t)p.lay.max_items * nkv, 8LL * num_sms()));
+  const dim3 cgrid((unsigned)std::min<int64_t>((int64_t)p.lay.max_entries * nkv, 4LL * num_sms()));
+  if (head_dim == 128) {
+    st = launch(paged::attn_rows_kernel<128>, grid, dim3(256), 0, as_stream(stream), p);
+    return st ? st : launch(paged::combine_kernel<128>, cgrid, dim3(256), 0, as_stream(stream), p);
+  }
+  st = launch(paged::attn_rows_kernel<256>, grid, dim3(256), 0, as_stream(stream), p);
+  return st ? st : launch(paged::combine_kernel<256>, cgrid, dim3(256), 0, as_stream(stream), p);
+}
+
+}  // extern "C"

@@ -1,0 +1,703 @@
+// paged.cuh -- kernels of a batch of requests over the paged KV cache: block tables and
+// slot maps from request lengths, the per-head norm + rotation + store of new rows, the
+// work list of the paged attention, and the join of its partial results.
+//
+// All metadata lives on the device and is checked there: lengths, page ids and slots that
+// do not fit are recorded in the caller's error word (kBad*) and never dereferenced.
+#pragma once
+
+#include "common.cuh"
+
+namespace spark {
+namespace paged {
+
+// error word bits (the attention kernel's wait codes 1 and 2 are in attn_paged.cuh)
+constexpr int kBadLength = 4;    // a negative length, or starts that go down
+constexpr int kNoPages = 8;      // the free list is shorter than the pages needed
+constexpr int kTableWidth = 16;  // a request is longer than its block table row
+constexpr int kNoRows = 32;      // more tokens than output rows
+constexpr int kBadPage = 64;     // a block table entry outside the cache
+constexpr int kBadPosition = 128;  // a position outside the rotation table
+constexpr int kBadSlot = 256;    // a slot outside the cache
+
+// ------------------------------------------------------------------ block tables and slot maps
+// Requests r = 0 .. R-1 with ctx[r] cached and nw[r] new tokens:
+//   start[r] = sum of nw below r, len[r] = ctx[r] + nw[r];
+//   pages ceil(ctx / bs) .. ceil(len / bs) - 1 of request r are the next ids of the free
+//   list, in request order (free == nullptr: the table holds them already);
+//   token t of request r: position ctx[r] + t - start[r], slot = page * bs + offset.
+// Every CTA scans the R lengths itself (R <= kPlanMaxReqs: 8 bytes each, from L2) and
+// keeps token starts and page starts in shared memory, so one launch does it all: the
+// tokens and the new table entries are then dealt to all threads of the grid, a token
+// finding its request by binary search.  All or nothing: when something does not fit,
+// every CTA sees it in its own scan, no page is taken and the batch comes out empty.
+constexpr int kPlanThreads = 512;
+constexpr int kPlanMaxReqs = 8192;
+
+struct PlanArgs {
+  const int32_t *ctx, *nw, *free_ids, *free_head;
+  int32_t *free_head_out, *table, *query_start, *seq_lens;
+  int64_t *positions, *slots;
+  int64_t table_stride;
+  int reqs, num_free, width, bs, rows;
+  int *counter, *error;
+};
+
+// inclusive scan over the CTA of two values per thread (sums of up to 8192 int32 values:
+// 64 bits); returns the CTA totals in tot
+__device__ __forceinline__ void block_scan2(long long& a, long long& b, long long (&tot)[2], long long (*ws)[2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) {
+      a += x;
+      b += y;
+    }
+  }
+  if (lane == 31) {
+    ws[warp][0] = a;
+    ws[warp][1] = b;
+  }
+  __syncthreads();
+  long long pa = 0, pb = 0;
+  tot[0] = tot[1] = 0;
+  for (int w = 0; w < (int)(blockDim.x >> 5); w++) {
+    if (w < warp) {
+      pa += ws[w][0];
+      pb += ws[w][1];
+    }
+    tot[0] += ws[w][0];
+    tot[1] += ws[w][1];
+  }
+  a += pa;
+  b += pb;
+  __syncthreads();
+}
+
+// largest r with start[r] <= i (start ascending, start[0] = 0)
+__device__ __forceinline__ int find_request(const int* start, int reqs, int i) {
+  int lo = 0, hi = reqs - 1;
+  while (lo < hi) {
+    const int m = (lo + hi + 1) >> 1;
+    if (start[m] <= i) lo = m;
+    else hi = m - 1;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs p) {
+  extern __shared__ int plan_sm[];
+  __shared__ long long ws[kPlanThreads / 32][2];
+  __shared__ int bad_s;
+  int* start = plan_sm;              // [R + 1]
+  int* page0 = plan_sm + p.reqs + 1;  // [R + 1] new pages below request r
+  const int tid = threadIdx.x, R = p.reqs, bs = p.bs;
+  pdl_wait();
+  if (tid == 0) bad_s = 0;
+  __syncthreads();
+  const int head = p.free_ids ? p.free_head[0] : 0;
+  long long t_sum = 0, p_sum = 0;
+  int bad = 0;
+  for (int r0 = 0; r0 < R; r0 += kPlanThreads) {
+    const int r = r0 + tid;
+    long long n = 0, np = 0;
+    if (r < R) {
+      const long long c = p.ctx[r], w = p.nw[r];
+      if (c < 0 || w < 0 || c + w > 0x7fffffffLL) bad |= kBadLength;
+      else {
+        const long long need = (c + w + bs - 1) / bs;
+        if (need > p.width) bad |= kTableWidth;
+        n = w;
+        np = p.free_ids ? need - (c + bs - 1) / bs : 0;
+      }
+    }
+    long long tot[2], a = n, b = np;
+    block_scan2(a, b, tot, ws);
+    if (r < R) {  // (sums past int32 are refused below before they are read)
+      start[r] = (int)(t_sum + a - n);
+      page0[r] = (int)(p_sum + b - np);
+    }
+    t_sum += tot[0];
+    p_sum += tot[1];
+  }
+  if (tid == 0) {
+    start[R] = (int)t_sum;
+    page0[R] = (int)p_sum;
+  }
+  if (t_sum > p.rows) bad |= kNoRows;
+  if (p.free_ids && (head < 0 || p_sum > (long long)p.num_free - head)) bad |= kNoPages;
+  if (bad) atomicOr(&bad_s, bad);
+  __syncthreads();
+  bad = bad_s;
+  if (bad && blockIdx.x == 0 && tid == 0) atomicOr(p.error, bad);
+  const int tokens = bad ? 0 : (int)t_sum, pages = bad ? 0 : (int)p_sum;
+  const int gtid = blockIdx.x * kPlanThreads + tid, gthreads = gridDim.x * kPlanThreads;
+  for (int r = gtid; r <= R; r += gthreads) {
+    p.query_start[r] = bad ? 0 : start[r];
+    if (r < R) p.seq_lens[r] = bad ? 0 : p.ctx[r] + p.nw[r];
+  }
+  for (int i = gtid; i < pages; i += gthreads) {
+    const int r = find_request(page0, R, i);
+    const int first = (int)(((long long)p.ctx[r] + bs - 1) / bs);
+    p.table[r * p.table_stride + first + (i - page0[r])] = p.free_ids[head + i];
+  }
+  for (int i = gtid; i < p.rows; i += gthreads) {
+    long long pos = 0, slot = -1;
+    if (i < tokens) {
+      const int r = find_request(start, R, i);
+      const int c = p.ctx[r];
+      pos = (long long)c + (i - start[r]);
+      const int pg = (int)(pos / bs), first = (int)(((long long)c + bs - 1) / bs);
+      // a page taken in this call is read from the free list: another CTA may not have
+      // written its table entry yet
+      const int id = p.free_ids && pg >= first ? p.free_ids[head + page0[r] + pg - first]
+                                               : p.table[r * p.table_stride + pg];
+      if (id >= 0) slot = (long long)id * bs + (pos - (long long)pg * bs);
+      else atomicOr(p.error, kBadPage);
+    }
+    p.positions[i] = pos;
+    p.slots[i] = slot;
+  }
+  if (p.free_head_out) {  // after every CTA has read free_head (the two may be one tensor)
+    __syncthreads();
+    if (tid == 0) {
+      __threadfence();
+      if (atomicAdd(p.counter, 1) == (int)gridDim.x - 1) {
+        *p.counter = 0;
+        p.free_head_out[0] = head + pages;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ norm + rotation + store
+// One pass over the rows of a fused qkv output: per head of q and k
+//   y = x * rsqrt(mean(x^2) + eps) * gamma          (gamma == nullptr: y = x)
+//   (y_i, y_{i + r/2}) -> (y_i c_i - y_{i+r/2} s_i, y_{i+r/2} c_i + y_i s_i),  i < r/2
+// in fp32, rounded to bf16 once at the end (the input's own rounding is the last one
+// before it: no bf16 between the norm and the rotation); q to q_out, k and v to the pages
+// at slot_mapping.  D / 8 lanes hold one head, 8 elements (16 bytes) each: the norm is a
+// butterfly over them and the rotation partner is the lane r / 16 away.
+struct RopeArgs {
+  const uint16_t *qkv, *qg, *kg, *cos_sin;
+  const int64_t *positions, *slots;
+  uint16_t *k_cache, *v_cache, *q_out;
+  int64_t row_stride, max_pos, num_slots;
+  float eps;
+  int rows, nq, nkv, rot, bs;
+  int* error;
+};
+
+__device__ __forceinline__ void unpack8(const uint4 u, float (&v)[8]) {
+  v[0] = bf_lo(u.x), v[1] = bf_hi(u.x), v[2] = bf_lo(u.y), v[3] = bf_hi(u.y);
+  v[4] = bf_lo(u.z), v[5] = bf_hi(u.z), v[6] = bf_lo(u.w), v[7] = bf_hi(u.w);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <int D>
+__global__ void __launch_bounds__(256) rope_store_kernel(RopeArgs p) {
+  constexpr int L = D / 8;  // lanes per head
+  pdl_wait();
+  const int nh = p.nq + 2 * p.nkv;
+  const int64_t total = (int64_t)p.rows * nh;
+  const int sub = threadIdx.x % L;
+  const int64_t step = (int64_t)gridDim.x * (256 / L);
+  const int64_t first = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  const int half = p.rot >> 1, hl = half >> 3;  // rotation partner: hl lanes away
+  const int src = (threadIdx.x & 31) + (sub < hl ? hl : (sub < 2 * hl ? -hl : 0));
+  const float sg = sub < hl ? -1.0f : 1.0f;
+  // (all lanes of a warp stay to the last head: the shuffles are the whole warp's)
+  for (int64_t i = first; __any_sync(0xffffffffu, i < total); i += step) {
+    const bool live = i < total;
+    const int64_t row = live ? i / nh : 0;
+    const int h = live ? (int)(i - row * nh) : 0;
+    const bool is_v = h >= p.nq + p.nkv, is_k = !is_v && h >= p.nq;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    int64_t pos = 0, slot = 0;
+    if (live) {
+      w = ldg_stream(p.qkv + row * p.row_stride + h * D + 8 * sub);
+      if (!is_v) pos = p.positions[row];
+      if (is_k || is_v) slot = p.slots[row];
+    }
+    const bool pos_ok = pos >= 0 && pos < p.max_pos;
+    float x[8], y[8];
+    unpack8(w, x);
+    const uint16_t* gamma = is_k ? p.kg : p.qg;
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) ss = __fmaf_rn(x[j], x[j], ss);
+#pragma unroll
+    for (int o = L / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (gamma && !is_v) {
+      const float inv = rsqrtf(ss * (1.0f / D) + p.eps);
+      float g[8];
+      unpack8(*reinterpret_cast<const uint4*>(gamma + 8 * sub), g);
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = x[j] * inv * g[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) y[j] = __shfl_sync(0xffffffffu, x[j], src);
+    if (!is_v) {
+      if (sub < 2 * hl && pos_ok) {
+        const uint16_t* cs = p.cos_sin + pos * p.rot + 8 * (sub < hl ? sub : sub - hl);
+        float c[8], s[8];
+        unpack8(*reinterpret_cast<const uint4*>(cs), c);
+        unpack8(*reinterpret_cast<const uint4*>(cs + half), s);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = __fadd_rn(__fmul_rn(x[j], c[j]), __fmul_rn(sg * y[j], s[j]));
+      }
+      w = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+    }
+    if (!live) continue;
+    if (!pos_ok) {
+      if (sub == 0) atomicOr(p.error, kBadPosition);
+      continue;
+    }
+    if (!is_v && !is_k) {
+      *reinterpret_cast<uint4*>(p.q_out + (row * p.nq + h) * D + 8 * sub) = w;
+      continue;
+    }
+    if (slot < 0) continue;  // padding
+    if (slot >= p.num_slots) {
+      if (sub == 0) atomicOr(p.error, kBadSlot);
+      continue;
+    }
+    const int kh = h - p.nq - (is_v ? p.nkv : 0);
+    const int64_t blk = slot / p.bs, off = slot - blk * p.bs;
+    uint16_t* dst = (is_v ? p.v_cache : p.k_cache) + ((blk * p.nkv + kh) * p.bs + off) * D + 8 * sub;
+    *reinterpret_cast<uint4*>(dst) = w;
+  }
+}
+
+// ------------------------------------------------------------------ attention work list
+// The attention kernel walks items: a tile of consecutive query tokens of one request (the
+// rows of a tile are its tokens x the g query heads of a kv head) against a run of 128-key
+// tiles.  The list is per kv head (item i stands for nkv of them).  A tile whose run is
+// long against the even share of all work is cut into parts, whose unnormalised sums go to
+// the partial buffers and are joined by combine_kernel.
+constexpr int kKeyTile = 128;
+constexpr int kPromptPlan = 1, kPrefixPlan = 2;
+
+struct Item {
+  int tok0, ntok;   // query tokens
+  int pos0;         // position of the first one (kFlagLens: unused)
+  int req;          // block table row
+  int key0, nkt;    // first key (a multiple of kKeyTile), key tiles
+  int klo, khi;     // keys of the part: [klo, khi)
+  int len;          // keys the request holds: rows of its pages at or past it are stale
+  int flags;
+  int part;         // first partial row, or -1: the part is the whole tile
+  int pad;
+};
+constexpr int kFlagFew = 1;   // the tokens fit half a tile: the two halves take alternate key tiles
+constexpr int kFlagLens = 2;  // row limits are the requests' lengths (shared prefix), not causal
+static_assert(sizeof(Item) == 48, "items are three 16-byte words");
+
+struct Entry {  // rows to join: tokens tok0 .. tok0 + ntok - 1, part i of a list at base + i * stride
+  int tok0, ntok, base_a, n_a, stride_a, base_b, n_b, stride_b;
+};
+
+struct Header {
+  int items, entries, kind, part_rows, reqs, tokens, window, pad[9];
+};
+
+struct Layout {
+  int tile_tok, half_tok, max_tiles, max_items, max_entries, budget, part_rows;
+  int64_t items, entries, starts, tiles, bases, lens, bytes;
+};
+
+// Sizes of a plan for up to T tokens and R requests.  `budget` bounds the parts beyond one
+// per tile (4 per SM over the kv heads), so that partial rows stay bounded.
+__host__ __device__ inline Layout layout_of(int T, int R, int nq, int nkv, int D) {
+  Layout l;
+  const int g = nq / nkv;
+  l.half_tok = 128 / g;
+  l.tile_tok = D == 128 ? 2 * l.half_tok : l.half_tok;
+  const int tk = T > R ? T : R;
+  l.max_tiles = tk / l.tile_tok + R + 1;
+  l.budget = 4 * kNumSMs / nkv + 1;
+  l.max_items = l.max_tiles + l.budget;
+  l.max_entries = R > l.budget ? R : l.budget;
+  const int64_t rows = l.tile_tok < tk ? l.tile_tok : tk;
+  l.part_rows = (int)((2 * (int64_t)l.budget * rows + 2 * (int64_t)R) * g);
+  int64_t at = 0;  // every array starts on a 16-byte boundary
+  auto take = [&at](int64_t bytes) {
+    const int64_t o = at;
+    at += (bytes + 15) / 16 * 16;
+    return o;
+  };
+  take(sizeof(Header));
+  l.items = take((int64_t)l.max_items * sizeof(Item));
+  l.entries = take((int64_t)l.max_entries * sizeof(Entry));
+  l.starts = take(((int64_t)R + 1) * sizeof(int));
+  l.tiles = take((int64_t)l.max_tiles * sizeof(int2));
+  l.bases = take((int64_t)l.max_tiles * sizeof(int2));
+  l.lens = take(((int64_t)R + 1) * sizeof(int));
+  l.bytes = at;
+  return l;
+}
+
+struct AttnPlanArgs {
+  const int32_t *query_start, *seq_lens, *prefix_len;  // prefix_len: the shared-prefix plan
+  int reqs, tokens, nq, nkv, D, window;
+  Layout lay;
+  unsigned char* plan;
+  int* error;
+};
+
+constexpr int kAttnPlanThreads = 1024;
+constexpr int kBins = 1024;
+
+// Tile i of the batch: everything but how it is cut.
+struct Tile {
+  int tok0, ntok, pos0, req, key0, nkt, klo, khi, len, flags;
+};
+
+__device__ __forceinline__ Tile prompt_tile(const AttnPlanArgs& p, int q0, int n, int len, int r, int k) {
+  Tile t;
+  const int off = k * p.lay.tile_tok;
+  t.tok0 = q0 + off;
+  t.ntok = n - off < p.lay.tile_tok ? n - off : p.lay.tile_tok;
+  t.pos0 = len - n + off;  // (negative when the request has more queries than keys)
+  t.req = r;
+  t.len = len;
+  const int last = t.pos0 + t.ntok;  // exclusive causal limit of the last row
+  t.khi = last < 0 ? 0 : last;
+  const int lo = p.window > 0 ? t.pos0 + 1 - p.window : 0;
+  t.klo = lo < 0 ? 0 : lo;
+  t.key0 = t.klo / kKeyTile * kKeyTile;
+  t.nkt = t.khi > t.klo ? (t.khi - t.key0 + kKeyTile - 1) / kKeyTile : 0;
+  t.flags = p.D == 128 && t.ntok <= p.lay.half_tok ? kFlagFew : 0;
+  return t;
+}
+
+__device__ __forceinline__ Tile prefix_tile(const AttnPlanArgs& p, const int* lens, int prefix, int npre, int i) {
+  Tile t;
+  t.pos0 = 0;
+  t.flags = kFlagLens;
+  if (i < npre) {  // a tile of requests against the prefix, through the first request's table
+    t.tok0 = i * p.lay.tile_tok;
+    t.ntok = p.reqs - t.tok0 < p.lay.tile_tok ? p.reqs - t.tok0 : p.lay.tile_tok;
+    t.req = 0;
+    t.klo = 0;
+    t.khi = t.len = prefix;
+  } else {  // one request's own keys
+    t.tok0 = t.req = i - npre;
+    t.ntok = 1;
+    t.klo = prefix;
+    t.khi = t.len = lens[t.req];
+  }
+  t.key0 = t.klo / kKeyTile * kKeyTile;
+  t.nkt = t.khi > t.klo ? (t.khi - t.key0 + kKeyTile - 1) / kKeyTile : 0;
+  if (p.D == 128 && t.ntok <= p.lay.half_tok) t.flags |= kFlagFew;
+  return t;
+}
+
+__device__ __forceinline__ int block_sum(int v, int* ws) {
+  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int s = 0;
+  for (int w = 0; w < kAttnPlanThreads / 32; w++) s += ws[w];
+  return s;
+}
+
+__global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArgs p) {
+  __shared__ long long ws2[kAttnPlanThreads / 32][2];
+  __shared__ int ws[kAttnPlanThreads / 32];
+  __shared__ int hist[kBins];
+  __shared__ int entries_s, rows_s, bad_s;
+  const int tid = threadIdx.x, R = p.reqs;
+  Header* hdr = reinterpret_cast<Header*>(p.plan);
+  Item* items = reinterpret_cast<Item*>(p.plan + p.lay.items);
+  Entry* entries = reinterpret_cast<Entry*>(p.plan + p.lay.entries);
+  int* starts = reinterpret_cast<int*>(p.plan + p.lay.starts);  // first tile of request r
+  int2* tiles = reinterpret_cast<int2*>(p.plan + p.lay.tiles);  // (request, tile of the request)
+  int2* bases = reinterpret_cast<int2*>(p.plan + p.lay.bases);  // (first partial row, parts)
+  int* lens = reinterpret_cast<int*>(p.plan + p.lay.lens);
+  pdl_wait();
+  if (tid == 0) entries_s = rows_s = bad_s = 0;
+  __syncthreads();
+  const bool prefix_kind = p.prefix_len != nullptr;
+  int prefix = 0, npre = 0, nt = 0;
+  // tiles per request
+  if (prefix_kind) {
+    prefix = p.prefix_len[0];
+    if (prefix < 0) {
+      prefix = 0;
+      if (tid == 0) bad_s = kBadLength;
+    }
+    for (int r = tid; r < R; r += kAttnPlanThreads) {
+      const int n = p.seq_lens[r];
+      if (n < 0) atomicOr(&bad_s, kBadLength);
+      lens[r] = n < 0 ? 0 : n;
+    }
+    npre = (R + p.lay.tile_tok - 1) / p.lay.tile_tok;
+    nt = npre + R;
+  } else {
+    long long sum = 0;
+    for (int r0 = 0; r0 < R; r0 += kAttnPlanThreads) {
+      const int r = r0 + tid;
+      long long n = 0, dummy = 0, tot[2];
+      if (r < R) {
+        const int q0 = p.query_start[r], q1 = p.query_start[r + 1], len = p.seq_lens[r];
+        const bool ok = q0 >= 0 && q1 >= q0 && q1 <= p.tokens && len >= 0;
+        if (!ok) atomicOr(&bad_s, kBadLength);
+        lens[r] = len < 0 ? 0 : len;
+        n = ok ? (q1 - q0 + p.lay.tile_tok - 1) / p.lay.tile_tok : 0;
+      }
+      long long a = n;
+      block_scan2(a, dummy, tot, ws2);
+      // (overlapping starts could list more tokens than there are: the excess is cut)
+      if (r < R) {
+        const long long s = sum + a - n;
+        starts[r] = (int)(s < p.lay.max_tiles ? s : p.lay.max_tiles);
+      }
+      sum += tot[0];
+    }
+    if (sum > p.lay.max_tiles) {
+      sum = p.lay.max_tiles;
+      if (tid == 0) atomicOr(&bad_s, kBadLength);
+    }
+    nt = (int)sum;
+  }
+  __syncthreads();
+  auto tile_at = [&](int i) {
+    if (prefix_kind) return prefix_tile(p, lens, prefix, npre, i);
+    const int2 t = tiles[i];
+    const int q0 = p.query_start[t.x];
+    return prompt_tile(p, q0, p.query_start[t.x + 1] - q0, lens[t.x], t.x, t.y);
+  };
+  int work = 0;
+  for (int i = tid; i < nt; i += kAttnPlanThreads) {
+    if (!prefix_kind) {
+      const int r = find_request(starts, R, i);
+      tiles[i] = make_int2(r, i - starts[r]);
+    }
+    work += tile_at(i).nkt;
+  }
+  const int total = block_sum(work, ws);
+  // keys a part may have: an even share of the work, or more until the parts fit the buffers
+  const long long share = ((long long)total * p.nkv + kNumSMs - 1) / kNumSMs;
+  int cut = share < 1 ? 1 : (int)share;
+  for (;;) {
+    int extra = 0, rows = 0;
+    for (int i = tid; i < nt; i += kAttnPlanThreads) {
+      const Tile t = tile_at(i);
+      const int np = (t.nkt + cut - 1) / cut;
+      if (np > 1) extra += np - 1;
+      if (np > 1 || prefix_kind) rows += np * t.ntok;
+    }
+    const int e = block_sum(extra, ws), rw = block_sum(rows, ws);
+    if ((e <= p.lay.budget && (long long)rw * (p.nq / p.nkv) <= p.lay.part_rows) || cut >= total) break;
+    cut = cut + (cut + 1) / 2;
+  }
+  // longest parts first (a counting sort by length; the order inside a length does not
+  // matter to any result)
+  for (int b = tid; b < kBins; b += kAttnPlanThreads) hist[b] = 0;
+  __syncthreads();
+  auto bin_of = [&](const Tile& t, int keys) {
+    const int c = (t.flags & kFlagFew) ? (keys + 1) / 2 : keys;
+    return kBins - 1 - (c < kBins - 1 ? c : kBins - 1);
+  };
+  for (int pass = 0; pass < 2; pass++) {
+    for (int i = tid; i < nt; i += kAttnPlanThreads) {
+      const Tile t = tile_at(i);
+      int np = (t.nkt + cut - 1) / cut;
+      if (np == 0 && !prefix_kind) np = 1;  // rows without keys are written as zeros
+      const bool parts = np > 1 || prefix_kind;
+      int base = -1;
+      if (pass == 1) {
+        const int g = p.nq / p.nkv;
+        if (parts) base = atomicAdd(&rows_s, np * t.ntok * g);
+        bases[i] = make_int2(base, np);
+        if (parts && !prefix_kind) {
+          const int e = atomicAdd(&entries_s, 1);
+          entries[e] = {t.tok0, t.ntok, base, np, t.ntok * g, 0, 0, 0};
+        }
+      }
+      for (int k = 0; k < np; k++) {
+        const int a = (int)((long long)k * t.nkt / np), b = (int)((long long)(k + 1) * t.nkt / np);
+        const int slot = atomicAdd(&hist[bin_of(t, b - a)], 1);
+        if (pass == 1) {
+          Item it;
+          it.tok0 = t.tok0, it.ntok = t.ntok, it.pos0 = t.pos0, it.req = t.req;
+          it.key0 = t.key0 + a * kKeyTile;
+          it.nkt = b - a;
+          it.klo = a ? it.key0 : t.klo;
+          it.khi = k + 1 < np ? t.key0 + b * kKeyTile : t.khi;
+          it.len = t.len, it.flags = t.flags;
+          it.part = parts ? base + k * t.ntok * (p.nq / p.nkv) : -1;
+          it.pad = 0;
+          items[slot] = it;
+        }
+      }
+    }
+    __syncthreads();
+    if (pass == 0) {  // counts -> first slot of each bin
+      long long a = tid < kBins ? hist[tid] : 0, n = a, dummy = 0, tot[2];
+      block_scan2(a, dummy, tot, ws2);
+      if (tid < kBins) hist[tid] = (int)(a - n);
+      if (tid == 0) hdr->items = (int)tot[0];
+      __syncthreads();
+    }
+  }
+  if (prefix_kind) {
+    const int g = p.nq / p.nkv;
+    for (int r = tid; r < R; r += kAttnPlanThreads) {
+      const int i = r / p.lay.tile_tok;
+      const Tile t = prefix_tile(p, lens, prefix, npre, i);
+      const int2 a = bases[i], b = bases[npre + r];
+      entries[r] = {r, 1, a.x + (r - t.tok0) * g, a.y, t.ntok * g, b.x, b.y, g};
+    }
+  }
+  if (tid == 0) {
+    hdr->entries = prefix_kind ? R : entries_s;
+    hdr->kind = prefix_kind ? kPrefixPlan : kPromptPlan;
+    hdr->part_rows = rows_s;
+    hdr->reqs = R;
+    hdr->tokens = p.tokens;
+    hdr->window = p.window;
+    if (bad_s) atomicOr(p.error, bad_s);
+  }
+}
+
+// ------------------------------------------------------------------ attention
+struct AttnArgs {
+  const uint16_t *q, *k_cache, *v_cache;
+  int64_t q_tok, q_head, o_tok, o_head;  // strides in elements
+  const int32_t* table;
+  int64_t table_stride, num_blocks;
+  int table_width, bs, tokens, nq, nkv, window;
+  float scale;
+  const unsigned char* plan;
+  Layout lay;
+  float* part_o;    // [part rows][nkv][D] unnormalised sums
+  float2* part_ml;  // [part rows][nkv]: (running maximum of scale * s * log2 e, sum)
+  uint16_t* out;
+  int* error;
+};
+
+// keys row (token i of the item) may see, within the item's part
+__device__ __forceinline__ int2 row_keys(const Item& it, const int* lens, int window, int i) {
+  int lo = it.klo, hi = it.khi;
+  if (it.flags & kFlagLens) {
+    const int n = lens[it.tok0 + i];
+    hi = n < hi ? n : hi;
+  } else {
+    const int pos = it.pos0 + i;
+    hi = pos + 1 < hi ? pos + 1 : hi;
+    if (window > 0 && pos + 1 - window > lo) lo = pos + 1 - window;
+  }
+  return make_int2(lo, hi);
+}
+
+// The plain form of the attention: one warp per query row, a lane holding D / 32 elements,
+// keys one after the other with the running maximum and sum in fp32.
+template <int D>
+__global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs p) {
+  constexpr int E = D / 32;
+  pdl_wait();
+  const Header* hdr = reinterpret_cast<const Header*>(p.plan);
+  const Item* items = reinterpret_cast<const Item*>(p.plan + p.lay.items);
+  const int* lens = reinterpret_cast<const int*>(p.plan + p.lay.lens);
+  const int g = p.nq / p.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float c = p.scale * kLog2e;
+  const int64_t n = (int64_t)hdr->items * p.nkv;
+  for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
+    const Item it = items[w / p.nkv];
+    const int kvh = (int)(w % p.nkv);
+    for (int row = warp; row < it.ntok * g; row += 8) {
+      const int i = row / g, tok = it.tok0 + i, head = kvh * g + row % g;
+      if (tok >= p.tokens) continue;
+      float q[E], o[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        q[e] = bf2f(p.q[tok * p.q_tok + head * p.q_head + lane * E + e]);
+        o[e] = 0.0f;
+      }
+      float m = -INFINITY, l = 0.0f;
+      const int2 kk = row_keys(it, lens, p.window, i);
+      for (int key = kk.x; key < kk.y; key++) {
+        const int pg = key / p.bs;
+        const int id = pg < p.table_width ? p.table[it.req * p.table_stride + pg] : -1;
+        if (id < 0 || id >= p.num_blocks) {
+          if (lane == 0) atomicOr(p.error, kBadPage);
+          continue;
+        }
+        const int64_t base = (((int64_t)id * p.nkv + kvh) * p.bs + key % p.bs) * D + lane * E;
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++) s = __fmaf_rn(q[e], bf2f(p.k_cache[base + e]), s);
+        s = butterfly_sum<32>(s) * c;
+        const float mn = fmaxf(m, s);
+        const float a = exp2f(m - mn), x = exp2f(s - mn);
+        m = mn;
+        l = l * a + x;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = __fmaf_rn(x, bf2f(p.v_cache[base + e]), o[e] * a);
+      }
+      if (it.part < 0) {
+        const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
+#pragma unroll
+        for (int e = 0; e < E; e++) p.out[tok * p.o_tok + head * p.o_head + lane * E + e] = f2bf(o[e] * inv);
+      } else {
+        const int64_t pr = (int64_t)(it.part + row) * p.nkv + kvh;
+#pragma unroll
+        for (int e = 0; e < E; e++) p.part_o[pr * D + lane * E + e] = o[e];
+        if (lane == 0) p.part_ml[pr] = make_float2(m, l);
+      }
+    }
+  }
+}
+
+// Join of the parts of cut tiles: with M = max m_i over a row's parts,
+//   out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i,
+// the parts in list order whatever order they were computed in.  A row without any key is
+// zero.  One warp per row.
+template <int D>
+__global__ void __launch_bounds__(256) combine_kernel(AttnArgs p) {
+  constexpr int E = D / 32;
+  pdl_wait();
+  const Header* hdr = reinterpret_cast<const Header*>(p.plan);
+  const Entry* entries = reinterpret_cast<const Entry*>(p.plan + p.lay.entries);
+  const int g = p.nq / p.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = hdr->entries;
+  for (int64_t w = blockIdx.x; w < (int64_t)n * p.nkv; w += gridDim.x) {
+    const Entry en = entries[w / p.nkv];
+    const int kvh = (int)(w % p.nkv);
+    for (int row = warp; row < en.ntok * g; row += 8) {
+      const int tok = en.tok0 + row / g, head = kvh * g + row % g;
+      if (tok >= p.tokens) continue;
+      float M = -INFINITY, l = 0.0f, o[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) o[e] = 0.0f;
+      const int parts = en.n_a + en.n_b;
+      for (int k = 0; k < parts; k++) {
+        const int64_t r = k < en.n_a ? en.base_a + (int64_t)k * en.stride_a
+                                     : en.base_b + (int64_t)(k - en.n_a) * en.stride_b;
+        const int64_t pr = (r + row) * p.nkv + kvh;
+        const float2 ml = p.part_ml[pr];
+        if (ml.y == 0.0f) continue;  // no key in this part (its sums are not written)
+        const float mn = fmaxf(M, ml.x);
+        const float a = exp2f(M - mn), b = exp2f(ml.x - mn);
+        M = mn;
+        l = l * a + ml.y * b;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = o[e] * a + p.part_o[pr * D + lane * E + e] * b;
+      }
+      const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
+#pragma unroll
+      for (int e = 0; e < E; e++) p.out[tok * p.o_tok + head * p.o_head + lane * E + e] = f2bf(o[e] * inv);
+    }
+  }
+}
+
+}  // namespace paged
+}  // namespace spark

@@ -45,6 +45,14 @@ SIGNATURES: dict[str, list] = {
     "spark_set_gemv_ring": [_I],
     "spark_read_device_error": [_P, _I],
     "spark_kv_store": [_P, _P, _P, _I64, _I, _I, _I, _P, _P, _P],
+    "spark_paged_plan": [_P, _P, _I, _P, _I, _P, _P, _P, _I64, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P],
+    "spark_qk_norm_rope_store_rows": [_P, _I64, _I, _I, _I, _I, _P, _P, _F, _P, _I64, _I, _P, _P, _I, _I64, _P, _P,
+                                      _P, _P, _P],
+    "spark_attn_plan_bytes": [_I, _I, _I, _I, _I],
+    "spark_attn_part_rows": [_I, _I, _I, _I, _I],
+    "spark_attn_plan": [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P],
+    "spark_attn_paged": [_P, _I64, _I64, _I, _P, _P, _I64, _I, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P,
+                         _P, _I64, _I64, _P, _I64, _P],
     "spark_t16_bytes": [_I, _I, _I],
     "spark_q4_pack_t16": [_P, _P, _I, _I, _I, _I, _I, _P, _P],
     "spark_step_ring_bytes": [],
@@ -61,7 +69,8 @@ SIGNATURES: dict[str, list] = {
     "spark_ipc_close": [_P],
 }
 # entry points whose return value is a quantity, not a status
-RESTYPES = {"spark_t16_bytes": _I64, "spark_t6_bytes": _I64}
+RESTYPES = {"spark_t16_bytes": _I64, "spark_t6_bytes": _I64, "spark_attn_plan_bytes": _I64,
+            "spark_attn_part_rows": _I64}
 
 
 class SparkStage(ctypes.Structure):

@@ -20,7 +20,7 @@ import ctypes
 
 import torch
 
-from ._lib import call
+from ._lib import call, lib
 
 BF16 = torch.bfloat16
 
@@ -295,6 +295,219 @@ def kv_store_(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
          k_cache.shape[2], _p(k_cache), _p(v_cache), _stream())
 
 
+# ---------------------------------------------------------------- batches over the paged cache
+# error-word bits of these operators (include/spark_b200.h)
+ERR_WAIT, ERR_LENGTH, ERR_NO_PAGES, ERR_TABLE_WIDTH, ERR_NO_ROWS = 1, 4, 8, 16, 32
+ERR_PAGE, ERR_POSITION, ERR_SLOT = 64, 128, 256
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """Launch on the tensors' own device, on its current stream."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, _stream())
+        return
+    with torch.cuda.device(device):
+        call(name, *args, _stream())
+
+
+def _same_device(device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None:
+            _check(t.device == device, f"{name} must be on {device}, got {t.device}")
+
+
+def _error_word(error: torch.Tensor) -> None:
+    _cuda(error, "error", torch.int32)
+    _check(error.numel() >= 1, "error must hold one int32")
+
+
+def _block_table(block_table: torch.Tensor, reqs: int) -> None:
+    _check(block_table.is_cuda and block_table.dtype == torch.int32, "block_table must be a CUDA int32 tensor")
+    _check(block_table.dim() == 2 and block_table.stride(1) == 1, "block_table must be [requests, pages], rows dense")
+    _check(block_table.shape[0] >= reqs and block_table.shape[1] >= 1,
+           f"block_table must have {reqs} rows, got {tuple(block_table.shape)}")
+
+
+def paged_plan_out(ctx_lens, new_lens, block_table, block_size, query_start, seq_lens, positions, slot_mapping,
+                   counter, error, free_blocks=None, free_head=None, free_head_out=None):
+    """Block tables, token positions and slot maps of a batch from its request lengths, in
+    one launch on the device.  ``ctx_lens`` / ``new_lens`` int32 [R]: cached and new tokens;
+    writes ``query_start`` int32 [R + 1], ``seq_lens`` int32 [R], ``positions`` and
+    ``slot_mapping`` int64 [rows] (rows behind the last token: 0 and -1) and, given
+    ``free_blocks`` (int32 [F]) with ``free_head`` (int32 [1], ids taken so far), the new
+    pages' ids into ``block_table`` and the advanced head into ``free_head_out`` (default:
+    ``free_head`` itself).  All or nothing: a batch that does not fit comes out empty, with
+    the reason in ``error`` (ERR_* bits).  ``counter`` int32 [1], zero."""
+    R = ctx_lens.numel()
+    for t, nm in ((ctx_lens, "ctx_lens"), (new_lens, "new_lens"), (query_start, "query_start"),
+                  (seq_lens, "seq_lens"), (counter, "counter")):
+        _cuda(t, nm, torch.int32)
+    for t, nm in ((positions, "positions"), (slot_mapping, "slot_mapping")):
+        _cuda(t, nm, torch.int64)
+    _error_word(error)
+    _check(R >= 1 and new_lens.numel() == R and seq_lens.numel() == R and query_start.numel() == R + 1,
+           "ctx_lens, new_lens, seq_lens hold one entry per request, query_start one more")
+    _check(positions.numel() == slot_mapping.numel(), "positions and slot_mapping must have the same length")
+    _check(counter.numel() >= 1, "counter must hold one int32")
+    _check(block_size >= 1, "block_size must be positive")
+    _block_table(block_table, R)
+    _check((free_blocks is None) == (free_head is None), "give free_blocks and free_head together")
+    _check(free_head_out is None or free_head is not None, "free_head_out needs free_head")
+    if free_blocks is not None:
+        free_head_out = free_head if free_head_out is None else free_head_out
+        for t, nm in ((free_blocks, "free_blocks"), (free_head, "free_head"), (free_head_out, "free_head_out")):
+            _cuda(t, nm, torch.int32)
+            _check(nm == "free_blocks" or t.numel() == 1, f"{nm} must hold one int32")
+    dev = ctx_lens.device
+    _same_device(dev, new_lens=new_lens, block_table=block_table, query_start=query_start, seq_lens=seq_lens,
+                 positions=positions, slot_mapping=slot_mapping, counter=counter, error=error,
+                 free_blocks=free_blocks, free_head=free_head, free_head_out=free_head_out)
+    _call_on(dev, "spark_paged_plan", _p(ctx_lens), _p(new_lens), R, _p(free_blocks),
+             0 if free_blocks is None else free_blocks.numel(), _p(free_head), _p(free_head_out), _p(block_table),
+             block_table.stride(0) if R > 1 else block_table.shape[1], block_table.shape[1], int(block_size),
+             positions.numel(), _p(query_start), _p(seq_lens), _p(positions), _p(slot_mapping), _p(counter),
+             _p(error))
+
+
+def qk_norm_rope_store_rows(qkv, nq, nkv, head_dim, q_gamma, k_gamma, eps, cos_sin, positions, slot_mapping, k_cache,
+                            v_cache, q_out, error):
+    """Rows of a fused qkv output (bf16 [rows, >= (nq + 2 nkv) * head_dim], rows dense) in one
+    pass: per-head RMS norm of q and k (``q_gamma`` / ``k_gamma`` bf16 [head_dim], or both
+    None), rotation at ``positions`` (int64 [rows]) by ``cos_sin`` bf16 [max_pos,
+    rotary_dim], q to ``q_out`` bf16 [rows, nq, head_dim] and k, v to the paged caches at
+    ``slot_mapping`` (int64 [rows], negative: not stored).  fp32 inside, one rounding."""
+    _check(qkv.is_cuda and qkv.dtype == BF16, "qkv must be a CUDA bfloat16 tensor")
+    _check(qkv.dim() == 2 and (qkv.stride(1) == 1 or qkv.shape[1] == 1), "qkv must be [rows, cols], rows dense")
+    rows = qkv.shape[0]
+    _check(qkv.shape[1] >= (nq + 2 * nkv) * head_dim, "qkv rows must hold (nq + 2 nkv) * head_dim columns")
+    for t, nm in ((cos_sin, "cos_sin"), (k_cache, "k_cache"), (v_cache, "v_cache"), (q_out, "q_out")):
+        _cuda(t, nm, BF16)
+    for t, nm in ((positions, "positions"), (slot_mapping, "slot_mapping")):
+        _cuda(t, nm, torch.int64)
+        _check(t.numel() >= rows, f"{nm} must hold one entry per row")
+    _error_word(error)
+    _check((q_gamma is None) == (k_gamma is None), "give q_gamma and k_gamma together")
+    if q_gamma is not None:
+        for t, nm in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
+            _cuda(t, nm, BF16)
+            _check(t.numel() == head_dim, f"{nm} must hold head_dim values")
+    _check(cos_sin.dim() == 2, "cos_sin must be [max_pos, rotary_dim]")
+    _check(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[1] == nkv and
+           k_cache.shape[3] == head_dim, "caches must be [blocks, nkv, block_size, head_dim]")
+    _check(q_out.numel() == rows * nq * head_dim, "q_out must be [rows, nq, head_dim]")
+    _same_device(qkv.device, q_gamma=q_gamma, k_gamma=k_gamma, cos_sin=cos_sin, positions=positions,
+                 slot_mapping=slot_mapping, k_cache=k_cache, v_cache=v_cache, q_out=q_out, error=error)
+    _call_on(qkv.device, "spark_qk_norm_rope_store_rows", _p(qkv), qkv.stride(0) if rows > 1 else
+             (qkv.shape[1] + 7) // 8 * 8, rows, nq, nkv, head_dim, _p(q_gamma), _p(k_gamma), float(eps), _p(cos_sin),
+             cos_sin.shape[0], cos_sin.shape[1], _p(positions), _p(slot_mapping), k_cache.shape[2], k_cache.shape[0],
+             _p(k_cache), _p(v_cache), _p(q_out), _p(error))
+    return q_out
+
+
+class AttnPlan:
+    """Work list and workspace of the paged attention for one head layout and window.
+
+    ``update`` (packed prompts, chunks, single tokens) or ``update_prefix`` (one token per
+    request behind a common prefix) makes the list from device tensors, without a host
+    copy, once per step; every layer of that layout then uses it.  Both can be captured
+    into a CUDA graph.  Calls that may overlap on the device need a plan each: the plan and
+    the partial results are overwritten by the next one.  ``error`` int32 [1] collects what
+    ``update`` found (ERR_* bits)."""
+
+    def __init__(self, max_tokens: int, max_reqs: int, nq: int, nkv: int, head_dim: int, device="cuda",
+                 window: int = 0):
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        _check(device.type == "cuda", "the plan lives on a CUDA device")
+        _check(window >= 0, "window must be positive, or 0 for none")
+        nbytes = lib().spark_attn_plan_bytes(max_tokens, max_reqs, nq, nkv, head_dim)
+        _check(nbytes > 0, f"unsupported attention shape: {max_tokens} tokens, {max_reqs} requests, {nq} query / "
+                           f"{nkv} kv heads of {head_dim}")
+        rows = lib().spark_attn_part_rows(max_tokens, max_reqs, nq, nkv, head_dim)
+        self.max_tokens, self.max_reqs, self.window = int(max_tokens), int(max_reqs), int(window)
+        self.nq, self.nkv, self.head_dim, self.device = nq, nkv, head_dim, device
+        self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        self.part_o = torch.empty((rows, nkv, head_dim), dtype=torch.float32, device=device)
+        self.part_ml = torch.empty((rows, nkv, 2), dtype=torch.float32, device=device)
+        self.error = torch.zeros(1, dtype=torch.int32, device=device)
+        self.kind, self.reqs = None, 0
+
+    def _make(self, kind, reqs, query_start, seq_lens, prefix_len):
+        _check(reqs <= self.max_reqs, f"{reqs} requests in a plan for {self.max_reqs}")
+        _same_device(self.device, query_start=query_start, seq_lens=seq_lens, prefix_len=prefix_len)
+        _call_on(self.device, "spark_attn_plan", _p(query_start), _p(seq_lens), _p(prefix_len), reqs,
+                 self.max_tokens, self.max_reqs, self.nq, self.nkv, self.head_dim, self.window, _p(self.buf),
+                 _p(self.error))
+        self.kind, self.reqs = kind, reqs
+        return self
+
+    def update(self, query_start: torch.Tensor, seq_lens: torch.Tensor) -> "AttnPlan":
+        """A packed batch: request r's query tokens are rows query_start[r] ..
+        query_start[r + 1] - 1 (int32 [R + 1]), the last of its seq_lens[r] (int32 [R]) keys."""
+        _cuda(query_start, "query_start", torch.int32)
+        _cuda(seq_lens, "seq_lens", torch.int32)
+        reqs = seq_lens.numel()
+        _check(reqs >= 1 and query_start.numel() == reqs + 1, "query_start must have one entry more than seq_lens")
+        return self._make("prompt", reqs, query_start, seq_lens, None)
+
+    def update_prefix(self, seq_lens: torch.Tensor, prefix_len: torch.Tensor) -> "AttnPlan":
+        """One query token per request, seq_lens[r] (int32 [R]) keys each, the first
+        prefix_len (int32 [1]) of them the same for all."""
+        _cuda(seq_lens, "seq_lens", torch.int32)
+        _cuda(prefix_len, "prefix_len", torch.int32)
+        _check(self.window == 0, "a shared prefix is read without a window")
+        _check(prefix_len.numel() == 1, "prefix_len must hold one int32")
+        reqs = seq_lens.numel()
+        _check(1 <= reqs <= self.max_tokens, f"{reqs} requests in a plan for {self.max_tokens} tokens")
+        return self._make("prefix", reqs, None, seq_lens, prefix_len)
+
+
+def _attn_paged(kind, q, k_cache, v_cache, block_table, plan, scale, out, error, wait_ns):
+    _check(plan.kind == kind, f"the plan was made for {plan.kind!r}, not {kind!r}")
+    nq, nkv, D = plan.nq, plan.nkv, plan.head_dim
+    for t, nm in ((q, "q"), (out, "out")):
+        _check(t.is_cuda and t.dtype == BF16, f"{nm} must be a CUDA bfloat16 tensor")
+        _check(t.dim() == 3 and t.shape[1] == nq and t.shape[2] == D and (t.stride(2) == 1 or t.numel() == 0),
+               f"{nm} must be [tokens, {nq}, {D}], heads dense")
+    tokens = q.shape[0]
+    _check(out.shape[0] >= tokens, "out must have a row per token")
+    _check(tokens <= plan.max_tokens, f"{tokens} tokens in a plan for {plan.max_tokens}")
+    _cuda(k_cache, "k_cache", BF16)
+    _cuda(v_cache, "v_cache", BF16)
+    _check(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[1] == nkv and
+           k_cache.shape[3] == D, f"caches must be [blocks, {nkv}, block_size, {D}]")
+    _block_table(block_table, plan.reqs)
+    _error_word(error)
+    _same_device(plan.device, q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, out=out, error=error)
+    _call_on(plan.device, "spark_attn_paged", _p(q), q.stride(0), q.stride(1), tokens, _p(k_cache), _p(v_cache),
+             k_cache.shape[0], k_cache.shape[2], _p(block_table), block_table.stride(0), block_table.shape[1],
+             plan.max_tokens, plan.max_reqs, nq, nkv, D, plan.window, float(scale), _p(plan.buf), _p(plan.part_o),
+             _p(plan.part_ml), _p(out), out.stride(0), out.stride(1), _p(error), int(wait_ns))
+    return out
+
+
+def attn_prompt_out(q, k_cache, v_cache, block_table, plan: AttnPlan, scale, out, error, wait_ns: int = -1):
+    """Causal attention of a packed batch over the paged caches (``plan.update`` made this
+    step's list): q / out bf16 [tokens, nq, D] (any token and head strides that are
+    multiples of 8), caches bf16 [blocks, nkv, block_size, D], block_table int32 [R, pages].
+    Whole prompts, chunks on top of cached context and single tokens alike; tokens without
+    keys give zero, rows of ``out`` behind the last planned token are left as they were.
+    Keys and values at positions a request does hold must be finite; what its pages carry
+    past its length does not matter.  ``error`` (int32 [1], required): nonzero, out is not
+    valid (ERR_* bits)."""
+    return _attn_paged("prompt", q, k_cache, v_cache, block_table, plan, scale, out, error, wait_ns)
+
+
+def attn_shared_prefix_out(q, k_cache, v_cache, block_table, plan: AttnPlan, scale, out, error, wait_ns: int = -1):
+    """Attention of one query token per request (q / out bf16 [R, nq, D]) where all requests
+    share their first positions (``plan.update_prefix``): the prefix's pages are read once
+    for the whole batch, through the first request's table, each request's own keys through
+    its own; the parts join by log-sum-exp.  Otherwise as ``attn_prompt_out``."""
+    _check(q.shape[0] >= plan.reqs, "q must have a row per request")
+    return _attn_paged("prefix", q, k_cache, v_cache, block_table, plan, scale, out, error, wait_ns)
+
+
 def set_pdl(enabled: bool) -> None:
     call("spark_set_pdl", 1 if enabled else 0)
 
@@ -412,6 +625,59 @@ def _op_silu_mul(gu: torch.Tensor) -> torch.Tensor:
 @_op_silu_mul.register_fake
 def _(gu):
     return gu.new_empty((*gu.shape[:-1], gu.shape[-1] // 2))
+
+
+@torch.library.custom_op("spark_b200::qk_norm_rope_store_rows", mutates_args=("k_cache", "v_cache", "error"))
+def _op_qk_rows(qkv: torch.Tensor, nq: int, nkv: int, head_dim: int, q_gamma: torch.Tensor | None,
+                k_gamma: torch.Tensor | None, eps: float, cos_sin: torch.Tensor, positions: torch.Tensor,
+                slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                error: torch.Tensor) -> torch.Tensor:
+    q = qkv.new_empty((qkv.shape[0], nq, head_dim))
+    return qk_norm_rope_store_rows(qkv, nq, nkv, head_dim, q_gamma, k_gamma, eps, cos_sin, positions, slot_mapping,
+                                   k_cache, v_cache, q, error)
+
+
+@_op_qk_rows.register_fake
+def _(qkv, nq, nkv, head_dim, q_gamma, k_gamma, eps, cos_sin, positions, slot_mapping, k_cache, v_cache, error):
+    return qkv.new_empty((qkv.shape[0], nq, head_dim))
+
+
+@torch.library.custom_op("spark_b200::attn_prompt", mutates_args=("error",))
+def _op_attn_prompt(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    query_start: torch.Tensor, seq_lens: torch.Tensor, scale: float, window: int,
+                    error: torch.Tensor) -> torch.Tensor:
+    out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    if q.shape[0] == 0:
+        return out
+    plan = AttnPlan(q.shape[0], seq_lens.numel(), q.shape[1], k_cache.shape[1], q.shape[2], q.device, window)
+    plan.update(query_start, seq_lens)
+    attn_prompt_out(q, k_cache, v_cache, block_table, plan, scale, out, error)
+    error.bitwise_or_(plan.error)
+    return out
+
+
+@_op_attn_prompt.register_fake
+def _(q, k_cache, v_cache, block_table, query_start, seq_lens, scale, window, error):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("spark_b200::attn_shared_prefix", mutates_args=("error",))
+def _op_attn_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    seq_lens: torch.Tensor, prefix_len: torch.Tensor, scale: float,
+                    error: torch.Tensor) -> torch.Tensor:
+    out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    if q.shape[0] == 0:
+        return out
+    plan = AttnPlan(q.shape[0], seq_lens.numel(), q.shape[1], k_cache.shape[1], q.shape[2], q.device)
+    plan.update_prefix(seq_lens, prefix_len)
+    attn_shared_prefix_out(q, k_cache, v_cache, block_table, plan, scale, out, error)
+    error.bitwise_or_(plan.error)
+    return out
+
+
+@_op_attn_prefix.register_fake
+def _(q, k_cache, v_cache, block_table, seq_lens, prefix_len, scale, error):
+    return q.new_empty(q.shape)
 
 
 def q6k_dequantize(blocks: torch.Tensor) -> torch.Tensor:
