@@ -1,0 +1,732 @@
+// attn_paged.cuh -- attention of a planned batch over the paged KV cache on the tensor cores.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = 2^(c (s_ij - m_i)),  s_ij = q_i . k_j,
+//   c = scale log2 e,
+// one pass over the keys: m_i is a running reference maximum and l_i = sum p_ij and the
+// unnormalised o_i follow it.  m_i is only moved when a score passes it by more than 8 / c
+// (probabilities then stay below 2^8), so the o accumulators are rescaled rarely instead
+// of at every tile; any reference gives the same quotient.  s, m, l and o are fp32; p is
+// rounded to bf16 as the matrix operand (v is bf16: both operands have one type), which is
+// the one rounding besides the output's.
+//
+// Persistent, warp-specialized, one CTA per SM; the CTA walks the plan's items (paged.cuh),
+// longest first, CTA order reversed every other pass so that loads even out.  A tile has
+// the query tokens' g heads as rows, so the K / V of a kv head are read once for the whole
+// group.  352 threads:
+//   warps 0-3, 4-7  softmax of accumulator halves 0 / 1, a thread owning one row: scores
+//                   from tensor memory, maximum, p to tensor memory (as the next product's
+//                   A operand) and the item's epilogue;
+//   warp 8          K / V producer: page ids of 32 pieces at a time, one TMA copy per page
+//                   piece and 64 columns into the ring, 128-byte swizzle;
+//   warp 9          owns the tensor memory; one lane issues all MMAs and commits;
+//   warp 10         Q of the next item, as soon as the last score product has read the
+//                   buffer.
+// Shared memory: Q 64 KB, a ring of five 32-KB chunks (128 keys x 128 columns of K or V).
+// Tensor memory: scores S0 S1 (128 columns each, p written over them), sums O0 O1.
+//
+// Three ways through one loop:
+//   head_dim 128, many rows: half h has its own 128 rows, S_h, O_h; every K / V chunk is
+//     used by both, and half 1's products run while half 0's softmax does;
+//   head_dim 128, few rows (up to 128: single tokens): both halves have the same rows and
+//     take alternate key tiles, each with its own m, l, O; they are merged through the Q
+//     buffer at the end;
+//   head_dim 256: 128 rows, S0 and S1 take alternate key tiles of one softmax, O0 O1 are
+//     the two column halves of one sum.
+// In all of them the scores of tile t + 1 (or + 2) are computed while the softmax of tile t
+// runs, and the issuing order makes every hazard on S, P and O an in-order one: the product
+// that overwrites S_h is issued after the one that reads P_h, and a commit that announces
+// S_h covers all earlier products, so the softmax may touch O_h as soon as it holds S_h
+// (head_dim 256: after a commit of its own).
+//
+// Stale memory: a K / V row at or past the request's length (or before the window) may hold
+// anything.  Scores are masked by selection, and V rows outside [klo, len) are zeroed in
+// shared memory before their product, since 0 * NaN is NaN.
+//
+// Every mbarrier wait is bounded by %globaltimer; one that runs out sets bit 1 of *error
+// and an abort flag that every other wait checks.  Before the CTA gives up shared or
+// tensor memory it waits (2 s bound) for the copies and MMAs in flight; bit 2 means that
+// this ran out too and the tensor memory was kept.
+#pragma once
+
+#include <cuda.h>
+
+#include <climits>
+
+#include "paged.cuh"
+
+namespace spark {
+namespace paged {
+namespace tc {
+
+constexpr int kThreads = 352;
+constexpr int kProducerWarp = 8, kMmaWarp = 9, kQWarp = 10;
+constexpr int kStages = 5;
+constexpr int kChunk = 32 * 1024;  // 128 keys x 128 columns
+constexpr int kSub = 16 * 1024;    // 128 keys x 64 columns (one swizzle row of 128 bytes)
+constexpr int kOffRing = 64 * 1024;
+constexpr int kOffMl = kOffRing + kStages * kChunk;  // few rows: (m, l) of half 1
+constexpr int kOffBar = kOffMl + 128 * 8;
+constexpr int kBarFull = 0, kBarEmpty = kBarFull + kStages, kBarQFull = kBarEmpty + kStages,
+              kBarQEmpty = kBarQFull + 1, kBarS = kBarQEmpty + 1, kBarP = kBarS + 2, kBarO = kBarP + 2,
+              kBarPV = kBarO + 2, kBarMerge = kBarPV + 2, kBarDrain = kBarMerge + 1, kNumBars = kBarDrain + 1;
+constexpr int kOffMisc = kOffBar + 8 * kNumBars;  // tensor-memory base, abort flag, drained flag
+constexpr int kSmemBytes = kOffMisc + 16 + 1024;  // + 1024-byte alignment slack
+constexpr int kTmemCols = 512;
+constexpr int kColS = 0, kColO = 256;
+constexpr unsigned long long kWaitNs = 500ull * 1000 * 1000;
+constexpr unsigned long long kDrainNs = 2000ull * 1000 * 1000;
+static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+
+// instruction descriptors (kind::f16): fp32 D, bf16 A and B, N = 128, M = 128; scores: both
+// operands K-major; sums: B (= V, keys x columns) N-major (bit 16)
+constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t kIdescO = kIdescS | (1u << 16);
+
+// 128-byte-swizzled operand tiles.  K-major (Q, K): 8-row groups 1024 bytes apart, 16
+// columns = 32 bytes along the row.  N-major (V): 64-column blocks kSub apart (leading
+// offset), 8-key groups 1024 bytes apart, 16 keys = 2048 bytes.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(kSub >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+
+// Wait for the phase of `parity`; false: limit_ns ran out or another role gave up.  The
+// clock and the flag are looked at every 16th try only.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, unsigned long long limit_ns,
+                                         const volatile int* abort) {
+  unsigned long long t0 = 0;
+  for (uint32_t spin = 1;; spin++) {
+    uint32_t done;
+    asm volatile(
+        "{.reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((spin & 15u) == 0) {
+      if (abort && *abort) return false;
+      const unsigned long long t = now_ns();
+      if (t0 == 0) t0 = t;
+      else if (t - t0 >= limit_ns) return false;
+    }
+  }
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accum) {
+  asm volatile(
+      "{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d), "l"(a),
+      "l"(b), "r"(id), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accum) {
+  asm volatile(
+      "{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes (the caller waits)
+__device__ __forceinline__ void tm_load32(uint32_t addr, float* v) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(addr));
+}
+// the wait ties the registers, so that no use moves above it
+__device__ __forceinline__ void tm_wait32(float* v) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]),
+                 "+r"(u[8]), "+r"(u[9]), "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]),
+                 "+r"(u[15]), "+r"(u[16]), "+r"(u[17]), "+r"(u[18]), "+r"(u[19]), "+r"(u[20]), "+r"(u[21]),
+                 "+r"(u[22]), "+r"(u[23]), "+r"(u[24]), "+r"(u[25]), "+r"(u[26]), "+r"(u[27]), "+r"(u[28]),
+                 "+r"(u[29]), "+r"(u[30]), "+r"(u[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tm_store32(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(u[0]),
+      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+      "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]),
+      "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]),
+      "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(addr)
+      : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ int warp_min_i(int v) {
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) v = min(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// The CTA's i-th work index (item x kv head): forward and backward through the CTAs in
+// turn, so that a CTA that got a long item of one pass gets a short one of the next.
+__device__ __forceinline__ int64_t work_index(int pass) {
+  return (int64_t)pass * gridDim.x + ((pass & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
+struct TcArgs {
+  AttnArgs a;
+  int piece;  // keys per TMA copy: the largest power of two up to 128 that divides a page
+  unsigned long long limit_ns;
+};
+
+// Position of V tile t of n in the item's sequence of K / V tiles: d K tiles lead, then
+// V_t, K_{t+d} alternate.
+__device__ __forceinline__ int v_index(int t, int n, int d) {
+  const int lead = d < n ? d : n, past = t - (n - lead);
+  return lead + 2 * t - (past > 0 ? past : 0);
+}
+
+// Tensor maps: tmq over q [tokens][nq][D], box {64, g, 128 / g}; tmk, tmv over the caches as
+// rows of D, box {64, piece}; all with the 128-byte swizzle.
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                const __grid_constant__ CUtensorMap tmv, const __grid_constant__ TcArgs args) {
+  constexpr int NC = D / 128;  // chunks per K or V tile
+  const AttnArgs& p = args.a;
+  const unsigned long long limit_ns = args.limit_ns;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
+  const uint32_t pad = ((raw + 1023u) & ~1023u) - raw;
+  const uint32_t base = raw + pad;
+  unsigned char* gbase = smem_raw + pad;
+  const uint32_t bars = base + kOffBar;
+  const uint32_t tslot = base + kOffMisc;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + kOffMisc + 4);
+  volatile int* drained_flag = reinterpret_cast<volatile int*>(gbase + kOffMisc + 8);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
+  auto fail = [&]() {
+    atomicOr(p.error, 1);
+    *abort_flag = 1;
+  };
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; s++) {
+      bar_init(bar(kBarFull + s), 1);
+      bar_init(bar(kBarEmpty + s), 1);
+    }
+    bar_init(bar(kBarQFull), 1);
+    bar_init(bar(kBarQEmpty), 5);  // the last score product's commit, and softmax half 0's warps
+    for (int h = 0; h < 2; h++) {
+      bar_init(bar(kBarS + h), 1);
+      bar_init(bar(kBarP + h), 4);
+      bar_init(bar(kBarO + h), 1);
+      bar_init(bar(kBarPV + h), 1);
+    }
+    bar_init(bar(kBarMerge), 4);
+    bar_init(bar(kBarDrain), 1);
+    *abort_flag = 0;
+    *drained_flag = 1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tslot), "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tslot) : "memory");
+  pdl_wait();
+  pdl_launch_dependents();  // (the next launch in the stream is combine_kernel, which waits)
+  const Header* hdr = reinterpret_cast<const Header*>(p.plan);
+  const Item* items = reinterpret_cast<const Item*>(p.plan + p.lay.items);
+  const int64_t nwork = (int64_t)hdr->items * p.nkv;
+  const int g = p.nq / p.nkv;
+
+  if (warp == kProducerWarp) {
+    // ---------------------------------------------------------------- K / V producer
+    uint32_t ring = 0;
+    bool ok = true;
+    const int pr = args.piece, pp = kKeyTile / pr;
+    const int64_t rows_total = p.num_blocks * p.nkv * p.bs;
+    for (int pass = 0; ok; pass++) {
+      const int64_t w = work_index(pass);
+      if (w >= nwork) break;
+      const Item it = items[w / p.nkv];
+      const int kvh = (int)(w % p.nkv);
+      const int n = it.nkt;
+      if (n == 0) continue;
+      const int d = (D == 256 || (it.flags & kFlagFew)) ? 2 : 1;
+      // row of the cache that piece x (of pr keys, counted from key0) starts at; -1: the
+      // piece holds no key of the item and is not read
+      auto piece_row = [&](int x) -> int {
+        const int key = it.key0 + x * pr;
+        if (x >= n * pp || key >= it.len || key + pr <= it.klo) return -1;
+        const int pg = key / p.bs;
+        const int id = pg < p.table_width ? __ldg(p.table + it.req * p.table_stride + pg) : -1;
+        if (id < 0 || id >= p.num_blocks) {
+          atomicOr(p.error, kBadPage);
+          return (int)rows_total;  // outside the map: zeros
+        }
+        return (int)(((int64_t)id * p.nkv + kvh) * p.bs + (key - pg * p.bs));
+      };
+      int win[2] = {-1, -1}, rows[2] = {-1, -1};  // 32 pieces each for K and V
+      auto load = [&](int v, int t) -> bool {
+        const int x0 = t * pp;
+        if (win[v] != (x0 >> 5)) {
+          win[v] = x0 >> 5;
+          rows[v] = piece_row((x0 & ~31) + lane);
+        }
+        const int row = __shfl_sync(0xffffffffu, rows[v], (x0 & 31) + (lane & (pp - 1)));
+        const bool mine = lane < pp && row >= 0;
+        const uint32_t live = __popc(__ballot_sync(0xffffffffu, mine));
+        const CUtensorMap* map = v ? &tmv : &tmk;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          const uint32_t s = ring % kStages;
+          const bool free_ok = bar_wait(bar(kBarEmpty + s), ((ring / kStages) & 1) ^ 1, limit_ns, abort_flag);
+          if (!__all_sync(0xffffffffu, free_ok)) return false;
+          if (lane == 0) bar_expect_tx(bar(kBarFull + s), live * (uint32_t)(pr * 256));
+          __syncwarp();
+          if (mine) {
+            const uint32_t dst = base + kOffRing + s * kChunk + (uint32_t)(lane * pr * 128);
+            tma_2d(dst, map, c * 128, row, bar(kBarFull + s));
+            tma_2d(dst + kSub, map, c * 128 + 64, row, bar(kBarFull + s));
+          }
+          ring++;
+        }
+        return true;
+      };
+      for (int t = 0; t < d && t < n && ok; t++) ok = load(0, t);
+      for (int t = 0; t < n && ok; t++) {
+        ok = load(1, t);
+        if (ok && t + d < n) ok = load(0, t + d);
+      }
+    }
+    if (!ok && lane == 0) fail();
+    // every issued copy lands before the CTA can give its shared memory up
+    bool drained = true;
+    for (uint32_t i = ring > (uint32_t)kStages ? ring - kStages : 0; i < ring; i++)
+      drained &= bar_wait(bar(kBarFull + i % kStages), (i / kStages) & 1, kDrainNs, nullptr);
+    if (!drained && lane == 0) {
+      atomicOr(p.error, 2);
+      *drained_flag = 0;
+    }
+    __syncwarp();
+  } else if (warp == kQWarp) {
+    // ---------------------------------------------------------------- Q
+    if (lane == 0) {
+      uint32_t qi = 0;
+      bool ok = true;
+      const uint32_t box = (uint32_t)(g * p.lay.half_tok) * 128u;
+      for (int pass = 0; ok; pass++) {
+        const int64_t w = work_index(pass);
+        if (w >= nwork) break;
+        const Item it = items[w / p.nkv];
+        const int kvh = (int)(w % p.nkv);
+        if (it.nkt == 0) continue;
+        if (!bar_wait(bar(kBarQEmpty), (qi & 1) ^ 1, limit_ns, abort_flag)) {
+          ok = false;
+          break;
+        }
+        const int halves = D == 128 && !(it.flags & kFlagFew) ? 2 : 1;
+        bar_expect_tx(bar(kBarQFull), box * (uint32_t)(halves * (D / 64)));
+        for (int h = 0; h < halves; h++)
+          for (int c = 0; c < D / 64; c++)
+            tma_3d(base + (uint32_t)(h * kChunk + c * kSub), &tmq, c * 64, kvh * g, it.tok0 + h * p.lay.half_tok,
+                   bar(kBarQFull));
+        qi++;
+      }
+      if (!ok) fail();
+      if (qi > 0 && !bar_wait(bar(kBarQFull), (qi - 1) & 1, kDrainNs, nullptr)) {
+        atomicOr(p.error, 2);
+        *drained_flag = 0;
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      uint32_t ring = 0, qi = 0, np[2] = {0, 0};
+      bool ok = true;
+      auto full = [&](uint32_t r) {
+        return bar_wait(bar(kBarFull + r % kStages), (r / kStages) & 1, limit_ns, abort_flag);
+      };
+      auto stage = [&](uint32_t r) { return base + kOffRing + (r % kStages) * kChunk; };
+      // S_h = Q_q K^T of the tile whose first chunk is r
+      auto scores = [&](int h, int q, uint32_t r) {
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          const uint32_t kb = stage(r + c), qb = base + (uint32_t)(q * kChunk + c * kChunk);
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            mma_ss(tmem + kColS + h * 128, desc_k(qb + (j >> 2) * kSub) + 2 * (j & 3),
+                   desc_k(kb + (j >> 2) * kSub) + 2 * (j & 3), kIdescS, (c | j) != 0);
+        }
+        commit(bar(kBarS + h));
+      };
+      // O += P_h V of the tile whose first chunk is r
+      auto sums = [&](int h, int o, uint32_t r, uint32_t accum) {
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          const uint64_t vd = desc_v(stage(r + c));
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            mma_ts(tmem + kColO + (o + c) * 128, tmem + kColS + h * 128 + j * 8, vd + j * (2048 >> 4), kIdescO,
+                   accum | (j != 0));
+        }
+      };
+      auto release = [&](uint32_t r) {
+#pragma unroll
+        for (int c = 0; c < NC; c++) commit(bar(kBarEmpty + (r + c) % kStages));
+      };
+      auto full_tile = [&](uint32_t r) {
+        bool f = full(r);
+        if (NC == 2) f = f && full(r + 1);
+        return f;
+      };
+      auto probs = [&](int h) { return bar_wait(bar(kBarP + h), np[h]++ & 1, limit_ns, abort_flag); };
+      for (int pass = 0; ok; pass++) {
+        const int64_t w = work_index(pass);
+        if (w >= nwork) break;
+        const Item* ip = items + w / p.nkv;
+        const int n = ip->nkt;
+        if (n == 0) continue;
+        const bool few = D == 128 && (ip->flags & kFlagFew);
+        ok = bar_wait(bar(kBarQFull), qi++ & 1, limit_ns, abort_flag);
+        if (!ok) break;
+        if (D == 128 && !few) {
+          if (!(ok = full(ring))) break;
+          fence_after();
+          scores(0, 0, ring);
+          scores(1, 1, ring);
+          release(ring);
+          if (n == 1) commit(bar(kBarQEmpty));
+          ring++;
+          for (int t = 0; t < n && ok; t++) {
+            const uint32_t rv = ring, rk = ring + 1;
+            const bool more = t + 1 < n;
+            if (!(ok = full(rv))) break;
+            for (int h = 0; h < 2; h++) {
+              if (!(ok = probs(h))) break;
+              if (h == 0 && more && !(ok = full(rk))) break;
+              fence_after();
+              sums(h, h, rv, t > 0);
+              if (more) scores(h, h, rk);
+              else commit(bar(kBarO + h));
+            }
+            if (!ok) break;
+            release(rv);
+            if (more) release(rk);
+            if (t + 2 == n) commit(bar(kBarQEmpty));
+            ring += more ? 2 : 1;
+          }
+        } else {
+          for (int t = 0; t < 2 && t < n; t++) {
+            if (!(ok = full_tile(ring))) break;
+            fence_after();
+            scores(t, 0, ring);
+            release(ring);
+            ring += NC;
+          }
+          if (!ok) break;
+          if (n <= 2) commit(bar(kBarQEmpty));
+          for (int t = 0; t < n; t++) {
+            const int h = t & 1;
+            if (!(ok = full_tile(ring) && probs(h))) break;
+            fence_after();
+            sums(h, D == 128 ? h : 0, ring, D == 128 ? t > 1 : t > 0);
+            if (D == 256) commit(bar(kBarPV + h));
+            release(ring);
+            ring += NC;
+            if (t + 2 < n) {
+              if (!(ok = full_tile(ring))) break;
+              fence_after();
+              scores(h, 0, ring);
+              release(ring);
+              ring += NC;
+              if (t + 3 == n) commit(bar(kBarQEmpty));
+            }
+          }
+          if (!ok) break;
+          commit(bar(kBarO));  // after the whole item: the merge may then overwrite Q
+          if (D == 128 && n > 1) commit(bar(kBarO + 1));
+        }
+      }
+      if (!ok) fail();
+      commit(bar(kBarDrain));  // tracks every MMA issued before it
+      if (!bar_wait(bar(kBarDrain), 0, kDrainNs, nullptr)) {
+        atomicOr(p.error, 2);
+        *drained_flag = 0;
+      }
+    }
+    __syncwarp();
+  } else if (warp < 8 && (D == 128 || warp < 4)) {
+    // ---------------------------------------------------------------- softmax and epilogue
+    const int h = warp >> 2, r = tid & 127;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int* lens = reinterpret_cast<const int*>(p.plan + p.lay.lens);
+    const float c = p.scale * kLog2e;
+    float2* ml_s = reinterpret_cast<float2*>(gbase + kOffMl);
+    float* o_s = reinterpret_cast<float*>(gbase);  // few rows: half 1's sums, [column][row]
+    uint32_t ns[2] = {0, 0}, no = 0, nm = 0, npv[2] = {0, 0}, ring0 = 0;
+    bool ok = true;
+    auto wait = [&](int i, uint32_t parity) {
+      return __all_sync(0xffffffffu, bar_wait(bar(i), parity, limit_ns, abort_flag));
+    };
+    for (int pass = 0; ok; pass++) {
+      const int64_t w = work_index(pass);
+      if (w >= nwork) break;
+      const Item it = items[w / p.nkv];
+      const int kvh = (int)(w % p.nkv);
+      const int n = it.nkt;
+      const bool few = D == 128 && (it.flags & kFlagFew), alt = D == 256 || few;
+      const int local = r / g + (D == 128 && !few ? h * p.lay.half_tok : 0);
+      const int tok = it.tok0 + local, head = kvh * g + r % g;
+      const bool valid = r < g * p.lay.half_tok && local < it.ntok && tok < p.tokens;
+      int2 kk = valid ? row_keys(it, lens, p.window, local) : make_int2(0, 0);
+      const bool any_valid = __any_sync(0xffffffffu, valid);
+      // keys that some row (lo0, hi1) / every row (lo1, hi0) of the warp sees
+      const int lo0 = warp_min_i(valid ? kk.x : INT_MAX), lo1 = -warp_min_i(valid ? -kk.x : INT_MAX);
+      const int hi0 = warp_min_i(valid ? kk.y : INT_MAX), hi1 = -warp_min_i(valid ? -kk.y : INT_MAX);
+      // head_dim 256: the sums of tile t are done.  Even and odd tiles have a barrier each:
+      // a parity tells a phase from its neighbours only, and when the sums of tile t are
+      // asked for (by the softmax of tile t + 1) those of tile t - 2 were announced before
+      // the scores of tile t, and those of tile t + 2 cannot have begun.
+      auto sums_done = [&](int t) { return wait(kBarPV + (t & 1), (npv[t & 1] + (uint32_t)(t >> 1)) & 1); };
+      float m = -INFINITY, l = 0.0f;
+      if (n > 0 && !few && h == 0 && lane == 0) bar_arrive(bar(kBarQEmpty));
+      for (int t = few ? h : 0; t < n; t += few ? 2 : 1) {
+        const int b = D == 256 ? (t & 1) : h;  // score buffer
+        const bool first = few ? t < 2 : t == 0;
+        const uint32_t sb = lanes + kColS + b * 128;
+        if (!(ok = wait(kBarS + b, ns[b]++ & 1))) break;
+        fence_after();
+        const int k0 = it.key0 + t * kKeyTile;
+        if (any_valid && k0 < hi1 && k0 + kKeyTile > lo0) {
+          float s[128];
+#pragma unroll
+          for (int i = 0; i < 4; i++) tm_load32(sb + 32 * i, s + 32 * i);
+#pragma unroll
+          for (int i = 0; i < 4; i++) tm_wait32(s + 32 * i);
+          if (k0 < lo1 || k0 + kKeyTile > hi0) {  // a boundary in this tile
+            const int a = kk.x - k0, z = kk.y - kk.x;
+#pragma unroll
+            for (int i = 0; i < 128; i++) s[i] = z > 0 && (uint32_t)(i - a) < (uint32_t)z ? s[i] : -INFINITY;
+          }
+          float mx = fmaxf(s[0], s[1]);
+#pragma unroll
+          for (int i = 2; i < 128; i += 2) mx = fmaxf(mx, fmaxf(s[i], s[i + 1]));
+          const float mn = fmaxf(m, mx);
+          if (first) {
+            m = mn;
+          } else if (__any_sync(0xffffffffu, (mn - m) * c > 8.0f)) {
+            const float f = mn == -INFINITY ? 1.0f : ex2((m - mn) * c);
+            m = mn;
+            l *= f;
+            if (D == 256) {  // the product before this one has to be done with O
+              if (!(ok = sums_done(t - 1))) break;
+              fence_after();
+            }
+#pragma unroll
+            for (int i = 0; i < D / 32; i++) {
+              float o[32];
+              const uint32_t ob = lanes + kColO + (D == 128 ? h * 128 : 0) + 32 * i;
+              tm_load32(ob, o);
+              tm_wait32(o);
+#pragma unroll
+              for (int j = 0; j < 32; j++) o[j] *= f;
+              tm_store32(ob, reinterpret_cast<const uint32_t*>(o));
+            }
+          }
+          const float neg = m == -INFINITY ? 0.0f : -m * c;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          uint32_t pk[64];
+#pragma unroll
+          for (int i = 0; i < 128; i += 2) {
+            const float x = ex2(__fmaf_rn(s[i], c, neg)), y = ex2(__fmaf_rn(s[i + 1], c, neg));
+            sum[i & 2] += x;
+            sum[(i & 2) + 1] += y;
+            pk[i >> 1] = pack_bf16(x, y);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tm_store32(sb, pk);
+          tm_store32(sb + 32, pk + 32);
+        } else {
+          uint32_t z[32];
+#pragma unroll
+          for (int i = 0; i < 32; i++) z[i] = 0;
+          tm_store32(sb, z);
+          tm_store32(sb + 32, z);
+        }
+        // V rows that hold no key of the request (stale) are zeroed before their product
+        const int tail = it.len - k0, front = it.klo - k0;
+        if ((tail < kKeyTile || front > 0) && (alt || h == 0)) {
+          if (D == 256 && t > 0) {  // (then the ring position read below is this tile's)
+            if (!(ok = sums_done(t - 1))) break;
+          }
+          const uint32_t rv = ring0 + (uint32_t)(NC * v_index(t, n, alt ? 2 : 1));
+          const int z0 = front > 0 ? front : 0, z1 = tail < kKeyTile ? tail : kKeyTile;
+          for (int cc = 0; cc < NC && ok; cc++) {
+            const uint32_t st = (rv + cc) % kStages;
+            if (!(ok = wait(kBarFull + st, ((rv + cc) / kStages) & 1))) break;
+            unsigned char* vb = gbase + kOffRing + st * kChunk;
+            for (int i = r; i < 128 * 16; i += 128) {  // (row, 16 bytes of its two swizzle rows)
+              const int row = i >> 4, q = i & 15;
+              if (row < z0 || row >= z1)
+                *reinterpret_cast<uint4*>(vb + (q >> 3) * kSub + row * 128 + (q & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          if (!ok) break;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar(kBarP + b));
+      }
+      if (!ok) break;
+      ring0 += (uint32_t)(2 * NC * n);
+      npv[0] += (uint32_t)((n + 1) >> 1);
+      npv[1] += (uint32_t)(n >> 1);
+      // -------------------------------------------------------------- epilogue
+      const int mine = few ? (n + 1 - h) / 2 : n;
+      if (mine > 0) {
+        if (!(ok = wait(kBarO + h, no++ & 1))) break;
+        fence_after();
+      }
+      const uint32_t ob = lanes + kColO + (D == 128 ? h * 128 : 0);
+      if (few && h == 1) {  // hand the odd tiles' sums over
+        if (mine > 0) {
+          if (any_valid) {
+#pragma unroll
+            for (int i = 0; i < D / 32; i++) {
+              float o[32];
+              tm_load32(ob + 32 * i, o);
+              tm_wait32(o);
+#pragma unroll
+              for (int j = 0; j < 32; j++) o_s[(32 * i + j) * 128 + r] = o[j];
+            }
+            ml_s[r] = make_float2(m, l);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (Q is loaded over it next)
+          __syncwarp();
+          if (lane == 0) bar_arrive(bar(kBarMerge));
+        }
+        continue;
+      }
+      float f0 = 1.0f, f1 = 0.0f;
+      const bool merge = few && n > 1;
+      if (merge) {
+        if (!(ok = wait(kBarMerge, nm++ & 1))) break;
+        if (any_valid) {
+          const float2 o1 = ml_s[r];
+          const float M = fmaxf(m, o1.x);
+          if (M != -INFINITY) {
+            f0 = ex2((m - M) * c);
+            f1 = ex2((o1.x - M) * c);
+          }
+          l = l * f0 + o1.y * f1;
+          m = M;
+        }
+      }
+      if (any_valid) {
+        const float inv = 1.0f / l;
+        const int64_t prow = (int64_t)(it.part + local * g + r % g) * p.nkv + kvh;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+          float o[32];
+          if (n > 0) {
+            tm_load32(ob + 32 * i, o);
+            tm_wait32(o);
+          }
+          if (merge) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) o[j] = o[j] * f0 + o_s[(32 * i + j) * 128 + r] * f1;
+          }
+          if (valid && it.part < 0) {
+            uint16_t* dst = p.out + tok * p.o_tok + head * p.o_head + 32 * i;
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (l != 0.0f)  // (no key at all: zero)
+                v = make_uint4(pack_bf16(o[j] * inv, o[j + 1] * inv), pack_bf16(o[j + 2] * inv, o[j + 3] * inv),
+                               pack_bf16(o[j + 4] * inv, o[j + 5] * inv), pack_bf16(o[j + 6] * inv, o[j + 7] * inv));
+              *reinterpret_cast<uint4*>(dst + j) = v;
+            }
+          } else if (valid && l != 0.0f) {
+            float* dst = p.part_o + prow * D + 32 * i;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              *reinterpret_cast<float4*>(dst + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+          __syncwarp();  // (the next load is the whole warp's)
+        }
+        if (valid && it.part >= 0) p.part_ml[prow] = make_float2(m * c, l);
+      }
+      if (few && n > 0) {  // Q's buffer may be loaded once all four warps have read the hand-over
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar(kBarQEmpty));
+      }
+    }
+    if (!ok) fail();
+  }
+
+  fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp && *drained_flag) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+}  // namespace tc
+}  // namespace paged
+}  // namespace spark

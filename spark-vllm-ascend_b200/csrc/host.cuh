@@ -97,6 +97,20 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
+// 3-D tensor map of 2-byte elements with the 128-byte swizzle (pitches in bytes)
+inline bool encode_map3(CUtensorMap* m, CUtensorMapDataType dt, const void* base, const uint64_t (&dim)[3],
+                        const uint64_t (&pitch)[2], const uint32_t (&boxes)[3]) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {dim[0], dim[1], dim[2]};
+  cuuint64_t strides[2] = {pitch[0], pitch[1]};
+  cuuint32_t box[3] = {boxes[0], boxes[1], boxes[2]};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(m, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
 // 2-D tensor map: `inner` elements per row (row pitch `pitch` bytes), `outer` rows
 inline bool encode_map(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t outer,
                        uint64_t pitch, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw) {

@@ -4,11 +4,36 @@
 #include <cstdint>
 #include <cstring>
 
+#include "attn_paged.cuh"
 #include "host.cuh"
 #include "paged.cuh"
 #include "spark_b200.h"
 
 using namespace spark;
+
+template <int D>
+static int attn_launch(const paged::AttnArgs& p, int64_t wait_ns, cudaStream_t stream) {
+  const int g = p.nq / p.nkv;
+  paged::tc::TcArgs t;
+  t.a = p;
+  t.piece = p.bs & -p.bs;
+  if (t.piece > paged::kKeyTile) t.piece = paged::kKeyTile;
+  t.limit_ns = wait_ns < 0 ? paged::tc::kWaitNs : (unsigned long long)wait_ns;
+  const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t rows = (uint64_t)p.num_blocks * p.nkv * p.bs;
+  CUtensorMap mq, mk, mv;
+  if (!encode_map3(&mq, bf, p.q, {(uint64_t)D, (uint64_t)p.nq, (uint64_t)p.tokens},
+                   {(uint64_t)p.q_head * 2, (uint64_t)p.q_tok * 2}, {64u, (uint32_t)g, (uint32_t)p.lay.half_tok}) ||
+      !encode_map(&mk, bf, p.k_cache, D, rows, D * 2, 64, (uint32_t)t.piece, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode_map(&mv, bf, p.v_cache, D, rows, D * 2, 64, (uint32_t)t.piece, CU_TENSOR_MAP_SWIZZLE_128B))
+    return SPARK_ERR_LAUNCH;
+  const int grid = (int)std::min<int64_t>((int64_t)p.lay.max_items * p.nkv, num_sms());
+  const int st = launch(paged::tc::attn_kernel<D>, dim3(grid), dim3(paged::tc::kThreads), paged::tc::kSmemBytes,
+                        stream, mq, mk, mv, t);
+  if (st) return st;
+  const int cgrid = (int)std::min<int64_t>((int64_t)p.lay.max_entries * p.nkv, 4LL * num_sms());
+  return launch(paged::combine_kernel<D>, dim3(cgrid), dim3(256), 0, stream, p);
+}
 
 extern "C" {
 
@@ -120,6 +145,11 @@ int spark_attn_paged(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_str
     return SPARK_ERR_UNSUPPORTED_SHAPE;
   if (tokens == 0) return SPARK_OK;
   if (!q || !out) return SPARK_ERR_INVALID_ARG;
+  if ((tokens > 1 && (q_tok_stride <= 0 || out_tok_stride <= 0)) ||
+      (nq > 1 && (q_head_stride <= 0 || out_head_stride <= 0)))
+    return SPARK_ERR_UNSUPPORTED_SHAPE;
+  if (tokens == 1) q_tok_stride = (int64_t)nq * head_dim;  // (of no meaning: any valid pitch)
+  if (nq == 1) q_head_stride = head_dim;
   // tensor-map coordinates are 32-bit rows of the caches
   if (num_blocks * nkv * block_size > 0x7fffffffLL - 128) return SPARK_ERR_TOO_LARGE;
   if (q_tok_stride % 8 || q_head_stride % 8 || out_tok_stride % 8 || out_head_stride % 8 || !aligned(q, 16) ||
@@ -135,15 +165,8 @@ int spark_attn_paged(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_str
   p.plan = static_cast<const unsigned char*>(plan);
   p.lay = paged::layout_of(max_tokens, max_reqs, nq, nkv, head_dim);
   p.part_o = part_o, p.part_ml = reinterpret_cast<float2*>(part_ml), p.out = out, p.error = error;
-  (void)wait_ns;
-  const dim3 grid((unsigned)std::min<int64_t>((int64_t)p.lay.max_items * nkv, 8LL * num_sms()));
-  const dim3 cgrid((unsigned)std::min<int64_t>((int64_t)p.lay.max_entries * nkv, 4LL * num_sms()));
-  if (head_dim == 128) {
-    st = launch(paged::attn_rows_kernel<128>, grid, dim3(256), 0, as_stream(stream), p);
-    return st ? st : launch(paged::combine_kernel<128>, cgrid, dim3(256), 0, as_stream(stream), p);
-  }
-  st = launch(paged::attn_rows_kernel<256>, grid, dim3(256), 0, as_stream(stream), p);
-  return st ? st : launch(paged::combine_kernel<256>, cgrid, dim3(256), 0, as_stream(stream), p);
+  if (head_dim == 128) return attn_launch<128>(p, wait_ns, as_stream(stream));
+  return attn_launch<256>(p, wait_ns, as_stream(stream));
 }
 
 }  // extern "C"

@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(256) rope_store_kernel(RopeArgs p) {
 constexpr int kKeyTile = 128;
 constexpr int kPromptPlan = 1, kPrefixPlan = 2;
 
-struct Item {
+struct alignas(16) Item {
   int tok0, ntok;   // query tokens
   int pos0;         // position of the first one (kFlagLens: unused)
   int req;          // block table row
@@ -298,7 +298,7 @@ constexpr int kFlagFew = 1;   // the tokens fit half a tile: the two halves take
 constexpr int kFlagLens = 2;  // row limits are the requests' lengths (shared prefix), not causal
 static_assert(sizeof(Item) == 48, "items are three 16-byte words");
 
-struct Entry {  // rows to join: tokens tok0 .. tok0 + ntok - 1, part i of a list at base + i * stride
+struct alignas(16) Entry {  // rows to join: tokens tok0 .. tok0 + ntok - 1, part i of a list at base + i * stride
   int tok0, ntok, base_a, n_a, stride_a, base_b, n_b, stride_b;
 };
 
@@ -596,65 +596,6 @@ __device__ __forceinline__ int2 row_keys(const Item& it, const int* lens, int wi
     if (window > 0 && pos + 1 - window > lo) lo = pos + 1 - window;
   }
   return make_int2(lo, hi);
-}
-
-// The plain form of the attention: one warp per query row, a lane holding D / 32 elements,
-// keys one after the other with the running maximum and sum in fp32.
-template <int D>
-__global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs p) {
-  constexpr int E = D / 32;
-  pdl_wait();
-  const Header* hdr = reinterpret_cast<const Header*>(p.plan);
-  const Item* items = reinterpret_cast<const Item*>(p.plan + p.lay.items);
-  const int* lens = reinterpret_cast<const int*>(p.plan + p.lay.lens);
-  const int g = p.nq / p.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const float c = p.scale * kLog2e;
-  const int64_t n = (int64_t)hdr->items * p.nkv;
-  for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
-    const Item it = items[w / p.nkv];
-    const int kvh = (int)(w % p.nkv);
-    for (int row = warp; row < it.ntok * g; row += 8) {
-      const int i = row / g, tok = it.tok0 + i, head = kvh * g + row % g;
-      if (tok >= p.tokens) continue;
-      float q[E], o[E];
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        q[e] = bf2f(p.q[tok * p.q_tok + head * p.q_head + lane * E + e]);
-        o[e] = 0.0f;
-      }
-      float m = -INFINITY, l = 0.0f;
-      const int2 kk = row_keys(it, lens, p.window, i);
-      for (int key = kk.x; key < kk.y; key++) {
-        const int pg = key / p.bs;
-        const int id = pg < p.table_width ? p.table[it.req * p.table_stride + pg] : -1;
-        if (id < 0 || id >= p.num_blocks) {
-          if (lane == 0) atomicOr(p.error, kBadPage);
-          continue;
-        }
-        const int64_t base = (((int64_t)id * p.nkv + kvh) * p.bs + key % p.bs) * D + lane * E;
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; e++) s = __fmaf_rn(q[e], bf2f(p.k_cache[base + e]), s);
-        s = butterfly_sum<32>(s) * c;
-        const float mn = fmaxf(m, s);
-        const float a = exp2f(m - mn), x = exp2f(s - mn);
-        m = mn;
-        l = l * a + x;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = __fmaf_rn(x, bf2f(p.v_cache[base + e]), o[e] * a);
-      }
-      if (it.part < 0) {
-        const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
-#pragma unroll
-        for (int e = 0; e < E; e++) p.out[tok * p.o_tok + head * p.o_head + lane * E + e] = f2bf(o[e] * inv);
-      } else {
-        const int64_t pr = (int64_t)(it.part + row) * p.nkv + kvh;
-#pragma unroll
-        for (int e = 0; e < E; e++) p.part_o[pr * D + lane * E + e] = o[e];
-        if (lane == 0) p.part_ml[pr] = make_float2(m, l);
-      }
-    }
-  }
 }
 
 // Join of the parts of cut tiles: with M = max m_i over a row's parts,
