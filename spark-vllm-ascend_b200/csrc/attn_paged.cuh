@@ -12,7 +12,7 @@
 // Persistent, warp-specialized, one CTA per SM; the CTA walks the plan's items (paged.cuh),
 // longest first, CTA order reversed every other pass so that loads even out.  A tile has
 // the query tokens' g heads as rows, so the K / V of a kv head are read once for the whole
-// group.  352 threads:
+// group.  384 threads:
 //   warps 0-3, 4-7  softmax of accumulator halves 0 / 1, a thread owning one row: scores
 //                   from tensor memory, maximum, p to tensor memory (as the next product's
 //                   A operand) and the item's epilogue;
@@ -20,7 +20,7 @@
 //                   piece and 64 columns into the ring, 128-byte swizzle;
 //   warp 9          owns the tensor memory; one lane issues all MMAs and commits;
 //   warp 10         Q of the next item, as soon as the last score product has read the
-//                   buffer.
+//                   buffer (warp 11 only completes the register split).
 // Shared memory: Q 64 KB, a ring of five 32-KB chunks (128 keys x 128 columns of K or V).
 // Tensor memory: scores S0 S1 (128 columns each, p written over them), sums O0 O1.
 //
@@ -58,7 +58,10 @@ namespace spark {
 namespace paged {
 namespace tc {
 
-constexpr int kThreads = 352;
+constexpr int kThreads = 384;
+// registers: 168 a thread at launch; warps 8-11 give up 80 each, the softmax warps take 40
+// (2 x 208 + 88 = 3 x 168)
+constexpr int kRegsSoftmax = 208, kRegsRest = 88;
 constexpr int kProducerWarp = 8, kMmaWarp = 9, kQWarp = 10;
 constexpr int kStages = 5;
 constexpr int kChunk = 32 * 1024;  // 128 keys x 128 columns
@@ -199,6 +202,15 @@ __device__ __forceinline__ void tm_store32(uint32_t addr, const uint32_t* u) {
       : "memory");
 }
 
+__device__ __forceinline__ void tm_store16(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(
+          u[0]),
+      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+      "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(addr)
+      : "memory");
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -289,225 +301,231 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t nwork = (int64_t)hdr->items * p.nkv;
   const int g = p.nq / p.nkv;
 
-  if (warp == kProducerWarp) {
-    // ---------------------------------------------------------------- K / V producer
-    uint32_t ring = 0;
-    bool ok = true;
-    const int pr = args.piece, pp = kKeyTile / pr;
-    const int64_t rows_total = p.num_blocks * p.nkv * p.bs;
-    for (int pass = 0; ok; pass++) {
-      const int64_t w = work_index(pass);
-      if (w >= nwork) break;
-      const Item it = items[w / p.nkv];
-      const int kvh = (int)(w % p.nkv);
-      const int n = it.nkt;
-      if (n == 0) continue;
-      const int d = (D == 256 || (it.flags & kFlagFew)) ? 2 : 1;
-      // row of the cache that piece x (of pr keys, counted from key0) starts at; -1: the
-      // piece holds no key of the item and is not read
-      auto piece_row = [&](int x) -> int {
-        const int key = it.key0 + x * pr;
-        if (x >= n * pp || key >= it.len || key + pr <= it.klo) return -1;
-        const int pg = key / p.bs;
-        const int id = pg < p.table_width ? __ldg(p.table + it.req * p.table_stride + pg) : -1;
-        if (id < 0 || id >= p.num_blocks) {
-          atomicOr(p.error, kBadPage);
-          return (int)rows_total;  // outside the map: zeros
-        }
-        return (int)(((int64_t)id * p.nkv + kvh) * p.bs + (key - pg * p.bs));
-      };
-      int win[2] = {-1, -1}, rows[2] = {-1, -1};  // 32 pieces each for K and V
-      auto load = [&](int v, int t) -> bool {
-        const int x0 = t * pp;
-        if (win[v] != (x0 >> 5)) {
-          win[v] = x0 >> 5;
-          rows[v] = piece_row((x0 & ~31) + lane);
-        }
-        const int row = __shfl_sync(0xffffffffu, rows[v], (x0 & 31) + (lane & (pp - 1)));
-        const bool mine = lane < pp && row >= 0;
-        const uint32_t live = __popc(__ballot_sync(0xffffffffu, mine));
-        const CUtensorMap* map = v ? &tmv : &tmk;
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-          const uint32_t s = ring % kStages;
-          const bool free_ok = bar_wait(bar(kBarEmpty + s), ((ring / kStages) & 1) ^ 1, limit_ns, abort_flag);
-          if (!__all_sync(0xffffffffu, free_ok)) return false;
-          if (lane == 0) bar_expect_tx(bar(kBarFull + s), live * (uint32_t)(pr * 256));
-          __syncwarp();
-          if (mine) {
-            const uint32_t dst = base + kOffRing + s * kChunk + (uint32_t)(lane * pr * 128);
-            tma_2d(dst, map, c * 128, row, bar(kBarFull + s));
-            tma_2d(dst + kSub, map, c * 128 + 64, row, bar(kBarFull + s));
-          }
-          ring++;
-        }
-        return true;
-      };
-      for (int t = 0; t < d && t < n && ok; t++) ok = load(0, t);
-      for (int t = 0; t < n && ok; t++) {
-        ok = load(1, t);
-        if (ok && t + d < n) ok = load(0, t + d);
-      }
-    }
-    if (!ok && lane == 0) fail();
-    // every issued copy lands before the CTA can give its shared memory up
-    bool drained = true;
-    for (uint32_t i = ring > (uint32_t)kStages ? ring - kStages : 0; i < ring; i++)
-      drained &= bar_wait(bar(kBarFull + i % kStages), (i / kStages) & 1, kDrainNs, nullptr);
-    if (!drained && lane == 0) {
-      atomicOr(p.error, 2);
-      *drained_flag = 0;
-    }
-    __syncwarp();
-  } else if (warp == kQWarp) {
-    // ---------------------------------------------------------------- Q
-    if (lane == 0) {
-      uint32_t qi = 0;
+  // (each warpgroup changes its share inside its own branch, where the register allocator
+  // can tell which share holds)
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+    if (warp == kProducerWarp) {
+      // ---------------------------------------------------------------- K / V producer
+      uint32_t ring = 0;
       bool ok = true;
-      const uint32_t box = (uint32_t)(g * p.lay.half_tok) * 128u;
+      const int pr = args.piece, pp = kKeyTile / pr;
+      const int64_t rows_total = p.num_blocks * p.nkv * p.bs;
       for (int pass = 0; ok; pass++) {
         const int64_t w = work_index(pass);
         if (w >= nwork) break;
         const Item it = items[w / p.nkv];
         const int kvh = (int)(w % p.nkv);
-        if (it.nkt == 0) continue;
-        if (!bar_wait(bar(kBarQEmpty), (qi & 1) ^ 1, limit_ns, abort_flag)) {
-          ok = false;
-          break;
+        const int n = it.nkt;
+        if (n == 0) continue;
+        const int d = (D == 256 || (it.flags & kFlagFew)) ? 2 : 1;
+        // row of the cache that piece x (of pr keys, counted from key0) starts at; -1: the
+        // piece holds no key of the item and is not read
+        auto piece_row = [&](int x) -> int {
+          const int key = it.key0 + x * pr;
+          if (x >= n * pp || key >= it.len || key + pr <= it.klo) return -1;
+          const int pg = key / p.bs;
+          const int id = pg < p.table_width ? __ldg(p.table + it.req * p.table_stride + pg) : -1;
+          if (id < 0 || id >= p.num_blocks) {
+            atomicOr(p.error, kBadPage);
+            return (int)rows_total;  // outside the map: zeros
+          }
+          return (int)(((int64_t)id * p.nkv + kvh) * p.bs + (key - pg * p.bs));
+        };
+        int win[2] = {-1, -1}, rows[2] = {-1, -1};  // 32 pieces each for K and V
+        auto load = [&](int v, int t) -> bool {
+          const int x0 = t * pp;
+          if (win[v] != (x0 >> 5)) {
+            win[v] = x0 >> 5;
+            rows[v] = piece_row((x0 & ~31) + lane);
+          }
+          const int row = __shfl_sync(0xffffffffu, rows[v], (x0 & 31) + (lane & (pp - 1)));
+          const bool mine = lane < pp && row >= 0;
+          const uint32_t live = __popc(__ballot_sync(0xffffffffu, mine));
+          const CUtensorMap* map = v ? &tmv : &tmk;
+#pragma unroll
+          for (int c = 0; c < NC; c++) {
+            const uint32_t s = ring % kStages;
+            const bool free_ok = bar_wait(bar(kBarEmpty + s), ((ring / kStages) & 1) ^ 1, limit_ns, abort_flag);
+            if (!__all_sync(0xffffffffu, free_ok)) return false;
+            if (lane == 0) bar_expect_tx(bar(kBarFull + s), live * (uint32_t)(pr * 256));
+            __syncwarp();
+            if (mine) {
+              const uint32_t dst = base + kOffRing + s * kChunk + (uint32_t)(lane * pr * 128);
+              tma_2d(dst, map, c * 128, row, bar(kBarFull + s));
+              tma_2d(dst + kSub, map, c * 128 + 64, row, bar(kBarFull + s));
+            }
+            ring++;
+          }
+          return true;
+        };
+        for (int t = 0; t < d && t < n && ok; t++) ok = load(0, t);
+        for (int t = 0; t < n && ok; t++) {
+          ok = load(1, t);
+          if (ok && t + d < n) ok = load(0, t + d);
         }
-        const int halves = D == 128 && !(it.flags & kFlagFew) ? 2 : 1;
-        bar_expect_tx(bar(kBarQFull), box * (uint32_t)(halves * (D / 64)));
-        for (int h = 0; h < halves; h++)
-          for (int c = 0; c < D / 64; c++)
-            tma_3d(base + (uint32_t)(h * kChunk + c * kSub), &tmq, c * 64, kvh * g, it.tok0 + h * p.lay.half_tok,
-                   bar(kBarQFull));
-        qi++;
       }
-      if (!ok) fail();
-      if (qi > 0 && !bar_wait(bar(kBarQFull), (qi - 1) & 1, kDrainNs, nullptr)) {
+      if (!ok && lane == 0) fail();
+      // every issued copy lands before the CTA can give its shared memory up
+      bool drained = true;
+      for (uint32_t i = ring > (uint32_t)kStages ? ring - kStages : 0; i < ring; i++)
+        drained &= bar_wait(bar(kBarFull + i % kStages), (i / kStages) & 1, kDrainNs, nullptr);
+      if (!drained && lane == 0) {
         atomicOr(p.error, 2);
         *drained_flag = 0;
       }
-    }
-    __syncwarp();
-  } else if (warp == kMmaWarp) {
-    // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      uint32_t ring = 0, qi = 0, np[2] = {0, 0};
-      bool ok = true;
-      auto full = [&](uint32_t r) {
-        return bar_wait(bar(kBarFull + r % kStages), (r / kStages) & 1, limit_ns, abort_flag);
-      };
-      auto stage = [&](uint32_t r) { return base + kOffRing + (r % kStages) * kChunk; };
-      // S_h = Q_q K^T of the tile whose first chunk is r
-      auto scores = [&](int h, int q, uint32_t r) {
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-          const uint32_t kb = stage(r + c), qb = base + (uint32_t)(q * kChunk + c * kChunk);
-#pragma unroll
-          for (int j = 0; j < 8; j++)
-            mma_ss(tmem + kColS + h * 128, desc_k(qb + (j >> 2) * kSub) + 2 * (j & 3),
-                   desc_k(kb + (j >> 2) * kSub) + 2 * (j & 3), kIdescS, (c | j) != 0);
-        }
-        commit(bar(kBarS + h));
-      };
-      // O += P_h V of the tile whose first chunk is r
-      auto sums = [&](int h, int o, uint32_t r, uint32_t accum) {
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-          const uint64_t vd = desc_v(stage(r + c));
-#pragma unroll
-          for (int j = 0; j < 8; j++)
-            mma_ts(tmem + kColO + (o + c) * 128, tmem + kColS + h * 128 + j * 8, vd + j * (2048 >> 4), kIdescO,
-                   accum | (j != 0));
-        }
-      };
-      auto release = [&](uint32_t r) {
-#pragma unroll
-        for (int c = 0; c < NC; c++) commit(bar(kBarEmpty + (r + c) % kStages));
-      };
-      auto full_tile = [&](uint32_t r) {
-        bool f = full(r);
-        if (NC == 2) f = f && full(r + 1);
-        return f;
-      };
-      auto probs = [&](int h) { return bar_wait(bar(kBarP + h), np[h]++ & 1, limit_ns, abort_flag); };
-      for (int pass = 0; ok; pass++) {
-        const int64_t w = work_index(pass);
-        if (w >= nwork) break;
-        const Item* ip = items + w / p.nkv;
-        const int n = ip->nkt;
-        if (n == 0) continue;
-        const bool few = D == 128 && (ip->flags & kFlagFew);
-        ok = bar_wait(bar(kBarQFull), qi++ & 1, limit_ns, abort_flag);
-        if (!ok) break;
-        if (D == 128 && !few) {
-          if (!(ok = full(ring))) break;
-          fence_after();
-          scores(0, 0, ring);
-          scores(1, 1, ring);
-          release(ring);
-          if (n == 1) commit(bar(kBarQEmpty));
-          ring++;
-          for (int t = 0; t < n && ok; t++) {
-            const uint32_t rv = ring, rk = ring + 1;
-            const bool more = t + 1 < n;
-            if (!(ok = full(rv))) break;
-            for (int h = 0; h < 2; h++) {
-              if (!(ok = probs(h))) break;
-              if (h == 0 && more && !(ok = full(rk))) break;
-              fence_after();
-              sums(h, h, rv, t > 0);
-              if (more) scores(h, h, rk);
-              else commit(bar(kBarO + h));
-            }
-            if (!ok) break;
-            release(rv);
-            if (more) release(rk);
-            if (t + 2 == n) commit(bar(kBarQEmpty));
-            ring += more ? 2 : 1;
+      __syncwarp();
+    } else if (warp == kQWarp) {
+      // ---------------------------------------------------------------- Q
+      if (lane == 0) {
+        uint32_t qi = 0;
+        bool ok = true;
+        const uint32_t box = (uint32_t)(g * p.lay.half_tok) * 128u;
+        for (int pass = 0; ok; pass++) {
+          const int64_t w = work_index(pass);
+          if (w >= nwork) break;
+          const Item it = items[w / p.nkv];
+          const int kvh = (int)(w % p.nkv);
+          if (it.nkt == 0) continue;
+          if (!bar_wait(bar(kBarQEmpty), (qi & 1) ^ 1, limit_ns, abort_flag)) {
+            ok = false;
+            break;
           }
-        } else {
-          for (int t = 0; t < 2 && t < n; t++) {
-            if (!(ok = full_tile(ring))) break;
-            fence_after();
-            scores(t, 0, ring);
-            release(ring);
-            ring += NC;
+          const int halves = D == 128 && !(it.flags & kFlagFew) ? 2 : 1;
+          bar_expect_tx(bar(kBarQFull), box * (uint32_t)(halves * (D / 64)));
+          for (int h = 0; h < halves; h++)
+            for (int c = 0; c < D / 64; c++)
+              tma_3d(base + (uint32_t)(h * kChunk + c * kSub), &tmq, c * 64, kvh * g, it.tok0 + h * p.lay.half_tok,
+                     bar(kBarQFull));
+          qi++;
+        }
+        if (!ok) fail();
+        if (qi > 0 && !bar_wait(bar(kBarQFull), (qi - 1) & 1, kDrainNs, nullptr)) {
+          atomicOr(p.error, 2);
+          *drained_flag = 0;
+        }
+      }
+      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      // ---------------------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        uint32_t ring = 0, qi = 0, np[2] = {0, 0};
+        bool ok = true;
+        auto full = [&](uint32_t r) {
+          return bar_wait(bar(kBarFull + r % kStages), (r / kStages) & 1, limit_ns, abort_flag);
+        };
+        auto stage = [&](uint32_t r) { return base + kOffRing + (r % kStages) * kChunk; };
+        // S_h = Q_q K^T of the tile whose first chunk is r
+        auto scores = [&](int h, int q, uint32_t r) {
+#pragma unroll
+          for (int c = 0; c < NC; c++) {
+            const uint32_t kb = stage(r + c), qb = base + (uint32_t)(q * kChunk + c * kChunk);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+              mma_ss(tmem + kColS + h * 128, desc_k(qb + (j >> 2) * kSub) + 2 * (j & 3),
+                     desc_k(kb + (j >> 2) * kSub) + 2 * (j & 3), kIdescS, (c | j) != 0);
           }
+          commit(bar(kBarS + h));
+        };
+        // O += P_h V of the tile whose first chunk is r
+        auto sums = [&](int h, int o, uint32_t r, uint32_t accum) {
+#pragma unroll
+          for (int c = 0; c < NC; c++) {
+            const uint64_t vd = desc_v(stage(r + c));
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+              mma_ts(tmem + kColO + (o + c) * 128, tmem + kColS + h * 128 + j * 8, vd + j * (2048 >> 4), kIdescO,
+                     accum | (j != 0));
+          }
+        };
+        auto release = [&](uint32_t r) {
+#pragma unroll
+          for (int c = 0; c < NC; c++) commit(bar(kBarEmpty + (r + c) % kStages));
+        };
+        auto full_tile = [&](uint32_t r) {
+          bool f = full(r);
+          if (NC == 2) f = f && full(r + 1);
+          return f;
+        };
+        auto probs = [&](int h) { return bar_wait(bar(kBarP + h), np[h]++ & 1, limit_ns, abort_flag); };
+        for (int pass = 0; ok; pass++) {
+          const int64_t w = work_index(pass);
+          if (w >= nwork) break;
+          const Item* ip = items + w / p.nkv;
+          const int n = ip->nkt;
+          if (n == 0) continue;
+          const bool few = D == 128 && (ip->flags & kFlagFew);
+          ok = bar_wait(bar(kBarQFull), qi++ & 1, limit_ns, abort_flag);
           if (!ok) break;
-          if (n <= 2) commit(bar(kBarQEmpty));
-          for (int t = 0; t < n; t++) {
-            const int h = t & 1;
-            if (!(ok = full_tile(ring) && probs(h))) break;
+          if (D == 128 && !few) {
+            if (!(ok = full(ring))) break;
             fence_after();
-            sums(h, D == 128 ? h : 0, ring, D == 128 ? t > 1 : t > 0);
-            if (D == 256) commit(bar(kBarPV + h));
+            scores(0, 0, ring);
+            scores(1, 1, ring);
             release(ring);
-            ring += NC;
-            if (t + 2 < n) {
+            if (n == 1) commit(bar(kBarQEmpty));
+            ring++;
+            for (int t = 0; t < n && ok; t++) {
+              const uint32_t rv = ring, rk = ring + 1;
+              const bool more = t + 1 < n;
+              if (!(ok = full(rv))) break;
+              for (int h = 0; h < 2; h++) {
+                if (!(ok = probs(h))) break;
+                if (h == 0 && more && !(ok = full(rk))) break;
+                fence_after();
+                sums(h, h, rv, t > 0);
+                if (more) scores(h, h, rk);
+                else commit(bar(kBarO + h));
+              }
+              if (!ok) break;
+              release(rv);
+              if (more) release(rk);
+              if (t + 2 == n) commit(bar(kBarQEmpty));
+              ring += more ? 2 : 1;
+            }
+          } else {
+            for (int t = 0; t < 2 && t < n; t++) {
               if (!(ok = full_tile(ring))) break;
               fence_after();
-              scores(h, 0, ring);
+              scores(t, 0, ring);
               release(ring);
               ring += NC;
-              if (t + 3 == n) commit(bar(kBarQEmpty));
             }
+            if (!ok) break;
+            if (n <= 2) commit(bar(kBarQEmpty));
+            for (int t = 0; t < n; t++) {
+              const int h = t & 1;
+              if (!(ok = full_tile(ring) && probs(h))) break;
+              fence_after();
+              sums(h, D == 128 ? h : 0, ring, D == 128 ? t > 1 : t > 0);
+              if (D == 256) commit(bar(kBarPV + h));
+              release(ring);
+              ring += NC;
+              if (t + 2 < n) {
+                if (!(ok = full_tile(ring))) break;
+                fence_after();
+                scores(h, 0, ring);
+                release(ring);
+                ring += NC;
+                if (t + 3 == n) commit(bar(kBarQEmpty));
+              }
+            }
+            if (!ok) break;
+            commit(bar(kBarO));  // after the whole item: the merge may then overwrite Q
+            if (D == 128 && n > 1) commit(bar(kBarO + 1));
           }
-          if (!ok) break;
-          commit(bar(kBarO));  // after the whole item: the merge may then overwrite Q
-          if (D == 128 && n > 1) commit(bar(kBarO + 1));
+        }
+        if (!ok) fail();
+        commit(bar(kBarDrain));  // tracks every MMA issued before it
+        if (!bar_wait(bar(kBarDrain), 0, kDrainNs, nullptr)) {
+          atomicOr(p.error, 2);
+          *drained_flag = 0;
         }
       }
-      if (!ok) fail();
-      commit(bar(kBarDrain));  // tracks every MMA issued before it
-      if (!bar_wait(bar(kBarDrain), 0, kDrainNs, nullptr)) {
-        atomicOr(p.error, 2);
-        *drained_flag = 0;
-      }
+      __syncwarp();
     }
-    __syncwarp();
-  } else if (warp < 8 && (D == 128 || warp < 4)) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ---------------------------------------------------------------- softmax and epilogue
     const int h = warp >> 2, r = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -520,7 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto wait = [&](int i, uint32_t parity) {
       return __all_sync(0xffffffffu, bar_wait(bar(i), parity, limit_ns, abort_flag));
     };
-    for (int pass = 0; ok; pass++) {
+    // (head_dim 256: one softmax, by half 0)
+    for (int pass = 0; ok && (D == 128 || h == 0); pass++) {
       const int64_t w = work_index(pass);
       if (w >= nwork) break;
       const Item it = items[w / p.nkv];
@@ -551,22 +570,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int k0 = it.key0 + t * kKeyTile;
         if (any_valid && k0 < hi1 && k0 + kKeyTile > lo0) {
           float s[128];
+          for (;;) {  // (a second time after a rescale: the scores are not kept over it)
 #pragma unroll
-          for (int i = 0; i < 4; i++) tm_load32(sb + 32 * i, s + 32 * i);
+            for (int i = 0; i < 4; i++) tm_load32(sb + 32 * i, s + 32 * i);
 #pragma unroll
-          for (int i = 0; i < 4; i++) tm_wait32(s + 32 * i);
-          if (k0 < lo1 || k0 + kKeyTile > hi0) {  // a boundary in this tile
-            const int a = kk.x - k0, z = kk.y - kk.x;
+            for (int i = 0; i < 4; i++) tm_wait32(s + 32 * i);
+            if (k0 < lo1 || k0 + kKeyTile > hi0) {  // a boundary in this tile
+              const int a = kk.x - k0, z = kk.y - kk.x;
 #pragma unroll
-            for (int i = 0; i < 128; i++) s[i] = z > 0 && (uint32_t)(i - a) < (uint32_t)z ? s[i] : -INFINITY;
-          }
-          float mx = fmaxf(s[0], s[1]);
+              for (int i = 0; i < 128; i++) s[i] = z > 0 && (uint32_t)(i - a) < (uint32_t)z ? s[i] : -INFINITY;
+            }
+            float mx = fmaxf(s[0], s[1]);
 #pragma unroll
-          for (int i = 2; i < 128; i += 2) mx = fmaxf(mx, fmaxf(s[i], s[i + 1]));
-          const float mn = fmaxf(m, mx);
-          if (first) {
-            m = mn;
-          } else if (__any_sync(0xffffffffu, (mn - m) * c > 8.0f)) {
+            for (int i = 2; i < 128; i += 2) mx = fmaxf(mx, fmaxf(s[i], s[i + 1]));
+            const float mn = fmaxf(m, mx);
+            if (first) {
+              m = mn;
+              break;
+            }
+            if (!__any_sync(0xffffffffu, (mn - m) * c > 8.0f)) break;
             const float f = mn == -INFINITY ? 1.0f : ex2((m - mn) * c);
             m = mn;
             l *= f;
@@ -574,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!(ok = sums_done(t - 1))) break;
               fence_after();
             }
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < D / 32; i++) {
               float o[32];
               const uint32_t ob = lanes + kColO + (D == 128 ? h * 128 : 0) + 32 * i;
@@ -585,19 +607,22 @@ __global__ void __launch_bounds__(kThreads, 1)
               tm_store32(ob, reinterpret_cast<const uint32_t*>(o));
             }
           }
+          if (!ok) break;
           const float neg = m == -INFINITY ? 0.0f : -m * c;
           float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          uint32_t pk[64];
 #pragma unroll
-          for (int i = 0; i < 128; i += 2) {
-            const float x = ex2(__fmaf_rn(s[i], c, neg)), y = ex2(__fmaf_rn(s[i + 1], c, neg));
-            sum[i & 2] += x;
-            sum[(i & 2) + 1] += y;
-            pk[i >> 1] = pack_bf16(x, y);
+          for (int q = 0; q < 4; q++) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const float x = ex2(__fmaf_rn(s[32 * q + 2 * i], c, neg)), y = ex2(__fmaf_rn(s[32 * q + 2 * i + 1], c, neg));
+              sum[(i & 1) * 2] += x;
+              sum[(i & 1) * 2 + 1] += y;
+              pk[i] = pack_bf16(x, y);
+            }
+            tm_store16(sb + 16 * q, pk);
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tm_store32(sb, pk);
-          tm_store32(sb + 32, pk + 32);
         } else {
           uint32_t z[32];
 #pragma unroll
