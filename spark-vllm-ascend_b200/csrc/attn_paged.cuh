@@ -70,10 +70,11 @@ constexpr int kOffRing = 64 * 1024;
 constexpr int kOffMl = kOffRing + kStages * kChunk;  // few rows: (m, l) of half 1
 constexpr int kOffBar = kOffMl + 128 * 8;
 constexpr int kBarFull = 0, kBarEmpty = kBarFull + kStages, kBarQFull = kBarEmpty + kStages,
-              kBarQEmpty = kBarQFull + 1, kBarS = kBarQEmpty + 1, kBarP = kBarS + 2, kBarO = kBarP + 2,
+              kBarQEmpty = kBarQFull + 1, kBarS = kBarQEmpty + 1, kBarP = kBarS + 2, kBarP2 = kBarP + 2, kBarO = kBarP2 + 2,
               kBarPV = kBarO + 2, kBarMerge = kBarPV + 2, kBarDrain = kBarMerge + 1, kNumBars = kBarDrain + 1;
 constexpr int kOffMisc = kOffBar + 8 * kNumBars;  // tensor-memory base, abort flag, drained flag
-constexpr int kSmemBytes = kOffMisc + 16 + 1024;  // + 1024-byte alignment slack
+constexpr int kOffItem = (kOffMisc + 16 + 15) / 16 * 16;  // the current item and its kv head
+constexpr int kSmemBytes = kOffItem + 64 + 1024;  // + 1024-byte alignment slack
 constexpr int kTmemCols = 512;
 constexpr int kColS = 0, kColO = 256;
 constexpr unsigned long long kWaitNs = 500ull * 1000 * 1000;
@@ -211,10 +212,89 @@ __device__ __forceinline__ void tm_store16(uint32_t addr, const uint32_t* u) {
       : "memory");
 }
 
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 pack2(float lo, float hi) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(u64 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^x of a pair by arithmetic alone, for the special-function unit's relief: x = n + f with
+// n the nearest integer (adding 1.5 2^23 leaves n in the low bits), 2^f a cubic on
+// [-1/2, 1/2] fitted here to the least maximal relative error (7.5e-5, against the 2^-8 of
+// the bf16 rounding that follows), n added to the exponent.  x <= 127; below -127 the
+// result is a denormal of no weight, not zero: tiles with masked keys do not come here.
+__device__ __forceinline__ u64 ex2_poly(u64 x2) {
+  float x, y;
+  unpack2(x2, x, y);
+  x2 = pack2(fmaxf(x, -127.0f), fmaxf(y, -127.0f));
+  const u64 magic = pack2(12582912.0f, 12582912.0f), unmagic = pack2(-12582912.0f, -12582912.0f);
+  const u64 t = add2(x2, magic);
+  const u64 f = fma2(add2(t, unmagic), pack2(-1.0f, -1.0f), x2);
+  u64 r = fma2(pack2(0.05517132207751274f, 0.05517132207751274f), f, pack2(0.2426113337278366f, 0.2426113337278366f));
+  r = fma2(r, f, pack2(0.6932610869407654f, 0.6932610869407654f));
+  r = fma2(r, f, pack2(0.9999280571937561f, 0.9999280571937561f));
+  float a, b, n, k;
+  unpack2(r, a, b);
+  unpack2(t, n, k);
+  return pack2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(n) << 23)),
+               __uint_as_float(__float_as_uint(b) + (__float_as_uint(k) << 23)));
+}
+// p = 2^(s c + neg) of 32 scores: sums in fp32, the bf16 pairs to pk.  kPoly of 16 pairs go
+// through ex2_poly.
+template <int kPoly>
+__device__ __forceinline__ void probs32(const float* s, u64 c2, u64 neg2, u64 (&sum)[2], uint32_t (&pk)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    u64 x2 = fma2(pack2(s[2 * i], s[2 * i + 1]), c2, neg2);
+    float x, y;
+    if ((i * kPoly) / 16 != ((i + 1) * kPoly) / 16) {  // (kPoly pairs, evenly spread)
+      x2 = ex2_poly(x2);
+      unpack2(x2, x, y);
+    } else {
+      unpack2(x2, x, y);
+      x = ex2(x);
+      y = ex2(y);
+      x2 = pack2(x, y);
+    }
+    sum[i & 1] = add2(sum[i & 1], x2);
+    pk[i] = pack_bf16(x, y);
+  }
+}
+constexpr int kPolyPairs = 4;
+
+// 32 bytes (wide) or two times 16 to global memory
+__device__ __forceinline__ void store32(void* dst, const uint32_t* v, bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(dst)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<uint4*>(dst)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
 }
 __device__ __forceinline__ int warp_min_i(int v) {
 #pragma unroll
@@ -231,6 +311,7 @@ __device__ __forceinline__ int64_t work_index(int pass) {
 struct TcArgs {
   AttnArgs a;
   int piece;  // keys per TMA copy: the largest power of two up to 128 that divides a page
+  bool wide;  // out and its strides are multiples of 32 bytes
   unsigned long long limit_ns;
 };
 
@@ -272,10 +353,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(bar(kBarEmpty + s), 1);
     }
     bar_init(bar(kBarQFull), 1);
-    bar_init(bar(kBarQEmpty), 5);  // the last score product's commit, and softmax half 0's warps
+    bar_init(bar(kBarQEmpty), D == 128 ? 9 : 5);  // the last score product's commit, the softmax warps
     for (int h = 0; h < 2; h++) {
       bar_init(bar(kBarS + h), 1);
       bar_init(bar(kBarP + h), 4);
+      bar_init(bar(kBarP2 + h), 4);
       bar_init(bar(kBarO + h), 1);
       bar_init(bar(kBarPV + h), 1);
     }
@@ -381,15 +463,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t qi = 0;
         bool ok = true;
         const uint32_t box = (uint32_t)(g * p.lay.half_tok) * 128u;
+        Item* slot = reinterpret_cast<Item*>(gbase + kOffItem);
+        int* slot_kvh = reinterpret_cast<int*>(gbase + kOffItem + sizeof(Item));
         for (int pass = 0; ok; pass++) {
           const int64_t w = work_index(pass);
-          if (w >= nwork) break;
-          const Item it = items[w / p.nkv];
-          const int kvh = (int)(w % p.nkv);
-          if (it.nkt == 0) continue;
+          const bool have = w < nwork;
+          Item it;
+          int kvh = 0;
+          if (have) {  // (read before the wait, written after it)
+            it = items[w / p.nkv];
+            kvh = (int)(w % p.nkv);
+          }
           if (!bar_wait(bar(kBarQEmpty), (qi & 1) ^ 1, limit_ns, abort_flag)) {
             ok = false;
             break;
+          }
+          qi++;
+          if (!have) {
+            slot->nkt = -1;
+            bar_arrive(bar(kBarQFull));
+            break;
+          }
+          *slot = it;
+          *slot_kvh = kvh;
+          if (it.nkt == 0) {
+            bar_arrive(bar(kBarQFull));
+            continue;
           }
           const int halves = D == 128 && !(it.flags & kFlagFew) ? 2 : 1;
           bar_expect_tx(bar(kBarQFull), box * (uint32_t)(halves * (D / 64)));
@@ -397,7 +496,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < D / 64; c++)
               tma_3d(base + (uint32_t)(h * kChunk + c * kSub), &tmq, c * 64, kvh * g, it.tok0 + h * p.lay.half_tok,
                      bar(kBarQFull));
-          qi++;
         }
         if (!ok) fail();
         if (qi > 0 && !bar_wait(bar(kBarQFull), (qi - 1) & 1, kDrainNs, nullptr)) {
@@ -427,16 +525,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           commit(bar(kBarS + h));
         };
-        // O += P_h V of the tile whose first chunk is r
+        // O += P_h V of the tile whose first chunk is r, in two steps: the first 64 keys'
+        // probabilities are multiplied while the others are still computed
         auto sums = [&](int h, int o, uint32_t r, uint32_t accum) {
 #pragma unroll
-          for (int c = 0; c < NC; c++) {
-            const uint64_t vd = desc_v(stage(r + c));
+          for (int k = 0; k < 2; k++) {
+            if (!bar_wait(bar((k ? kBarP2 : kBarP) + h), np[h] & 1, limit_ns, abort_flag)) return false;
+            fence_after();
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-              mma_ts(tmem + kColO + (o + c) * 128, tmem + kColS + h * 128 + j * 8, vd + j * (2048 >> 4), kIdescO,
-                     accum | (j != 0));
+            for (int c = 0; c < NC; c++) {
+              const uint64_t vd = desc_v(stage(r + c));
+#pragma unroll
+              for (int j = 4 * k; j < 4 * k + 4; j++)
+                mma_ts(tmem + kColO + (o + c) * 128, tmem + kColS + h * 128 + j * 8, vd + j * (2048 >> 4), kIdescO,
+                       accum | (j != 0));
+            }
           }
+          np[h]++;
+          return true;
         };
         auto release = [&](uint32_t r) {
 #pragma unroll
@@ -447,16 +553,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (NC == 2) f = f && full(r + 1);
           return f;
         };
-        auto probs = [&](int h) { return bar_wait(bar(kBarP + h), np[h]++ & 1, limit_ns, abort_flag); };
-        for (int pass = 0; ok; pass++) {
-          const int64_t w = work_index(pass);
-          if (w >= nwork) break;
-          const Item* ip = items + w / p.nkv;
-          const int n = ip->nkt;
-          if (n == 0) continue;
-          const bool few = D == 128 && (ip->flags & kFlagFew);
+        const Item* slot = reinterpret_cast<const Item*>(gbase + kOffItem);
+        while (ok) {
           ok = bar_wait(bar(kBarQFull), qi++ & 1, limit_ns, abort_flag);
           if (!ok) break;
+          const int n = slot->nkt;
+          const bool few = D == 128 && (slot->flags & kFlagFew);
+          if (n < 0) break;
+          if (n == 0) {
+            bar_arrive(bar(kBarQEmpty));
+            continue;
+          }
           if (D == 128 && !few) {
             if (!(ok = full(ring))) break;
             fence_after();
@@ -470,10 +577,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               const bool more = t + 1 < n;
               if (!(ok = full(rv))) break;
               for (int h = 0; h < 2; h++) {
-                if (!(ok = probs(h))) break;
-                if (h == 0 && more && !(ok = full(rk))) break;
-                fence_after();
-                sums(h, h, rv, t > 0);
+                if (!(ok = sums(h, h, rv, t > 0))) break;
+                if (h == 0 && more) {
+                  if (!(ok = full(rk))) break;
+                  fence_after();
+                }
                 if (more) scores(h, h, rk);
                 else commit(bar(kBarO + h));
               }
@@ -495,9 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (n <= 2) commit(bar(kBarQEmpty));
             for (int t = 0; t < n; t++) {
               const int h = t & 1;
-              if (!(ok = full_tile(ring) && probs(h))) break;
-              fence_after();
-              sums(h, D == 128 ? h : 0, ring, D == 128 ? t > 1 : t > 0);
+              if (!(ok = full_tile(ring) && sums(h, D == 128 ? h : 0, ring, D == 128 ? t > 1 : t > 0))) break;
               if (D == 256) commit(bar(kBarPV + h));
               release(ring);
               ring += NC;
@@ -538,17 +644,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto wait = [&](int i, uint32_t parity) {
       return __all_sync(0xffffffffu, bar_wait(bar(i), parity, limit_ns, abort_flag));
     };
+    const int local_row = r / g, head_row = r % g;
+    const bool row_used = r < g * p.lay.half_tok;
+    const u64 c2 = pack2(c, c);
+    uint32_t qi = 0;
     // (head_dim 256: one softmax, by half 0)
-    for (int pass = 0; ok && (D == 128 || h == 0); pass++) {
-      const int64_t w = work_index(pass);
-      if (w >= nwork) break;
-      const Item it = items[w / p.nkv];
-      const int kvh = (int)(w % p.nkv);
+    while (ok && (D == 128 || h == 0)) {
+      if (!(ok = wait(kBarQFull, qi++ & 1))) break;
+      const Item it = *reinterpret_cast<const Item*>(gbase + kOffItem);
+      const int kvh = *reinterpret_cast<const int*>(gbase + kOffItem + sizeof(Item));
       const int n = it.nkt;
+      if (n < 0) break;
       const bool few = D == 128 && (it.flags & kFlagFew), alt = D == 256 || few;
-      const int local = r / g + (D == 128 && !few ? h * p.lay.half_tok : 0);
-      const int tok = it.tok0 + local, head = kvh * g + r % g;
-      const bool valid = r < g * p.lay.half_tok && local < it.ntok && tok < p.tokens;
+      const int local = local_row + (D == 128 && !few ? h * p.lay.half_tok : 0);
+      const int tok = it.tok0 + local, head = kvh * g + head_row;
+      const bool valid = row_used && local < it.ntok && tok < p.tokens;
       int2 kk = valid ? row_keys(it, lens, p.window, local) : make_int2(0, 0);
       const bool any_valid = __any_sync(0xffffffffu, valid);
       // keys that some row (lo0, hi1) / every row (lo1, hi0) of the warp sees
@@ -560,7 +670,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the scores of tile t, and those of tile t + 2 cannot have begun.
       auto sums_done = [&](int t) { return wait(kBarPV + (t & 1), (npv[t & 1] + (uint32_t)(t >> 1)) & 1); };
       float m = -INFINITY, l = 0.0f;
-      if (n > 0 && !few && h == 0 && lane == 0) bar_arrive(bar(kBarQEmpty));
+      // this half is done with the item slot, and with Q's buffer unless sums pass through it
+      if (n == 0 || !few || (h == 1 && n == 1)) {
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar(kBarQEmpty));
+      }
       for (int t = few ? h : 0; t < n; t += few ? 2 : 1) {
         const int b = D == 256 ? (t & 1) : h;  // score buffer
         const bool first = few ? t < 2 : t == 0;
@@ -568,21 +682,56 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = wait(kBarS + b, ns[b]++ & 1))) break;
         fence_after();
         const int k0 = it.key0 + t * kKeyTile;
+        // V rows that hold no key of the request (stale) are zeroed before their product
+        const int tail = it.len - k0, front = it.klo - k0;
+        if ((tail < kKeyTile || front > 0) && (alt || h == 0)) {
+          if (D == 256 && t > 0) {  // (then the ring position read below is this tile's)
+            if (!(ok = sums_done(t - 1))) break;
+          }
+          const uint32_t rv = ring0 + (uint32_t)(NC * v_index(t, n, alt ? 2 : 1));
+          const int z0 = front > 0 ? front : 0, z1 = tail < kKeyTile ? tail : kKeyTile;
+          for (int cc = 0; cc < NC && ok; cc++) {
+            const uint32_t st = (rv + cc) % kStages;
+            if (!(ok = wait(kBarFull + st, ((rv + cc) / kStages) & 1))) break;
+            unsigned char* vb = gbase + kOffRing + st * kChunk;
+            for (int i = r; i < 128 * 16; i += 128) {  // (row, 16 bytes of its two swizzle rows)
+              const int row = i >> 4, q = i & 15;
+              if (row < z0 || row >= z1)
+                *reinterpret_cast<uint4*>(vb + (q >> 3) * kSub + row * 128 + (q & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          if (!ok) break;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        // this warp's share of the first (k = 0) or last 64 keys' probabilities is written
+        auto announce = [&](int k) {
+          wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(bar((k ? kBarP2 : kBarP) + b));
+        };
         if (any_valid && k0 < hi1 && k0 + kKeyTile > lo0) {
+          const bool edge = k0 < lo1 || k0 + kKeyTile > hi0;  // some row sees a part of the tile only
           float s[128];
           for (;;) {  // (a second time after a rescale: the scores are not kept over it)
 #pragma unroll
             for (int i = 0; i < 4; i++) tm_load32(sb + 32 * i, s + 32 * i);
 #pragma unroll
             for (int i = 0; i < 4; i++) tm_wait32(s + 32 * i);
-            if (k0 < lo1 || k0 + kKeyTile > hi0) {  // a boundary in this tile
+            if (edge) {
               const int a = kk.x - k0, z = kk.y - kk.x;
 #pragma unroll
               for (int i = 0; i < 128; i++) s[i] = z > 0 && (uint32_t)(i - a) < (uint32_t)z ? s[i] : -INFINITY;
             }
-            float mx = fmaxf(s[0], s[1]);
+            float mx4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 2; i < 128; i += 2) mx = fmaxf(mx, fmaxf(s[i], s[i + 1]));
+            for (int i = 4; i < 124; i += 8) {
+#pragma unroll
+              for (int j = 0; j < 4; j++) mx4[j] = max3(mx4[j], s[i + 2 * j], s[i + 2 * j + 1]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) mx4[j] = fmaxf(mx4[j], s[124 + j]);
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
             const float mn = fmaxf(m, mx);
             if (first) {
               m = mn;
@@ -609,52 +758,28 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (!ok) break;
           const float neg = m == -INFINITY ? 0.0f : -m * c;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const u64 neg2 = pack2(neg, neg);
+          u64 sum[2] = {0, 0};
 #pragma unroll
           for (int q = 0; q < 4; q++) {
             uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const float x = ex2(__fmaf_rn(s[32 * q + 2 * i], c, neg)), y = ex2(__fmaf_rn(s[32 * q + 2 * i + 1], c, neg));
-              sum[(i & 1) * 2] += x;
-              sum[(i & 1) * 2 + 1] += y;
-              pk[i] = pack_bf16(x, y);
-            }
+            if (edge) probs32<0>(s + 32 * q, c2, neg2, sum, pk);
+            else probs32<kPolyPairs>(s + 32 * q, c2, neg2, sum, pk);
             tm_store16(sb + 16 * q, pk);
+            if (q & 1) announce(q >> 1);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          float s0, s1;
+          unpack2(add2(sum[0], sum[1]), s0, s1);
+          l += s0 + s1;
         } else {
           uint32_t z[32];
 #pragma unroll
           for (int i = 0; i < 32; i++) z[i] = 0;
           tm_store32(sb, z);
           tm_store32(sb + 32, z);
+          announce(0);
+          announce(1);
         }
-        // V rows that hold no key of the request (stale) are zeroed before their product
-        const int tail = it.len - k0, front = it.klo - k0;
-        if ((tail < kKeyTile || front > 0) && (alt || h == 0)) {
-          if (D == 256 && t > 0) {  // (then the ring position read below is this tile's)
-            if (!(ok = sums_done(t - 1))) break;
-          }
-          const uint32_t rv = ring0 + (uint32_t)(NC * v_index(t, n, alt ? 2 : 1));
-          const int z0 = front > 0 ? front : 0, z1 = tail < kKeyTile ? tail : kKeyTile;
-          for (int cc = 0; cc < NC && ok; cc++) {
-            const uint32_t st = (rv + cc) % kStages;
-            if (!(ok = wait(kBarFull + st, ((rv + cc) / kStages) & 1))) break;
-            unsigned char* vb = gbase + kOffRing + st * kChunk;
-            for (int i = r; i < 128 * 16; i += 128) {  // (row, 16 bytes of its two swizzle rows)
-              const int row = i >> 4, q = i & 15;
-              if (row < z0 || row >= z1)
-                *reinterpret_cast<uint4*>(vb + (q >> 3) * kSub + row * 128 + (q & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-          }
-          if (!ok) break;
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        wait_st();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(bar(kBarP + b));
       }
       if (!ok) break;
       ring0 += (uint32_t)(2 * NC * n);
@@ -682,7 +807,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (Q is loaded over it next)
           __syncwarp();
-          if (lane == 0) bar_arrive(bar(kBarMerge));
+          if (lane == 0) {
+            bar_arrive(bar(kBarMerge));
+            bar_arrive(bar(kBarQEmpty));
+          }
         }
         continue;
       }
@@ -703,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (any_valid) {
         const float inv = 1.0f / l;
-        const int64_t prow = (int64_t)(it.part + local * g + r % g) * p.nkv + kvh;
+        const int64_t prow = (int64_t)(it.part + local * g + head_row) * p.nkv + kvh;
 #pragma unroll
         for (int i = 0; i < D / 32; i++) {
           float o[32];
@@ -717,19 +845,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (valid && it.part < 0) {
             uint16_t* dst = p.out + tok * p.o_tok + head * p.o_head + 32 * i;
+            uint32_t v[16];
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (l != 0.0f)  // (no key at all: zero)
-                v = make_uint4(pack_bf16(o[j] * inv, o[j + 1] * inv), pack_bf16(o[j + 2] * inv, o[j + 3] * inv),
-                               pack_bf16(o[j + 4] * inv, o[j + 5] * inv), pack_bf16(o[j + 6] * inv, o[j + 7] * inv));
-              *reinterpret_cast<uint4*>(dst + j) = v;
-            }
+            for (int j = 0; j < 16; j++)  // (no key at all: zero)
+              v[j] = l != 0.0f ? pack_bf16(o[2 * j] * inv, o[2 * j + 1] * inv) : 0;
+            store32(dst, v, args.wide);
+            store32(dst + 16, v + 8, args.wide);
           } else if (valid && l != 0.0f) {
             float* dst = p.part_o + prow * D + 32 * i;
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<float4*>(dst + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            for (int j = 0; j < 32; j += 8) store32(dst + j, reinterpret_cast<const uint32_t*>(o) + j, true);
           }
           __syncwarp();  // (the next load is the whole warp's)
         }

@@ -18,6 +18,7 @@ static int attn_launch(const paged::AttnArgs& p, int64_t wait_ns, cudaStream_t s
   t.a = p;
   t.piece = p.bs & -p.bs;
   if (t.piece > paged::kKeyTile) t.piece = paged::kKeyTile;
+  t.wide = p.o_tok % 16 == 0 && p.o_head % 16 == 0 && aligned(p.out, 32);
   t.limit_ns = wait_ns < 0 ? paged::tc::kWaitNs : (unsigned long long)wait_ns;
   const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const uint64_t rows = (uint64_t)p.num_blocks * p.nkv * p.bs;
@@ -39,7 +40,9 @@ static int attn_launch(const paged::AttnArgs& p, int64_t wait_ns, cudaStream_t s
   const int st = launch(paged::tc::attn_kernel<D>, dim3(grid), dim3(paged::tc::kThreads), paged::tc::kSmemBytes,
                         stream, mq, mk, mv, t);
   if (st) return st;
-  const int cgrid = (int)std::min<int64_t>((int64_t)p.lay.max_entries * p.nkv, 4LL * num_sms());
+  // one row of a join per warp and pass; the device knows how many there are
+  const int64_t join_rows = (int64_t)p.lay.max_entries * p.nkv * std::min(p.lay.tile_tok, p.tokens) * g;
+  const int cgrid = (int)std::min<int64_t>((join_rows + 7) / 8, 4LL * num_sms());
   return launch(paged::combine_kernel<D>, dim3(cgrid), dim3(256), 0, stream, p);
 }
 
@@ -162,7 +165,7 @@ int spark_attn_paged(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_str
   if (num_blocks * nkv * block_size > 0x7fffffffLL - 128) return SPARK_ERR_TOO_LARGE;
   if (q_tok_stride % 8 || q_head_stride % 8 || out_tok_stride % 8 || out_head_stride % 8 || !aligned(q, 16) ||
       !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(out, 16) || !aligned(plan, 16) ||
-      !aligned(part_o, 16) || !aligned(part_ml, 8))
+      !aligned(part_o, 32) || !aligned(part_ml, 8))
     return SPARK_ERR_ALIGNMENT;
   paged::AttnArgs p;
   memset(&p, 0, sizeof(p));

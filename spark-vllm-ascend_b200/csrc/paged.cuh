@@ -303,7 +303,9 @@ struct alignas(16) Entry {  // rows to join: tokens tok0 .. tok0 + ntok - 1, par
 };
 
 struct Header {
-  int items, entries, kind, part_rows, reqs, tokens, window, pad[9];
+  int items, entries, kind, part_rows, reqs, tokens, window;
+  int join_rows;  // rows of the largest entry
+  int pad[8];
 };
 
 struct Layout {
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
   __shared__ long long ws2[kAttnPlanThreads / 32][2];
   __shared__ int ws[kAttnPlanThreads / 32];
   __shared__ int hist[kBins];
-  __shared__ int entries_s, rows_s, bad_s;
+  __shared__ int entries_s, rows_s, bad_s, join_s;
   const int tid = threadIdx.x, R = p.reqs;
   Header* hdr = reinterpret_cast<Header*>(p.plan);
   Item* items = reinterpret_cast<Item*>(p.plan + p.lay.items);
@@ -422,7 +424,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
   int2* bases = reinterpret_cast<int2*>(p.plan + p.lay.bases);  // (first partial row, parts)
   int* lens = reinterpret_cast<int*>(p.plan + p.lay.lens);
   pdl_wait();
-  if (tid == 0) entries_s = rows_s = bad_s = 0;
+  if (tid == 0) entries_s = rows_s = bad_s = join_s = 0;
   __syncthreads();
   const bool prefix_kind = p.prefix_len != nullptr;
   int prefix = 0, npre = 0, nt = 0;
@@ -520,6 +522,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
         if (parts && !prefix_kind) {
           const int e = atomicAdd(&entries_s, 1);
           entries[e] = {t.tok0, t.ntok, base, np, t.ntok * g, 0, 0, 0};
+          atomicMax(&join_s, t.ntok * g);
         }
       }
       for (int k = 0; k < np; k++) {
@@ -561,6 +564,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
     hdr->entries = prefix_kind ? R : entries_s;
     hdr->kind = prefix_kind ? kPrefixPlan : kPromptPlan;
     hdr->part_rows = rows_s;
+    hdr->join_rows = prefix_kind ? p.nq / p.nkv : join_s;
     hdr->reqs = R;
     hdr->tokens = p.tokens;
     hdr->window = p.window;
@@ -601,42 +605,68 @@ __device__ __forceinline__ int2 row_keys(const Item& it, const int* lens, int wi
 // Join of the parts of cut tiles: with M = max m_i over a row's parts,
 //   out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i,
 // the parts in list order whatever order they were computed in.  A row without any key is
-// zero.  One warp per row.
+// zero.  One warp per row: lanes hold 32 parts' (m, l) at a time, then the warp adds the
+// parts' sums, four in flight.
 template <int D>
 __global__ void __launch_bounds__(256) combine_kernel(AttnArgs p) {
-  constexpr int E = D / 32;
+  constexpr int E = D / 32;  // elements of a lane, contiguous
   pdl_wait();
   const Header* hdr = reinterpret_cast<const Header*>(p.plan);
   const Entry* entries = reinterpret_cast<const Entry*>(p.plan + p.lay.entries);
-  const int g = p.nq / p.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = hdr->entries;
-  for (int64_t w = blockIdx.x; w < (int64_t)n * p.nkv; w += gridDim.x) {
-    const Entry en = entries[w / p.nkv];
-    const int kvh = (int)(w % p.nkv);
-    for (int row = warp; row < en.ntok * g; row += 8) {
-      const int tok = en.tok0 + row / g, head = kvh * g + row % g;
-      if (tok >= p.tokens) continue;
-      float M = -INFINITY, l = 0.0f, o[E];
+  const int g = p.nq / p.nkv, lane = threadIdx.x & 31;
+  const int n = hdr->entries, jr = hdr->join_rows;
+  const int64_t total = (int64_t)n * p.nkv * jr, step = (int64_t)gridDim.x * 8;
+  for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += step) {
+    const int row = (int)(w % jr);
+    const int64_t x = w / jr;
+    const int kvh = (int)(x % p.nkv);
+    const Entry en = entries[x / p.nkv];
+    const int tok = en.tok0 + row / g, head = kvh * g + row % g;
+    if (row >= en.ntok * g || tok >= p.tokens) continue;
+    const int parts = en.n_a + en.n_b;
+    auto index = [&](int k) {
+      const int64_t r = k < en.n_a ? en.base_a + (int64_t)k * en.stride_a
+                                   : en.base_b + (int64_t)(k - en.n_a) * en.stride_b;
+      return (r + row) * p.nkv + kvh;
+    };
+    float M = -INFINITY, l = 0.0f, o[E];
 #pragma unroll
-      for (int e = 0; e < E; e++) o[e] = 0.0f;
-      const int parts = en.n_a + en.n_b;
-      for (int k = 0; k < parts; k++) {
-        const int64_t r = k < en.n_a ? en.base_a + (int64_t)k * en.stride_a
-                                     : en.base_b + (int64_t)(k - en.n_a) * en.stride_b;
-        const int64_t pr = (r + row) * p.nkv + kvh;
-        const float2 ml = p.part_ml[pr];
-        if (ml.y == 0.0f) continue;  // no key in this part (its sums are not written)
-        const float mn = fmaxf(M, ml.x);
-        const float a = exp2f(M - mn), b = exp2f(ml.x - mn);
-        M = mn;
-        l = l * a + ml.y * b;
+    for (int e = 0; e < E; e++) o[e] = 0.0f;
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+      // (parts without a key for this row have l = 0: their sums were not written)
+      const float2 ml = k0 + lane < parts ? p.part_ml[index(k0 + lane)] : make_float2(-INFINITY, 0.0f);
+      const float mn = fmaxf(M, warp_max(ml.y != 0.0f ? ml.x : -INFINITY));
+      const float wt = ml.y != 0.0f ? exp2f(ml.x - mn) : 0.0f;
+      const float a = M == -INFINITY ? 0.0f : exp2f(M - mn);
+      M = mn;
+      l = l * a + butterfly_sum<32>(wt * ml.y);
 #pragma unroll
-        for (int e = 0; e < E; e++) o[e] = o[e] * a + p.part_o[pr * D + lane * E + e] * b;
+      for (int e = 0; e < E; e++) o[e] *= a;
+      const int m = parts - k0 < 32 ? parts - k0 : 32;
+      for (int k = 0; k < m; k += 4) {
+        float v[4][E], f[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          f[j] = __shfl_sync(0xffffffffu, wt, (k + j) & 31);
+          const bool use = k + j < m && f[j] != 0.0f;
+          const float4* src = reinterpret_cast<const float4*>(p.part_o + index(k0 + k + j) * D + lane * E);
+#pragma unroll
+          for (int e = 0; e < E; e += 4) {
+            const float4 t = use ? src[e / 4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            v[j][e] = t.x, v[j][e + 1] = t.y, v[j][e + 2] = t.z, v[j][e + 3] = t.w;
+          }
+          if (!use) f[j] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int e = 0; e < E; e++) o[e] = __fmaf_rn(v[j][e], f[j], o[e]);
       }
-      const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
-#pragma unroll
-      for (int e = 0; e < E; e++) p.out[tok * p.o_tok + head * p.o_head + lane * E + e] = f2bf(o[e] * inv);
     }
+    const float inv = 1.0f / l;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + tok * p.o_tok + head * p.o_head + lane * E);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) dst[e / 2] = l != 0.0f ? pack_bf16(o[e] * inv, o[e + 1] * inv) : 0;
   }
 }
 
