@@ -12,17 +12,21 @@
 // Persistent, warp-specialized, one CTA per SM; the CTA walks the plan's items (paged.cuh),
 // longest first, CTA order reversed every other pass so that loads even out.  A tile has
 // the query tokens' g heads as rows, so the K / V of a kv head are read once for the whole
-// group.  384 threads:
-//   warps 0-3, 4-7  softmax of accumulator halves 0 / 1, a thread owning one row: scores
-//                   from tensor memory, maximum, p to tensor memory (as the next product's
-//                   A operand) and the item's epilogue;
-//   warp 8          K / V producer: page ids of 32 pieces at a time, one TMA copy per page
+// group.  640 threads:
+//   warps 0-15      softmax: scores from tensor memory, maximum, p to tensor memory (as the
+//                   next product's A operand) and the item's epilogue.  Warpgroups 0, 1 take
+//                   accumulator half 0 and 2, 3 half 1 (head_dim 256: all four the one
+//                   half); a half's warpgroups share its rows and split the columns, the
+//                   rows' maxima meeting in shared memory.  Four such warps per scheduler
+//                   instead of two: one alone issues every fourth cycle at best;
+//   warp 16         K / V producer: page ids of 32 pieces at a time, one TMA copy per page
 //                   piece and 64 columns into the ring, 128-byte swizzle;
-//   warp 9          owns the tensor memory; one lane issues all MMAs and commits;
-//   warp 10         Q of the next item, as soon as the last score product has read the
-//                   buffer (warp 11 only completes the register split).
+//   warp 17         owns the tensor memory; one lane issues all MMAs and commits;
+//   warp 18         the next item's description and Q, as soon as the last score product has
+//                   read the buffer (warp 19 only completes the register split).
 // Shared memory: Q 64 KB, a ring of five 32-KB chunks (128 keys x 128 columns of K or V).
-// Tensor memory: scores S0 S1 (128 columns each, p written over them), sums O0 O1.
+// Tensor memory: scores S0 S1 (128 columns each; the p of 32 keys are written over the first
+// half of their scores' columns, which no other warp reads), sums O0 O1.
 //
 // Three ways through one loop:
 //   head_dim 128, many rows: half h has its own 128 rows, S_h, O_h; every K / V chunk is
@@ -58,23 +62,24 @@ namespace spark {
 namespace paged {
 namespace tc {
 
-constexpr int kThreads = 384;
-// registers: 168 a thread at launch; warps 8-11 give up 80 each, the softmax warps take 40
-// (2 x 208 + 88 = 3 x 168)
-constexpr int kRegsSoftmax = 208, kRegsRest = 88;
-constexpr int kProducerWarp = 8, kMmaWarp = 9, kQWarp = 10;
+constexpr int kThreads = 640;
+// registers: 96 a thread at launch; warps 16-19 give up 32 each, the softmax warps take 8
+// (4 x 104 + 64 = 5 x 96)
+constexpr int kRegsLaunch = 96, kRegsSoftmax = 104, kRegsRest = 64;
+constexpr int kSoftmaxWarps = 16;
+constexpr int kProducerWarp = 16, kMmaWarp = 17, kQWarp = 18;
 constexpr int kStages = 5;
 constexpr int kChunk = 32 * 1024;  // 128 keys x 128 columns
 constexpr int kSub = 16 * 1024;    // 128 keys x 64 columns (one swizzle row of 128 bytes)
 constexpr int kOffRing = 64 * 1024;
-constexpr int kOffMl = kOffRing + kStages * kChunk;  // few rows: (m, l) of half 1
-constexpr int kOffBar = kOffMl + 128 * 8;
+constexpr int kOffX = kOffRing + kStages * kChunk;  // row values shared by a half's warpgroups: [4][128]
+constexpr int kOffBar = kOffX + 4 * 128 * 4;
 constexpr int kBarFull = 0, kBarEmpty = kBarFull + kStages, kBarQFull = kBarEmpty + kStages,
               kBarQEmpty = kBarQFull + 1, kBarS = kBarQEmpty + 1, kBarP = kBarS + 2, kBarP2 = kBarP + 2, kBarO = kBarP2 + 2,
-              kBarPV = kBarO + 2, kBarMerge = kBarPV + 2, kBarDrain = kBarMerge + 1, kNumBars = kBarDrain + 1;
+              kBarPV = kBarO + 2, kBarMerge = kBarPV + 2, kBarX = kBarMerge + 1, kBarDrain = kBarX + 8, kNumBars = kBarDrain + 1;
 constexpr int kOffMisc = kOffBar + 8 * kNumBars;  // tensor-memory base, abort flag, drained flag
 constexpr int kOffItem = (kOffMisc + 16 + 15) / 16 * 16;  // the current item and its kv head
-constexpr int kSmemBytes = kOffItem + 64 + 1024;  // + 1024-byte alignment slack
+constexpr int kSmemBytes = kOffItem + 64;
 constexpr int kTmemCols = 512;
 constexpr int kColS = 0, kColO = 256;
 constexpr unsigned long long kWaitNs = 500ull * 1000 * 1000;
@@ -164,6 +169,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(id), "r"(accum)
       : "memory");
 }
+// true in one lane of the (converged) warp, the same one every time
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(e));
+  return e != 0;
+}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -189,6 +200,20 @@ __device__ __forceinline__ void tm_wait32(float* v) {
                  "+r"(u[15]), "+r"(u[16]), "+r"(u[17]), "+r"(u[18]), "+r"(u[19]), "+r"(u[20]), "+r"(u[21]),
                  "+r"(u[22]), "+r"(u[23]), "+r"(u[24]), "+r"(u[25]), "+r"(u[26]), "+r"(u[27]), "+r"(u[28]),
                  "+r"(u[29]), "+r"(u[30]), "+r"(u[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tm_load16(uint32_t addr, float* v) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]),
+                 "+r"(u[8]), "+r"(u[9]), "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]),
+                 "+r"(u[15])
                :
                : "memory");
 }
@@ -331,11 +356,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int NC = D / 128;  // chunks per K or V tile
   const AttnArgs& p = args.a;
   const unsigned long long limit_ns = args.limit_ns;
-  extern __shared__ unsigned char smem_raw[];
-  const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
-  const uint32_t pad = ((raw + 1023u) & ~1023u) - raw;
-  const uint32_t base = raw + pad;
-  unsigned char* gbase = smem_raw + pad;
+  // (swizzled tiles want 1024-byte alignment; there is no room for slack, and no static
+  // shared memory in front: checked once, all threads together)
+  extern __shared__ __align__(1024) unsigned char gbase[];
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(gbase);
+  if (base & 1023u) {
+    if (threadIdx.x == 0) atomicOr(p.error, 1);
+    return;
+  }
   const uint32_t bars = base + kOffBar;
   const uint32_t tslot = base + kOffMisc;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + kOffMisc + 4);
@@ -353,15 +381,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(bar(kBarEmpty + s), 1);
     }
     bar_init(bar(kBarQFull), 1);
-    bar_init(bar(kBarQEmpty), D == 128 ? 9 : 5);  // the last score product's commit, the softmax warps
+    bar_init(bar(kBarQEmpty), 1 + kSoftmaxWarps);  // the last score product's commit, the softmax warps
     for (int h = 0; h < 2; h++) {
       bar_init(bar(kBarS + h), 1);
-      bar_init(bar(kBarP + h), 4);
-      bar_init(bar(kBarP2 + h), 4);
+      bar_init(bar(kBarP + h), 8);
+      bar_init(bar(kBarP2 + h), 8);
       bar_init(bar(kBarO + h), 1);
       bar_init(bar(kBarPV + h), 1);
     }
-    bar_init(bar(kBarMerge), 4);
+    bar_init(bar(kBarMerge), 8);
+    for (int i = 0; i < 8; i++) bar_init(bar(kBarX + i), D == 128 ? 2 : 4);
     bar_init(bar(kBarDrain), 1);
     *abort_flag = 0;
     *drained_flag = 1;
@@ -385,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // (each warpgroup changes its share inside its own branch, where the register allocator
   // can tell which share holds)
-  if (warp >= 8) {
+  if (warp >= kSoftmaxWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
     if (warp == kProducerWarp) {
       // ---------------------------------------------------------------- K / V producer
@@ -506,47 +535,64 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     } else if (warp == kMmaWarp) {
       // ---------------------------------------------------------------- MMA issuer
-      if (lane == 0) {
+      // (the whole warp walks the loop, so that addresses and descriptors are warp-uniform
+      // values in uniform registers; one lane, always the same, issues.  Issued from a
+      // one-lane branch instead, an MMA took about 80 cycles to hand over.)
+      {
         uint32_t ring = 0, qi = 0, np[2] = {0, 0};
         bool ok = true;
-        auto full = [&](uint32_t r) {
-          return bar_wait(bar(kBarFull + r % kStages), (r / kStages) & 1, limit_ns, abort_flag);
+        auto wait = [&](int i, uint32_t parity) -> bool {
+          return __all_sync(0xffffffffu, bar_wait(bar(i), parity, limit_ns, abort_flag));
+        };
+        auto full = [&](uint32_t r) -> bool {
+          return wait(kBarFull + r % kStages, (r / kStages) & 1);
         };
         auto stage = [&](uint32_t r) { return base + kOffRing + (r % kStages) * kChunk; };
         // S_h = Q_q K^T of the tile whose first chunk is r
         auto scores = [&](int h, int q, uint32_t r) {
 #pragma unroll
           for (int c = 0; c < NC; c++) {
-            const uint32_t kb = stage(r + c), qb = base + (uint32_t)(q * kChunk + c * kChunk);
+            const uint64_t kd = desc_k(stage(r + c)), qd = desc_k(base + (uint32_t)(q * kChunk + c * kChunk));
+            if (elect_one()) {
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-              mma_ss(tmem + kColS + h * 128, desc_k(qb + (j >> 2) * kSub) + 2 * (j & 3),
-                     desc_k(kb + (j >> 2) * kSub) + 2 * (j & 3), kIdescS, (c | j) != 0);
+              for (int j = 0; j < 8; j++) {
+                const uint32_t off = (uint32_t)((j >> 2) * (kSub >> 4) + 2 * (j & 3));
+                mma_ss(tmem + kColS + h * 128, qd + off, kd + off, kIdescS, (c | j) != 0);
+              }
+              if (c == NC - 1) commit(bar(kBarS + h));
+            }
+            __syncwarp();
           }
-          commit(bar(kBarS + h));
         };
         // O += P_h V of the tile whose first chunk is r, in two steps: the first 64 keys'
         // probabilities are multiplied while the others are still computed
-        auto sums = [&](int h, int o, uint32_t r, uint32_t accum) {
+        auto sums = [&](int h, int o, uint32_t r, uint32_t accum) -> bool {
 #pragma unroll
           for (int k = 0; k < 2; k++) {
-            if (!bar_wait(bar((k ? kBarP2 : kBarP) + h), np[h] & 1, limit_ns, abort_flag)) return false;
+            if (!wait((k ? kBarP2 : kBarP) + h, np[h] & 1)) return false;
             fence_after();
 #pragma unroll
             for (int c = 0; c < NC; c++) {
               const uint64_t vd = desc_v(stage(r + c));
+              if (elect_one()) {
 #pragma unroll
-              for (int j = 4 * k; j < 4 * k + 4; j++)
-                mma_ts(tmem + kColO + (o + c) * 128, tmem + kColS + h * 128 + j * 8, vd + j * (2048 >> 4), kIdescO,
-                       accum | (j != 0));
+                for (int j = 4 * k; j < 4 * k + 4; j++)
+                  mma_ts(tmem + kColO + (o + c) * 128, tmem + kColS + h * 128 + 32 * (j >> 1) + 8 * (j & 1),
+                         vd + j * (2048 >> 4), kIdescO, accum | (j != 0));
+              }
+              __syncwarp();
             }
           }
           np[h]++;
           return true;
         };
+        auto announce = [&](int i) {
+          if (elect_one()) commit(bar(i));
+          __syncwarp();
+        };
         auto release = [&](uint32_t r) {
 #pragma unroll
-          for (int c = 0; c < NC; c++) commit(bar(kBarEmpty + (r + c) % kStages));
+          for (int c = 0; c < NC; c++) announce(kBarEmpty + (r + c) % kStages);
         };
         auto full_tile = [&](uint32_t r) {
           bool f = full(r);
@@ -555,13 +601,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         const Item* slot = reinterpret_cast<const Item*>(gbase + kOffItem);
         while (ok) {
-          ok = bar_wait(bar(kBarQFull), qi++ & 1, limit_ns, abort_flag);
+          ok = wait(kBarQFull, qi++ & 1);
           if (!ok) break;
-          const int n = slot->nkt;
-          const bool few = D == 128 && (slot->flags & kFlagFew);
+          const int n = __shfl_sync(0xffffffffu, slot->nkt, 0);
+          const bool few = D == 128 && (__shfl_sync(0xffffffffu, slot->flags, 0) & kFlagFew);
           if (n < 0) break;
           if (n == 0) {
-            bar_arrive(bar(kBarQEmpty));
+            if (lane == 0) bar_arrive(bar(kBarQEmpty));
             continue;
           }
           if (D == 128 && !few) {
@@ -570,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             scores(0, 0, ring);
             scores(1, 1, ring);
             release(ring);
-            if (n == 1) commit(bar(kBarQEmpty));
+            if (n == 1) announce(kBarQEmpty);
             ring++;
             for (int t = 0; t < n && ok; t++) {
               const uint32_t rv = ring, rk = ring + 1;
@@ -583,12 +629,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                   fence_after();
                 }
                 if (more) scores(h, h, rk);
-                else commit(bar(kBarO + h));
+                else announce(kBarO + h);
               }
               if (!ok) break;
               release(rv);
               if (more) release(rk);
-              if (t + 2 == n) commit(bar(kBarQEmpty));
+              if (t + 2 == n) announce(kBarQEmpty);
               ring += more ? 2 : 1;
             }
           } else {
@@ -600,11 +646,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               ring += NC;
             }
             if (!ok) break;
-            if (n <= 2) commit(bar(kBarQEmpty));
+            if (n <= 2) announce(kBarQEmpty);
             for (int t = 0; t < n; t++) {
               const int h = t & 1;
               if (!(ok = full_tile(ring) && sums(h, D == 128 ? h : 0, ring, D == 128 ? t > 1 : t > 0))) break;
-              if (D == 256) commit(bar(kBarPV + h));
+              if (D == 256) announce(kBarPV + h);
               release(ring);
               ring += NC;
               if (t + 2 < n) {
@@ -613,17 +659,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 scores(h, 0, ring);
                 release(ring);
                 ring += NC;
-                if (t + 3 == n) commit(bar(kBarQEmpty));
+                if (t + 3 == n) announce(kBarQEmpty);
               }
             }
             if (!ok) break;
-            commit(bar(kBarO));  // after the whole item: the merge may then overwrite Q
-            if (D == 128 && n > 1) commit(bar(kBarO + 1));
+            announce(kBarO);  // after the whole item: the merge may then overwrite Q
+            if (D == 128 && n > 1) announce(kBarO + 1);
           }
         }
-        if (!ok) fail();
-        commit(bar(kBarDrain));  // tracks every MMA issued before it
-        if (!bar_wait(bar(kBarDrain), 0, kDrainNs, nullptr)) {
+        if (!ok && lane == 0) fail();
+        announce(kBarDrain);  // tracks every MMA issued before it
+        if (!bar_wait(bar(kBarDrain), 0, kDrainNs, nullptr) && lane == 0) {
           atomicOr(p.error, 2);
           *drained_flag = 0;
         }
@@ -633,23 +679,39 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ---------------------------------------------------------------- softmax and epilogue
-    const int h = warp >> 2, r = tid & 127;
+    // SP warpgroups share the rows of a half (a thread of each owns the same row), 128 / SP
+    // score columns and 64 sum columns each
+    constexpr int SP = D == 128 ? 2 : 4, NQ = 4 / SP;
+    const int wg = warp >> 2, h = D == 128 ? wg >> 1 : 0, sp = D == 128 ? wg & 1 : wg, r = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const int* lens = reinterpret_cast<const int*>(p.plan + p.lay.lens);
     const float c = p.scale * kLog2e;
-    float2* ml_s = reinterpret_cast<float2*>(gbase + kOffMl);
+    const u64 c2 = pack2(c, c);
+    float* xs = reinterpret_cast<float*>(gbase + kOffX) + h * SP * 128 + r;  // [warpgroup][row]
     float* o_s = reinterpret_cast<float*>(gbase);  // few rows: half 1's sums, [column][row]
-    uint32_t ns[2] = {0, 0}, no = 0, nm = 0, npv[2] = {0, 0}, ring0 = 0;
-    bool ok = true;
+    const int xbar = kBarX + h * 4 + (warp & 3);
+    uint32_t ns[2] = {0, 0}, no = 0, nm = 0, npv[2] = {0, 0}, ring0 = 0, qi = 0, nx = 0;
+    bool ok = true, unread = false;
     auto wait = [&](int i, uint32_t parity) {
       return __all_sync(0xffffffffu, bar_wait(bar(i), parity, limit_ns, abort_flag));
     };
+    // xs[128 j] = warpgroup j's value, for all j.  The next values overwrite these: within an
+    // item they follow the scores of the next tile, which every partner's probabilities
+    // precede; behind the item's last exchange each warp reports that it has read them
+    // (unread: that report is still to be awaited).
+    auto exchange = [&](float v) -> bool {
+      if (unread) {
+        if (!wait(xbar, nx++ & 1)) return false;
+        unread = false;
+      }
+      xs[128 * sp] = v;
+      __syncwarp();
+      if (lane == 0) bar_arrive(bar(xbar));
+      return wait(xbar, nx++ & 1);
+    };
     const int local_row = r / g, head_row = r % g;
     const bool row_used = r < g * p.lay.half_tok;
-    const u64 c2 = pack2(c, c);
-    uint32_t qi = 0;
-    // (head_dim 256: one softmax, by half 0)
-    while (ok && (D == 128 || h == 0)) {
+    while (ok) {
       if (!(ok = wait(kBarQFull, qi++ & 1))) break;
       const Item it = *reinterpret_cast<const Item*>(gbase + kOffItem);
       const int kvh = *reinterpret_cast<const int*>(gbase + kOffItem + sizeof(Item));
@@ -659,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int local = local_row + (D == 128 && !few ? h * p.lay.half_tok : 0);
       const int tok = it.tok0 + local, head = kvh * g + head_row;
       const bool valid = row_used && local < it.ntok && tok < p.tokens;
-      int2 kk = valid ? row_keys(it, lens, p.window, local) : make_int2(0, 0);
+      const int2 kk = valid ? row_keys(it, lens, p.window, local) : make_int2(0, 0);
       const bool any_valid = __any_sync(0xffffffffu, valid);
       // keys that some row (lo0, hi1) / every row (lo1, hi0) of the warp sees
       const int lo0 = warp_min_i(valid ? kk.x : INT_MAX), lo1 = -warp_min_i(valid ? -kk.x : INT_MAX);
@@ -670,11 +732,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the scores of tile t, and those of tile t + 2 cannot have begun.
       auto sums_done = [&](int t) { return wait(kBarPV + (t & 1), (npv[t & 1] + (uint32_t)(t >> 1)) & 1); };
       float m = -INFINITY, l = 0.0f;
-      // this half is done with the item slot, and with Q's buffer unless sums pass through it
+      // this warp is done with the item slot, and with Q's buffer unless sums pass through it
       if (n == 0 || !few || (h == 1 && n == 1)) {
         __syncwarp();
         if (lane == 0) bar_arrive(bar(kBarQEmpty));
       }
+      const uint32_t ob = lanes + kColO + (D == 128 ? h * 128 : 0) + sp * 64;
       for (int t = few ? h : 0; t < n; t += few ? 2 : 1) {
         const int b = D == 256 ? (t & 1) : h;  // score buffer
         const bool first = few ? t < 2 : t == 0;
@@ -694,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t st = (rv + cc) % kStages;
             if (!(ok = wait(kBarFull + st, ((rv + cc) / kStages) & 1))) break;
             unsigned char* vb = gbase + kOffRing + st * kChunk;
-            for (int i = r; i < 128 * 16; i += 128) {  // (row, 16 bytes of its two swizzle rows)
+            for (int i = sp * 128 + r; i < 128 * 16; i += SP * 128) {  // (row, 16 bytes of its two swizzle rows)
               const int row = i >> 4, q = i & 15;
               if (row < z0 || row >= z1)
                 *reinterpret_cast<uint4*>(vb + (q >> 3) * kSub + row * 128 + (q & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -712,32 +775,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         if (any_valid && k0 < hi1 && k0 + kKeyTile > lo0) {
           const bool edge = k0 < lo1 || k0 + kKeyTile > hi0;  // some row sees a part of the tile only
-          float s[128];
-          for (;;) {  // (a second time after a rescale: the scores are not kept over it)
-#pragma unroll
-            for (int i = 0; i < 4; i++) tm_load32(sb + 32 * i, s + 32 * i);
-#pragma unroll
-            for (int i = 0; i < 4; i++) tm_wait32(s + 32 * i);
+          const int col0 = kk.x - k0 - 32 * sp, cols = kk.y - kk.x;
+          float s[32];
+          auto load = [&](int q) {
+            tm_load32(sb + 64 * q + 32 * sp, s);
+            tm_wait32(s);
             if (edge) {
-              const int a = kk.x - k0, z = kk.y - kk.x;
 #pragma unroll
-              for (int i = 0; i < 128; i++) s[i] = z > 0 && (uint32_t)(i - a) < (uint32_t)z ? s[i] : -INFINITY;
+              for (int i = 0; i < 32; i++)
+                s[i] = cols > 0 && (uint32_t)(i + 64 * q - col0) < (uint32_t)cols ? s[i] : -INFINITY;
             }
-            float mx4[4] = {s[0], s[1], s[2], s[3]};
+          };
+          float mn = -INFINITY;
 #pragma unroll
-            for (int i = 4; i < 124; i += 8) {
+          for (int q = NQ - 1; q >= 0; q--) {  // (the first 32 scores stay for the second pass)
+            load(q);
+            float a = max3(mn, s[0], s[1]), b = max3(s[2], s[3], s[4]);
 #pragma unroll
-              for (int j = 0; j < 4; j++) mx4[j] = max3(mx4[j], s[i + 2 * j], s[i + 2 * j + 1]);
+            for (int i = 5; i < 29; i += 4) {
+              a = max3(a, s[i], s[i + 1]);
+              b = max3(b, s[i + 2], s[i + 3]);
             }
+            mn = max3(fmaxf(a, s[29]), fmaxf(b, s[30]), s[31]);
+          }
+          if (!(ok = exchange(mn))) break;
 #pragma unroll
-            for (int j = 0; j < 4; j++) mx4[j] = fmaxf(mx4[j], s[124 + j]);
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-            const float mn = fmaxf(m, mx);
-            if (first) {
-              m = mn;
-              break;
-            }
-            if (!__any_sync(0xffffffffu, (mn - m) * c > 8.0f)) break;
+          for (int j = 0; j < SP; j++) mn = fmaxf(mn, xs[128 * j]);
+          mn = fmaxf(m, mn);
+          if (first) {
+            m = mn;
+          } else if (__any_sync(0xffffffffu, (mn - m) * c > 8.0f)) {
             const float f = mn == -INFINITY ? 1.0f : ex2((m - mn) * c);
             m = mn;
             l *= f;
@@ -746,39 +813,38 @@ __global__ void __launch_bounds__(kThreads, 1)
               fence_after();
             }
 #pragma unroll 1
-            for (int i = 0; i < D / 32; i++) {
-              float o[32];
-              const uint32_t ob = lanes + kColO + (D == 128 ? h * 128 : 0) + 32 * i;
-              tm_load32(ob, o);
-              tm_wait32(o);
+            for (int i = 0; i < 4; i++) {
+              float o[16];
+              tm_load16(ob + 16 * i, o);
 #pragma unroll
-              for (int j = 0; j < 32; j++) o[j] *= f;
-              tm_store32(ob, reinterpret_cast<const uint32_t*>(o));
+              for (int j = 0; j < 16; j++) o[j] *= f;
+              tm_store16(ob + 16 * i, reinterpret_cast<const uint32_t*>(o));
             }
           }
-          if (!ok) break;
           const float neg = m == -INFINITY ? 0.0f : -m * c;
           const u64 neg2 = pack2(neg, neg);
           u64 sum[2] = {0, 0};
 #pragma unroll
-          for (int q = 0; q < 4; q++) {
+          for (int q = 0; q < NQ; q++) {
             uint32_t pk[16];
-            if (edge) probs32<0>(s + 32 * q, c2, neg2, sum, pk);
-            else probs32<kPolyPairs>(s + 32 * q, c2, neg2, sum, pk);
-            tm_store16(sb + 16 * q, pk);
-            if (q & 1) announce(q >> 1);
+            if (q > 0) load(q);
+            if (edge) probs32<0>(s, c2, neg2, sum, pk);
+            else probs32<kPolyPairs>(s, c2, neg2, sum, pk);
+            tm_store16(sb + 64 * q + 32 * sp, pk);
+            announce(D == 128 ? q : sp >> 1);
           }
           float s0, s1;
           unpack2(add2(sum[0], sum[1]), s0, s1);
           l += s0 + s1;
         } else {
-          uint32_t z[32];
+          uint32_t z[16];
 #pragma unroll
-          for (int i = 0; i < 32; i++) z[i] = 0;
-          tm_store32(sb, z);
-          tm_store32(sb + 32, z);
-          announce(0);
-          announce(1);
+          for (int i = 0; i < 16; i++) z[i] = 0;
+#pragma unroll
+          for (int q = 0; q < NQ; q++) {
+            tm_store16(sb + 64 * q + 32 * sp, z);
+            announce(D == 128 ? q : sp >> 1);
+          }
         }
       }
       if (!ok) break;
@@ -786,24 +852,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       npv[0] += (uint32_t)((n + 1) >> 1);
       npv[1] += (uint32_t)(n >> 1);
       // -------------------------------------------------------------- epilogue
-      const int mine = few ? (n + 1 - h) / 2 : n;
+      const int mine = few ? (n + 1 - h) / 2 : n;  // this half's tiles
       if (mine > 0) {
+        if (any_valid) {  // the row's sum over all columns, added in warpgroup order
+          if (!(ok = exchange(l))) break;
+          l = 0.0f;
+#pragma unroll
+          for (int j = 0; j < SP; j++) l += xs[128 * j];
+          __syncwarp();
+          if (lane == 0) bar_arrive(bar(xbar));
+          unread = true;
+        }
         if (!(ok = wait(kBarO + h, no++ & 1))) break;
         fence_after();
       }
-      const uint32_t ob = lanes + kColO + (D == 128 ? h * 128 : 0);
       if (few && h == 1) {  // hand the odd tiles' sums over
         if (mine > 0) {
           if (any_valid) {
+#pragma unroll 1
+            for (int i = 0; i < 4; i++) {
+              float o[16];
+              tm_load16(ob + 16 * i, o);
 #pragma unroll
-            for (int i = 0; i < D / 32; i++) {
-              float o[32];
-              tm_load32(ob + 32 * i, o);
-              tm_wait32(o);
-#pragma unroll
-              for (int j = 0; j < 32; j++) o_s[(32 * i + j) * 128 + r] = o[j];
+              for (int j = 0; j < 16; j++) o_s[(sp * 64 + 16 * i + j) * 128 + r] = o[j];
             }
-            ml_s[r] = make_float2(m, l);
+            if (!(ok = wait(xbar, nx++ & 1))) break;
+            unread = false;
+            if (sp == 0) {
+              xs[0] = m;
+              xs[128] = l;
+            }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (Q is loaded over it next)
           __syncwarp();
@@ -819,48 +897,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (merge) {
         if (!(ok = wait(kBarMerge, nm++ & 1))) break;
         if (any_valid) {
-          const float2 o1 = ml_s[r];
-          const float M = fmaxf(m, o1.x);
+          const float m1 = xs[SP * 128], l1 = xs[SP * 128 + 128];
+          const float M = fmaxf(m, m1);
           if (M != -INFINITY) {
             f0 = ex2((m - M) * c);
-            f1 = ex2((o1.x - M) * c);
+            f1 = ex2((m1 - M) * c);
           }
-          l = l * f0 + o1.y * f1;
+          l = l * f0 + l1 * f1;
           m = M;
         }
       }
       if (any_valid) {
         const float inv = 1.0f / l;
         const int64_t prow = (int64_t)(it.part + local * g + head_row) * p.nkv + kvh;
-#pragma unroll
-        for (int i = 0; i < D / 32; i++) {
-          float o[32];
-          if (n > 0) {
-            tm_load32(ob + 32 * i, o);
-            tm_wait32(o);
-          }
+#pragma unroll 1
+        for (int i = 0; i < 4; i++) {
+          const int col = sp * 64 + 16 * i;
+          float o[16];
+          if (n > 0) tm_load16(ob + 16 * i, o);
           if (merge) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) o[j] = o[j] * f0 + o_s[(32 * i + j) * 128 + r] * f1;
+            for (int j = 0; j < 16; j++) o[j] = o[j] * f0 + o_s[(col + j) * 128 + r] * f1;
           }
           if (valid && it.part < 0) {
-            uint16_t* dst = p.out + tok * p.o_tok + head * p.o_head + 32 * i;
-            uint32_t v[16];
+            uint32_t v[8];
 #pragma unroll
-            for (int j = 0; j < 16; j++)  // (no key at all: zero)
+            for (int j = 0; j < 8; j++)  // (no key at all: zero)
               v[j] = l != 0.0f ? pack_bf16(o[2 * j] * inv, o[2 * j + 1] * inv) : 0;
-            store32(dst, v, args.wide);
-            store32(dst + 16, v + 8, args.wide);
+            store32(p.out + tok * p.o_tok + head * p.o_head + col, v, args.wide);
           } else if (valid && l != 0.0f) {
-            float* dst = p.part_o + prow * D + 32 * i;
+            float* dst = p.part_o + prow * D + col;
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) store32(dst + j, reinterpret_cast<const uint32_t*>(o) + j, true);
+            for (int j = 0; j < 16; j += 8) store32(dst + j, reinterpret_cast<const uint32_t*>(o) + j, true);
           }
           __syncwarp();  // (the next load is the whole warp's)
         }
-        if (valid && it.part >= 0) p.part_ml[prow] = make_float2(m * c, l);
+        if (valid && it.part >= 0 && sp == 0) p.part_ml[prow] = make_float2(m * c, l);
       }
-      if (few && n > 0) {  // Q's buffer may be loaded once all four warps have read the hand-over
+      if (few && n > 0) {  // Q's buffer may be loaded once all warps have read the hand-over
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) bar_arrive(bar(kBarQEmpty));
