@@ -400,20 +400,24 @@ __device__ __forceinline__ Tile prefix_tile(const AttnPlanArgs& p, const int* le
   return t;
 }
 
-__device__ __forceinline__ int block_sum(int v, int* ws) {
-  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int s = 0;
-  for (int w = 0; w < kAttnPlanThreads / 32; w++) s += ws[w];
-  return s;
+// Cost of a part in quarters of a key tile of many rows: the tiles (alternating halves take
+// two at a time), what an item costs around them, and for a part that is joined the fp32
+// sums of its rows.  Measured with the attention kernel: see there.
+__host__ __device__ inline int part_cost(int flags, int parts, int tiles, int ntok) {
+  return tiles * ((flags & kFlagFew) ? 2 : 4) + 6 + (parts > 1 && !(flags & kFlagFew) ? 6 : 0);
 }
+constexpr int kPriceBins = 256;
+__device__ __forceinline__ int price_bin(int cost, int top) {
+  return min((int)((long long)cost * kPriceBins / (top + 1)), kPriceBins - 1);
+}
+__constant__ int kCuts[32] = {1,  2,  3,  4,  5,  6,  7,  8,  9,  10, 11, 12, 13, 14, 15, 16,
+                              18, 20, 22, 24, 27, 30, 34, 37, 42, 48, 55, 64, 74, 96, 128, 148};
 
 __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArgs p) {
   __shared__ long long ws2[kAttnPlanThreads / 32][2];
   __shared__ int ws[kAttnPlanThreads / 32];
   __shared__ int hist[kBins];
+  __shared__ int price[32 * (kPriceBins + 1)];
   __shared__ int entries_s, rows_s, bad_s, join_s;
   const int tid = threadIdx.x, R = p.reqs;
   Header* hdr = reinterpret_cast<Header*>(p.plan);
@@ -476,37 +480,105 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
     const int q0 = p.query_start[t.x];
     return prompt_tile(p, q0, p.query_start[t.x + 1] - q0, lens[t.x], t.x, t.y);
   };
-  int work = 0;
+  int longest = 0;
   for (int i = tid; i < nt; i += kAttnPlanThreads) {
     if (!prefix_kind) {
       const int r = find_request(starts, R, i);
       tiles[i] = make_int2(r, i - starts[r]);
     }
-    work += tile_at(i).nkt;
+    const int k = tile_at(i).nkt;
+    longest = k > longest ? k : longest;
   }
-  const int total = block_sum(work, ws);
-  // keys a part may have: an even share of the work, or more until the parts fit the buffers
-  const long long share = ((long long)total * p.nkv + kNumSMs - 1) / kNumSMs;
-  int cut = share < 1 ? 1 : (int)share;
-  for (;;) {
+  for (int o = 16; o >= 1; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  if ((tid & 31) == 0) ws[tid >> 5] = longest;
+  __syncthreads();
+  for (int w = 0; w < kAttnPlanThreads / 32; w++) longest = max(longest, ws[w]);
+  // How fine to cut: warp w prices "the longest tile in kCuts[w] parts, the others in parts
+  // no longer than those" by dealing the parts out as the attention kernel will.  (A batch of
+  // more than 8192 tiles balances without.)
+  const int g = p.nq / p.nkv;
+  int cut = longest > 0 ? longest : 1;
+  if (nt <= 8192 && longest > 1) {
+    const int w = tid >> 5, lane = tid & 31;
+    const int c = (longest + kCuts[w] - 1) / kCuts[w];
+    int* h = price + w * (kPriceBins + 1);
+    for (int b = lane; b <= kPriceBins; b += 32) h[b] = 0;
+    const int top = part_cost(0, 2, c, p.lay.tile_tok);  // (no part costs more)
+    __syncwarp();
     int extra = 0, rows = 0;
-    for (int i = tid; i < nt; i += kAttnPlanThreads) {
+    for (int i = lane; i < nt; i += 32) {
       const Tile t = tile_at(i);
-      const int np = (t.nkt + cut - 1) / cut;
-      if (np > 1) extra += np - 1;
-      if (np > 1 || prefix_kind) rows += np * t.ntok;
+      const int np = (t.nkt + c - 1) / c;
+      if (np == 0) continue;
+      extra += np - 1;
+      if (np > 1 || prefix_kind) rows += np * t.ntok * g;
+      const int lo = t.nkt / np, more = t.nkt - lo * np;  // `more` parts have one tile more
+      const int joined = prefix_kind ? 2 : np;
+      const int c0 = part_cost(t.flags, joined, lo, t.ntok), c1 = part_cost(t.flags, joined, lo + 1, t.ntok);
+      if (np > more) atomicAdd(&h[price_bin(c0, top)], (np - more) * p.nkv);
+      if (more) atomicAdd(&h[price_bin(c1, top)], more * p.nkv);
     }
-    const int e = block_sum(extra, ws), rw = block_sum(rows, ws);
-    if ((e <= p.lay.budget && (long long)rw * (p.nq / p.nkv) <= p.lay.part_rows) || cut >= total) break;
-    cut = cut + (cut + 1) / 2;
+    for (int o = 16; o >= 1; o >>= 1) {
+      extra += __shfl_xor_sync(0xffffffffu, extra, o);
+      rows += __shfl_xor_sync(0xffffffffu, rows, o);
+    }
+    __syncwarp();
+    // bin counts -> parts in this bin and above it (costlier), by a suffix scan of 8 bins a lane
+    int mine[kPriceBins / 32], sum = 0;
+    for (int j = kPriceBins / 32 - 1; j >= 0; j--) mine[j] = sum += h[lane * (kPriceBins / 32) + j];
+    int above = sum;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_down_sync(0xffffffffu, above, o);
+      if (lane + o < 32) above += v;
+    }
+    above -= sum;
+    __syncwarp();
+    for (int j = 0; j < kPriceBins / 32; j++) h[lane * (kPriceBins / 32) + j] = mine[j] + above;
+    __syncwarp();
+    const int parts = h[0];
+    // the load of some of the CTAs: lane = round, in the kernel's back-and-forth order
+    int worst = 0;
+    for (int s = 0; s < 8; s++) {
+      const int cta = s * (kNumSMs - 1) / 7;
+      int load = 0;
+      for (int round = lane; (int64_t)round * kNumSMs < parts; round += 32) {
+        const int at = round * kNumSMs + ((round & 1) ? kNumSMs - 1 - cta : cta);
+        if (at >= parts) continue;
+        int lo = 0, hi = kPriceBins - 1;  // largest bin with more than `at` parts in and above it
+        while (lo < hi) {
+          const int m = (lo + hi + 1) >> 1;
+          if (h[m] > at) lo = m;
+          else hi = m - 1;
+        }
+        load += lo + 1;
+      }
+      for (int o = 16; o >= 1; o >>= 1) load += __shfl_xor_sync(0xffffffffu, load, o);
+      worst = max(worst, load);
+    }
+    // bins back to cost (rounded up); what does not fit the buffers is out
+    const bool fits = extra <= p.lay.budget && rows <= p.lay.part_rows;
+    const long long cost = fits ? (long long)worst * top : (1LL << 60);
+    if (lane == 0) {
+      ws2[w][0] = cost;
+      ws2[w][1] = c;
+    }
+    __syncthreads();
+    long long best = ws2[0][0];  // (whole tiles always fit)
+    cut = (int)ws2[0][1];
+    for (int i = 1; i < kAttnPlanThreads / 32; i++)
+      if (ws2[i][0] < best) {
+        best = ws2[i][0];
+        cut = (int)ws2[i][1];
+      }
+    __syncthreads();
   }
   // longest parts first (a counting sort by length; the order inside a length does not
   // matter to any result)
   for (int b = tid; b < kBins; b += kAttnPlanThreads) hist[b] = 0;
   __syncthreads();
-  auto bin_of = [&](const Tile& t, int keys) {
-    const int c = (t.flags & kFlagFew) ? (keys + 1) / 2 : keys;
-    return kBins - 1 - (c < kBins - 1 ? c : kBins - 1);
+  const int top = part_cost(0, 2, cut, p.lay.tile_tok);
+  auto bin_of = [&](const Tile& t, int joined, int keys) {
+    return kBins - 1 - (int)((long long)min(part_cost(t.flags, joined, keys, t.ntok), top) * (kBins - 1) / top);
   };
   for (int pass = 0; pass < 2; pass++) {
     for (int i = tid; i < nt; i += kAttnPlanThreads) {
@@ -516,7 +588,6 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
       const bool parts = np > 1 || prefix_kind;
       int base = -1;
       if (pass == 1) {
-        const int g = p.nq / p.nkv;
         if (parts) base = atomicAdd(&rows_s, np * t.ntok * g);
         bases[i] = make_int2(base, np);
         if (parts && !prefix_kind) {
@@ -527,7 +598,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
       }
       for (int k = 0; k < np; k++) {
         const int a = (int)((long long)k * t.nkt / np), b = (int)((long long)(k + 1) * t.nkt / np);
-        const int slot = atomicAdd(&hist[bin_of(t, b - a)], 1);
+        const int slot = atomicAdd(&hist[bin_of(t, parts ? 2 : 1, b - a)], 1);
         if (pass == 1) {
           Item it;
           it.tok0 = t.tok0, it.ntok = t.ntok, it.pos0 = t.pos0, it.req = t.req;
@@ -536,7 +607,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
           it.klo = a ? it.key0 : t.klo;
           it.khi = k + 1 < np ? t.key0 + b * kKeyTile : t.khi;
           it.len = t.len, it.flags = t.flags;
-          it.part = parts ? base + k * t.ntok * (p.nq / p.nkv) : -1;
+          it.part = parts ? base + k * t.ntok * g : -1;
           it.pad = 0;
           items[slot] = it;
         }
@@ -552,7 +623,6 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
     }
   }
   if (prefix_kind) {
-    const int g = p.nq / p.nkv;
     for (int r = tid; r < R; r += kAttnPlanThreads) {
       const int i = r / p.lay.tile_tok;
       const Tile t = prefix_tile(p, lens, prefix, npre, i);
