@@ -69,7 +69,7 @@ int spark_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int reqs,
   p.counter = counter, p.error = error;
   const int64_t units = std::max<int64_t>(rows, reqs);
   const int grid = (int)std::min<int64_t>((units + paged::kPlanThreads - 1) / paged::kPlanThreads, num_sms());
-  return launch(paged::paged_plan_kernel, dim3(grid), dim3(paged::kPlanThreads), 2 * ((size_t)reqs + 1) * 4,
+  return launch(paged::paged_plan_kernel, dim3(grid), dim3(paged::kPlanThreads), (3 * (size_t)reqs + 2) * 4,
                 as_stream(stream), p);
 }
 
@@ -95,12 +95,13 @@ int spark_qk_norm_rope_store_rows(const uint16_t* qkv, int64_t row_stride, int r
   p.k_cache = k_cache, p.v_cache = v_cache, p.q_out = q_out, p.row_stride = row_stride, p.max_pos = max_pos;
   p.num_slots = num_blocks * block_size, p.eps = eps, p.rows = rows, p.nq = nq, p.nkv = nkv, p.rot = rotary_dim;
   p.bs = block_size, p.error = error;
-  const int per_cta = 256 / (head_dim / 8);
-  const int64_t total = (int64_t)rows * (nq + 2 * nkv);
-  const int grid = (int)std::min<int64_t>((total + per_cta - 1) / per_cta, 8LL * num_sms());
-  if (head_dim == 128)
-    return launch(paged::rope_store_kernel<128>, dim3(grid), dim3(256), 0, as_stream(stream), p);
-  return launch(paged::rope_store_kernel<256>, dim3(grid), dim3(256), 0, as_stream(stream), p);
+  const int lanes = (nq + 2 * nkv) * (head_dim / 16);  // 16 elements a thread
+  const int threads = std::min((lanes + 31) / 32 * 32, paged::kRopeMaxThreads);
+  const int gy = (lanes + threads - 1) / threads;
+  if (gy > 65535) return SPARK_ERR_TOO_LARGE;
+  const dim3 grid(rows, gy);
+  if (head_dim == 128) return launch(paged::rope_store_kernel<128>, grid, dim3(threads), 0, as_stream(stream), p);
+  return launch(paged::rope_store_kernel<256>, grid, dim3(threads), 0, as_stream(stream), p);
 }
 
 // ------------------------------------------------------------------ paged attention

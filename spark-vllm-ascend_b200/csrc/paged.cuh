@@ -60,18 +60,23 @@ __device__ __forceinline__ void block_scan2(long long& a, long long& b, long lon
     ws[warp][1] = b;
   }
   __syncthreads();
-  long long pa = 0, pb = 0;
-  tot[0] = tot[1] = 0;
-  for (int w = 0; w < (int)(blockDim.x >> 5); w++) {
-    if (w < warp) {
-      pa += ws[w][0];
-      pb += ws[w][1];
+  const int nw = blockDim.x >> 5;  // (at most 32 warps: every warp scans their totals)
+  long long x = lane < nw ? ws[lane][0] : 0, y = lane < nw ? ws[lane][1] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) {
+      x += u;
+      y += v;
     }
-    tot[0] += ws[w][0];
-    tot[1] += ws[w][1];
   }
-  a += pa;
-  b += pb;
+  const long long pa = __shfl_sync(0xffffffffu, x, (warp + 31) & 31), pb = __shfl_sync(0xffffffffu, y, (warp + 31) & 31);
+  tot[0] = __shfl_sync(0xffffffffu, x, 31);
+  tot[1] = __shfl_sync(0xffffffffu, y, 31);
+  if (warp) {
+    a += pa;
+    b += pb;
+  }
   __syncthreads();
 }
 
@@ -92,6 +97,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs p) {
   __shared__ int bad_s;
   int* start = plan_sm;              // [R + 1]
   int* page0 = plan_sm + p.reqs + 1;  // [R + 1] new pages below request r
+  int* ctx_s = page0 + p.reqs + 1;    // [R] cached tokens
   const int tid = threadIdx.x, R = p.reqs, bs = p.bs;
   pdl_wait();
   if (tid == 0) bad_s = 0;
@@ -102,14 +108,16 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs p) {
   for (int r0 = 0; r0 < R; r0 += kPlanThreads) {
     const int r = r0 + tid;
     long long n = 0, np = 0;
+    int c = 0;
     if (r < R) {
-      const long long c = p.ctx[r], w = p.nw[r];
+      c = p.ctx[r];
+      const long long w = p.nw[r];
       if (c < 0 || w < 0 || c + w > 0x7fffffffLL) bad |= kBadLength;
       else {
-        const long long need = (c + w + bs - 1) / bs;
+        const int need = (int)((c + w + bs - 1) / bs), have = (int)(((long long)c + bs - 1) / bs);
         if (need > p.width) bad |= kTableWidth;
         n = w;
-        np = p.free_ids ? need - (c + bs - 1) / bs : 0;
+        np = p.free_ids ? need - have : 0;
       }
     }
     long long tot[2], a = n, b = np;
@@ -117,6 +125,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs p) {
     if (r < R) {  // (sums past int32 are refused below before they are read)
       start[r] = (int)(t_sum + a - n);
       page0[r] = (int)(p_sum + b - np);
+      ctx_s[r] = c;
     }
     t_sum += tot[0];
     p_sum += tot[1];
@@ -135,25 +144,25 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs p) {
   const int gtid = blockIdx.x * kPlanThreads + tid, gthreads = gridDim.x * kPlanThreads;
   for (int r = gtid; r <= R; r += gthreads) {
     p.query_start[r] = bad ? 0 : start[r];
-    if (r < R) p.seq_lens[r] = bad ? 0 : p.ctx[r] + p.nw[r];
+    if (r < R) p.seq_lens[r] = bad ? 0 : ctx_s[r] + (start[r + 1] - start[r]);
   }
   for (int i = gtid; i < pages; i += gthreads) {
     const int r = find_request(page0, R, i);
-    const int first = (int)(((long long)p.ctx[r] + bs - 1) / bs);
+    const int first = (int)(((long long)ctx_s[r] + bs - 1) / bs);
     p.table[r * p.table_stride + first + (i - page0[r])] = p.free_ids[head + i];
   }
   for (int i = gtid; i < p.rows; i += gthreads) {
     long long pos = 0, slot = -1;
     if (i < tokens) {
       const int r = find_request(start, R, i);
-      const int c = p.ctx[r];
-      pos = (long long)c + (i - start[r]);
-      const int pg = (int)(pos / bs), first = (int)(((long long)c + bs - 1) / bs);
+      const int c = ctx_s[r], at = c + (i - start[r]);  // (below seq_lens[r]: fits)
+      const int pg = at / bs, first = (int)(((long long)c + bs - 1) / bs);
+      pos = at;
       // a page taken in this call is read from the free list: another CTA may not have
       // written its table entry yet
       const int id = p.free_ids && pg >= first ? p.free_ids[head + page0[r] + pg - first]
                                                : p.table[r * p.table_stride + pg];
-      if (id >= 0) slot = (long long)id * bs + (pos - (long long)pg * bs);
+      if (id >= 0) slot = (long long)id * bs + (at - pg * bs);
       else atomicOr(p.error, kBadPage);
     }
     p.positions[i] = pos;
@@ -189,89 +198,162 @@ struct RopeArgs {
   int* error;
 };
 
-__device__ __forceinline__ void unpack8(const uint4 u, float (&v)[8]) {
-  v[0] = bf_lo(u.x), v[1] = bf_hi(u.x), v[2] = bf_lo(u.y), v[3] = bf_hi(u.y);
-  v[4] = bf_lo(u.z), v[5] = bf_hi(u.z), v[6] = bf_lo(u.w), v[7] = bf_hi(u.w);
+// packed pairs of fp32 (each half rounded as the scalar operation)
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 pack2(float lo, float hi) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(u64 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack8(const uint4 u, u64 (&v)[4]) {
+  v[0] = pack2(bf_lo(u.x), bf_hi(u.x));
+  v[1] = pack2(bf_lo(u.y), bf_hi(u.y));
+  v[2] = pack2(bf_lo(u.z), bf_hi(u.z));
+  v[3] = pack2(bf_lo(u.w), bf_hi(u.w));
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+__device__ __forceinline__ uint4 pack8(const u64 (&v)[4]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    float a, b;
+    unpack2(v[j], a, b);
+    w[j] = pack_bf16(a, b);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// D / 16 lanes hold a head, 16 elements each: two runs of 8 that are rotation partners (i ..
+// i + 7 and i + r/2 ..), or two of the unrotated rest; so the norm's butterfly is the only
+// exchange between lanes.  A CTA is 128 threads of one row (blockIdx.y: which heads).  Memory
+// bound with two dependent loads (position, then rotation row) in a row's chain: small CTAs
+// at 48 registers, ten or more to an SM, hide that best (16111 rows of 24 heads of 256: 80
+// us, 4.9 TB/s; 256 threads 97-109 us, persistent CTAs reading four rows ahead 137 us).
+constexpr int kRopeMaxThreads = 128;
 
 template <int D>
-__global__ void __launch_bounds__(256) rope_store_kernel(RopeArgs p) {
-  constexpr int L = D / 8;  // lanes per head
-  pdl_wait();
+__global__ void __launch_bounds__(kRopeMaxThreads, 10) rope_store_kernel(RopeArgs p) {
+  constexpr int L = D / 16;  // lanes per head
   const int nh = p.nq + 2 * p.nkv;
-  const int64_t total = (int64_t)p.rows * nh;
-  const int sub = threadIdx.x % L;
-  const int64_t step = (int64_t)gridDim.x * (256 / L);
-  const int64_t first = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  const int half = p.rot >> 1, hl = half >> 3;  // rotation partner: hl lanes away
-  const int src = (threadIdx.x & 31) + (sub < hl ? hl : (sub < 2 * hl ? -hl : 0));
-  const float sg = sub < hl ? -1.0f : 1.0f;
-  // (all lanes of a warp stay to the last head: the shuffles are the whole warp's)
-  for (int64_t i = first; __any_sync(0xffffffffu, i < total); i += step) {
-    const bool live = i < total;
-    const int64_t row = live ? i / nh : 0;
-    const int h = live ? (int)(i - row * nh) : 0;
-    const bool is_v = h >= p.nq + p.nkv, is_k = !is_v && h >= p.nq;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    int64_t pos = 0, slot = 0;
-    if (live) {
-      w = ldg_stream(p.qkv + row * p.row_stride + h * D + 8 * sub);
-      if (!is_v) pos = p.positions[row];
-      if (is_k || is_v) slot = p.slots[row];
-    }
-    const bool pos_ok = pos >= 0 && pos < p.max_pos;
-    float x[8], y[8];
-    unpack8(w, x);
+  const int sub = threadIdx.x % L, h = blockIdx.y * (blockDim.x / L) + threadIdx.x / L;
+  const bool head_ok = h < nh, is_v = h >= p.nq + p.nkv, is_k = !is_v && h >= p.nq;
+  const int half = p.rot >> 1, hl = half >> 3;
+  const bool rotated = head_ok && !is_v && sub < hl;
+  const int e0 = sub < hl ? 8 * sub : 8 * (hl + sub);
+  const int e1 = e0 + (sub < hl ? half : 8 * (L - hl));
+  const int64_t row = blockIdx.x;
+  pdl_wait();
+  uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0, g0 = w0, g1 = w0, cw = w0, sw = w0;
+  int64_t pos = 0, slot = -1;
+  const bool norm = p.qg && head_ok && !is_v;
+  if (head_ok) {
+    const uint16_t* x_at = p.qkv + row * p.row_stride + h * D;
+    if (!is_v) pos = p.positions[row];
+    if (is_v || is_k) slot = p.slots[row];
+    w0 = ldg_stream(x_at + e0);
+    w1 = ldg_stream(x_at + e1);
+  }
+  if (norm) {
     const uint16_t* gamma = is_k ? p.kg : p.qg;
-    float ss = 0.0f;
+    g0 = __ldg(reinterpret_cast<const uint4*>(gamma + e0));
+    g1 = __ldg(reinterpret_cast<const uint4*>(gamma + e1));
+  }
+  const bool pos_ok = pos >= 0 && pos < p.max_pos;
+  if (rotated && pos_ok) {
+    cw = __ldg(reinterpret_cast<const uint4*>(p.cos_sin + pos * p.rot + e0));
+    sw = __ldg(reinterpret_cast<const uint4*>(p.cos_sin + pos * p.rot + e1));
+  }
+  u64 x[4], y[4];
+  unpack8(w0, x);
+  unpack8(w1, y);
+  if (p.qg) {  // (uniform: the shuffles are the whole warp's)
+    u64 s2 = mul2(x[0], x[0]);
 #pragma unroll
-    for (int j = 0; j < 8; j++) ss = __fmaf_rn(x[j], x[j], ss);
+    for (int j = 1; j < 4; j++) s2 = fma2(x[j], x[j], s2);
 #pragma unroll
-    for (int o = L / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (gamma && !is_v) {
-      const float inv = rsqrtf(ss * (1.0f / D) + p.eps);
-      float g[8];
-      unpack8(*reinterpret_cast<const uint4*>(gamma + 8 * sub), g);
+    for (int j = 0; j < 4; j++) s2 = fma2(y[j], y[j], s2);
+    float a, b;
+    unpack2(s2, a, b);
+    a += b;
 #pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = x[j] * inv * g[j];
+    for (int o = L / 2; o >= 1; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if (norm) {
+      const float inv = rsqrtf(a * (1.0f / D) + p.eps);
+      const u64 inv2 = pack2(inv, inv);
+      u64 g[4];
+      unpack8(g0, g);
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[j] = mul2(mul2(x[j], inv2), g[j]);
+      unpack8(g1, g);
+#pragma unroll
+      for (int j = 0; j < 4; j++) y[j] = mul2(mul2(y[j], inv2), g[j]);
     }
+  }
+  if (rotated) {
+    u64 c[4], s[4];
+    unpack8(cw, c);
+    unpack8(sw, s);
+    const u64 minus = pack2(-1.0f, -1.0f);
 #pragma unroll
-    for (int j = 0; j < 8; j++) y[j] = __shfl_sync(0xffffffffu, x[j], src);
-    if (!is_v) {
-      if (sub < 2 * hl && pos_ok) {
-        const uint16_t* cs = p.cos_sin + pos * p.rot + 8 * (sub < hl ? sub : sub - hl);
-        float c[8], s[8];
-        unpack8(*reinterpret_cast<const uint4*>(cs), c);
-        unpack8(*reinterpret_cast<const uint4*>(cs + half), s);
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = __fadd_rn(__fmul_rn(x[j], c[j]), __fmul_rn(sg * y[j], s[j]));
-      }
-      w = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+    for (int j = 0; j < 4; j++) {
+      const u64 xs = mul2(x[j], s[j]), ys = mul2(mul2(y[j], s[j]), minus);
+      x[j] = add2(mul2(x[j], c[j]), ys);
+      y[j] = add2(mul2(y[j], c[j]), xs);
     }
-    if (!live) continue;
-    if (!pos_ok) {
-      if (sub == 0) atomicOr(p.error, kBadPosition);
-      continue;
-    }
-    if (!is_v && !is_k) {
-      *reinterpret_cast<uint4*>(p.q_out + (row * p.nq + h) * D + 8 * sub) = w;
-      continue;
-    }
-    if (slot < 0) continue;  // padding
+  }
+  if (!head_ok) return;
+  if (!is_v) {
+    w0 = pack8(x);
+    w1 = pack8(y);
+  }
+  uint16_t* dst;
+  if (!pos_ok) {
+    if (sub == 0) atomicOr(p.error, kBadPosition);
+    return;
+  }
+  if (!is_v && !is_k) {
+    dst = p.q_out + (row * p.nq + h) * D;
+  } else {
+    if (slot < 0) return;  // padding
     if (slot >= p.num_slots) {
       if (sub == 0) atomicOr(p.error, kBadSlot);
-      continue;
+      return;
+    }
+    int64_t blk, off;
+    if (slot <= 0x7fffffff) {  // (a 64-bit division costs as much as the row's arithmetic)
+      blk = (uint32_t)slot / (uint32_t)p.bs;
+      off = (uint32_t)slot - (uint32_t)blk * (uint32_t)p.bs;
+    } else {
+      blk = slot / p.bs;
+      off = slot - blk * p.bs;
     }
     const int kh = h - p.nq - (is_v ? p.nkv : 0);
-    const int64_t blk = slot / p.bs, off = slot - blk * p.bs;
-    uint16_t* dst = (is_v ? p.v_cache : p.k_cache) + ((blk * p.nkv + kh) * p.bs + off) * D + 8 * sub;
-    *reinterpret_cast<uint4*>(dst) = w;
+    dst = (is_v ? p.v_cache : p.k_cache) + ((blk * p.nkv + kh) * p.bs + off) * D;
   }
+  *reinterpret_cast<uint4*>(dst + e0) = w0;
+  *reinterpret_cast<uint4*>(dst + e1) = w1;
 }
 
 // ------------------------------------------------------------------ attention work list

@@ -301,31 +301,44 @@ ERR_WAIT, ERR_LENGTH, ERR_NO_PAGES, ERR_TABLE_WIDTH, ERR_NO_ROWS = 1, 4, 8, 16, 
 ERR_PAGE, ERR_POSITION, ERR_SLOT = 64, 128, 256
 
 
-def _call_on(device: torch.device, name: str, *args) -> None:
-    """Launch on the tensors' own device, on its current stream."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, _stream())
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _launch(dev: int, name: str, *args) -> None:
+    """Launch on device ``dev`` (the tensors' own), on its current stream.  Pointers are
+    passed as integers and the checks below build no message before one fails: these
+    calls are made per layer and step, where host time counts."""
+    if dev == torch.cuda.current_device():
+        call(name, *args, _raw_stream(dev))
         return
-    with torch.cuda.device(device):
-        call(name, *args, _stream())
+    with torch.cuda.device(dev):
+        call(name, *args, _raw_stream(dev))
 
 
-def _same_device(device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None:
-            _check(t.device == device, f"{name} must be on {device}, got {t.device}")
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
 
 
-def _error_word(error: torch.Tensor) -> None:
-    _cuda(error, "error", torch.int32)
-    _check(error.numel() >= 1, "error must hold one int32")
+def _need(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int) -> None:
+    """t must be a dense ``dtype`` tensor on CUDA device ``dev``."""
+    if t.dtype is dtype and t.get_device() == dev and t.is_contiguous():
+        return
+    _cuda(t, name, dtype)
+    raise ValueError(f"{name} must be on cuda:{dev}, got {t.device}")
 
 
-def _block_table(block_table: torch.Tensor, reqs: int) -> None:
-    _check(block_table.is_cuda and block_table.dtype == torch.int32, "block_table must be a CUDA int32 tensor")
-    _check(block_table.dim() == 2 and block_table.stride(1) == 1, "block_table must be [requests, pages], rows dense")
-    _check(block_table.shape[0] >= reqs and block_table.shape[1] >= 1,
-           f"block_table must have {reqs} rows, got {tuple(block_table.shape)}")
+def _home(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
+    """The CUDA device index of ``t``, which must have ``dtype``."""
+    if not t.is_cuda or t.dtype is not dtype:
+        raise ValueError(f"{name} must be a CUDA {dtype} tensor, got {t.dtype} on {t.device}")
+    return t.get_device()
+
+
+def _block_table(t: torch.Tensor, reqs: int, dev: int) -> None:
+    if t.dtype is not torch.int32 or t.get_device() != dev:
+        raise ValueError(f"block_table must be an int32 tensor on cuda:{dev}, got {t.dtype} on {t.device}")
+    if t.dim() != 2 or t.stride(1) != 1 or t.shape[0] < reqs or t.shape[1] < 1:
+        raise ValueError(f"block_table must be [{reqs} requests, pages] with dense rows, got {tuple(t.shape)}")
 
 
 def paged_plan_out(ctx_lens, new_lens, block_table, block_size, query_start, seq_lens, positions, slot_mapping,
@@ -337,36 +350,41 @@ def paged_plan_out(ctx_lens, new_lens, block_table, block_size, query_start, seq
     ``free_blocks`` (int32 [F]) with ``free_head`` (int32 [1], ids taken so far), the new
     pages' ids into ``block_table`` and the advanced head into ``free_head_out`` (default:
     ``free_head`` itself).  All or nothing: a batch that does not fit comes out empty, with
-    the reason in ``error`` (ERR_* bits).  ``counter`` int32 [1], zero."""
-    R = ctx_lens.numel()
-    for t, nm in ((ctx_lens, "ctx_lens"), (new_lens, "new_lens"), (query_start, "query_start"),
-                  (seq_lens, "seq_lens"), (counter, "counter")):
-        _cuda(t, nm, torch.int32)
-    for t, nm in ((positions, "positions"), (slot_mapping, "slot_mapping")):
-        _cuda(t, nm, torch.int64)
-    _error_word(error)
-    _check(R >= 1 and new_lens.numel() == R and seq_lens.numel() == R and query_start.numel() == R + 1,
-           "ctx_lens, new_lens, seq_lens hold one entry per request, query_start one more")
-    _check(positions.numel() == slot_mapping.numel(), "positions and slot_mapping must have the same length")
-    _check(counter.numel() >= 1, "counter must hold one int32")
-    _check(block_size >= 1, "block_size must be positive")
-    _block_table(block_table, R)
-    _check((free_blocks is None) == (free_head is None), "give free_blocks and free_head together")
-    _check(free_head_out is None or free_head is not None, "free_head_out needs free_head")
+    the reason in ``error`` (ERR_* bits).  ``counter`` int32 [1], zero before the first call
+    and left zero; calls that may overlap on the device need one each."""
+    i32 = torch.int32
+    dev = _home(ctx_lens, "ctx_lens", i32)
+    R, rows = ctx_lens.numel(), positions.numel()
+    _need(ctx_lens, "ctx_lens", i32, dev)
+    _need(new_lens, "new_lens", i32, dev)
+    _need(query_start, "query_start", i32, dev)
+    _need(seq_lens, "seq_lens", i32, dev)
+    _need(counter, "counter", i32, dev)
+    _need(error, "error", i32, dev)
+    _need(positions, "positions", torch.int64, dev)
+    _need(slot_mapping, "slot_mapping", torch.int64, dev)
+    if R < 1 or new_lens.numel() != R or seq_lens.numel() != R or query_start.numel() != R + 1:
+        raise ValueError("ctx_lens, new_lens and seq_lens hold one entry per request, query_start one more")
+    if slot_mapping.numel() != rows:
+        raise ValueError("positions and slot_mapping must have the same length")
+    if counter.numel() < 1 or error.numel() < 1:
+        raise ValueError("counter and error must hold one int32")
+    _block_table(block_table, R, dev)
+    if (free_blocks is None) != (free_head is None) or (free_head_out is not None and free_head is None):
+        raise ValueError("give free_blocks and free_head together (and free_head_out only with them)")
     if free_blocks is not None:
         free_head_out = free_head if free_head_out is None else free_head_out
-        for t, nm in ((free_blocks, "free_blocks"), (free_head, "free_head"), (free_head_out, "free_head_out")):
-            _cuda(t, nm, torch.int32)
-            _check(nm == "free_blocks" or t.numel() == 1, f"{nm} must hold one int32")
-    dev = ctx_lens.device
-    _same_device(dev, new_lens=new_lens, block_table=block_table, query_start=query_start, seq_lens=seq_lens,
-                 positions=positions, slot_mapping=slot_mapping, counter=counter, error=error,
-                 free_blocks=free_blocks, free_head=free_head, free_head_out=free_head_out)
-    _call_on(dev, "spark_paged_plan", _p(ctx_lens), _p(new_lens), R, _p(free_blocks),
-             0 if free_blocks is None else free_blocks.numel(), _p(free_head), _p(free_head_out), _p(block_table),
-             block_table.stride(0) if R > 1 else block_table.shape[1], block_table.shape[1], int(block_size),
-             positions.numel(), _p(query_start), _p(seq_lens), _p(positions), _p(slot_mapping), _p(counter),
-             _p(error))
+        _need(free_blocks, "free_blocks", i32, dev)
+        _need(free_head, "free_head", i32, dev)
+        _need(free_head_out, "free_head_out", i32, dev)
+        if free_head.numel() != 1 or free_head_out.numel() != 1:
+            raise ValueError("free_head must hold one int32")
+    width = block_table.shape[1]
+    _launch(dev, "spark_paged_plan", ctx_lens.data_ptr(), new_lens.data_ptr(), R, _ptr(free_blocks),
+            0 if free_blocks is None else free_blocks.numel(), _ptr(free_head), _ptr(free_head_out),
+            block_table.data_ptr(), block_table.stride(0) if R > 1 else width, width, int(block_size), rows,
+            query_start.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(),
+            counter.data_ptr(), error.data_ptr())
 
 
 def qk_norm_rope_store_rows(qkv, nq, nkv, head_dim, q_gamma, k_gamma, eps, cos_sin, positions, slot_mapping, k_cache,
@@ -375,32 +393,41 @@ def qk_norm_rope_store_rows(qkv, nq, nkv, head_dim, q_gamma, k_gamma, eps, cos_s
     pass: per-head RMS norm of q and k (``q_gamma`` / ``k_gamma`` bf16 [head_dim], or both
     None), rotation at ``positions`` (int64 [rows]) by ``cos_sin`` bf16 [max_pos,
     rotary_dim], q to ``q_out`` bf16 [rows, nq, head_dim] and k, v to the paged caches at
-    ``slot_mapping`` (int64 [rows], negative: not stored).  fp32 inside, one rounding."""
-    _check(qkv.is_cuda and qkv.dtype == BF16, "qkv must be a CUDA bfloat16 tensor")
-    _check(qkv.dim() == 2 and (qkv.stride(1) == 1 or qkv.shape[1] == 1), "qkv must be [rows, cols], rows dense")
+    ``slot_mapping`` (int64 [rows], negative: not stored; no slot twice).  fp32 inside, one
+    rounding."""
+    dev = _home(qkv, "qkv", BF16)
+    if qkv.dim() != 2 or (qkv.stride(1) != 1 and qkv.shape[1] != 1) or qkv.shape[1] < (nq + 2 * nkv) * head_dim:
+        raise ValueError(f"qkv must be [rows, >= {(nq + 2 * nkv) * head_dim}] with dense rows, got {tuple(qkv.shape)}")
     rows = qkv.shape[0]
-    _check(qkv.shape[1] >= (nq + 2 * nkv) * head_dim, "qkv rows must hold (nq + 2 nkv) * head_dim columns")
-    for t, nm in ((cos_sin, "cos_sin"), (k_cache, "k_cache"), (v_cache, "v_cache"), (q_out, "q_out")):
-        _cuda(t, nm, BF16)
-    for t, nm in ((positions, "positions"), (slot_mapping, "slot_mapping")):
-        _cuda(t, nm, torch.int64)
-        _check(t.numel() >= rows, f"{nm} must hold one entry per row")
-    _error_word(error)
-    _check((q_gamma is None) == (k_gamma is None), "give q_gamma and k_gamma together")
+    _need(cos_sin, "cos_sin", BF16, dev)
+    _need(k_cache, "k_cache", BF16, dev)
+    _need(v_cache, "v_cache", BF16, dev)
+    _need(q_out, "q_out", BF16, dev)
+    _need(positions, "positions", torch.int64, dev)
+    _need(slot_mapping, "slot_mapping", torch.int64, dev)
+    _need(error, "error", torch.int32, dev)
+    if positions.numel() < rows or slot_mapping.numel() < rows:
+        raise ValueError("positions and slot_mapping must hold one entry per row")
+    if error.numel() < 1:
+        raise ValueError("error must hold one int32")
+    if (q_gamma is None) != (k_gamma is None):
+        raise ValueError("give q_gamma and k_gamma together")
     if q_gamma is not None:
-        for t, nm in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
-            _cuda(t, nm, BF16)
-            _check(t.numel() == head_dim, f"{nm} must hold head_dim values")
-    _check(cos_sin.dim() == 2, "cos_sin must be [max_pos, rotary_dim]")
-    _check(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[1] == nkv and
-           k_cache.shape[3] == head_dim, "caches must be [blocks, nkv, block_size, head_dim]")
-    _check(q_out.numel() == rows * nq * head_dim, "q_out must be [rows, nq, head_dim]")
-    _same_device(qkv.device, q_gamma=q_gamma, k_gamma=k_gamma, cos_sin=cos_sin, positions=positions,
-                 slot_mapping=slot_mapping, k_cache=k_cache, v_cache=v_cache, q_out=q_out, error=error)
-    _call_on(qkv.device, "spark_qk_norm_rope_store_rows", _p(qkv), qkv.stride(0) if rows > 1 else
-             (qkv.shape[1] + 7) // 8 * 8, rows, nq, nkv, head_dim, _p(q_gamma), _p(k_gamma), float(eps), _p(cos_sin),
-             cos_sin.shape[0], cos_sin.shape[1], _p(positions), _p(slot_mapping), k_cache.shape[2], k_cache.shape[0],
-             _p(k_cache), _p(v_cache), _p(q_out), _p(error))
+        _need(q_gamma, "q_gamma", BF16, dev)
+        _need(k_gamma, "k_gamma", BF16, dev)
+        if q_gamma.numel() != head_dim or k_gamma.numel() != head_dim:
+            raise ValueError("q_gamma and k_gamma must hold head_dim values")
+    if cos_sin.dim() != 2:
+        raise ValueError("cos_sin must be [max_pos, rotary_dim]")
+    ks = k_cache.shape
+    if len(ks) != 4 or v_cache.shape != ks or ks[1] != nkv or ks[3] != head_dim:
+        raise ValueError("caches must be [blocks, nkv, block_size, head_dim]")
+    if q_out.numel() != rows * nq * head_dim:
+        raise ValueError("q_out must be [rows, nq, head_dim]")
+    _launch(dev, "spark_qk_norm_rope_store_rows", qkv.data_ptr(), qkv.stride(0) if rows > 1 else
+            (qkv.shape[1] + 7) // 8 * 8, rows, nq, nkv, head_dim, _ptr(q_gamma), _ptr(k_gamma), eps,
+            cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1], positions.data_ptr(), slot_mapping.data_ptr(),
+            ks[2], ks[0], k_cache.data_ptr(), v_cache.data_ptr(), q_out.data_ptr(), error.data_ptr())
     return q_out
 
 
@@ -427,6 +454,7 @@ class AttnPlan:
         rows = lib().spark_attn_part_rows(max_tokens, max_reqs, nq, nkv, head_dim)
         self.max_tokens, self.max_reqs, self.window = int(max_tokens), int(max_reqs), int(window)
         self.nq, self.nkv, self.head_dim, self.device = nq, nkv, head_dim, device
+        self.dev = device.index
         self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
         self.part_o = torch.empty((rows, nkv, head_dim), dtype=torch.float32, device=device)
         self.part_ml = torch.empty((rows, nkv, 2), dtype=torch.float32, device=device)
@@ -434,19 +462,19 @@ class AttnPlan:
         self.kind, self.reqs = None, 0
 
     def _make(self, kind, reqs, query_start, seq_lens, prefix_len):
-        _check(reqs <= self.max_reqs, f"{reqs} requests in a plan for {self.max_reqs}")
-        _same_device(self.device, query_start=query_start, seq_lens=seq_lens, prefix_len=prefix_len)
-        _call_on(self.device, "spark_attn_plan", _p(query_start), _p(seq_lens), _p(prefix_len), reqs,
-                 self.max_tokens, self.max_reqs, self.nq, self.nkv, self.head_dim, self.window, _p(self.buf),
-                 _p(self.error))
+        if reqs > self.max_reqs:
+            raise ValueError(f"{reqs} requests in a plan for {self.max_reqs}")
+        _launch(self.dev, "spark_attn_plan", _ptr(query_start), _ptr(seq_lens), _ptr(prefix_len), reqs,
+                self.max_tokens, self.max_reqs, self.nq, self.nkv, self.head_dim, self.window, _ptr(self.buf),
+                _ptr(self.error))
         self.kind, self.reqs = kind, reqs
         return self
 
     def update(self, query_start: torch.Tensor, seq_lens: torch.Tensor) -> "AttnPlan":
         """A packed batch: request r's query tokens are rows query_start[r] ..
         query_start[r + 1] - 1 (int32 [R + 1]), the last of its seq_lens[r] (int32 [R]) keys."""
-        _cuda(query_start, "query_start", torch.int32)
-        _cuda(seq_lens, "seq_lens", torch.int32)
+        _need(query_start, "query_start", torch.int32, self.dev)
+        _need(seq_lens, "seq_lens", torch.int32, self.dev)
         reqs = seq_lens.numel()
         _check(reqs >= 1 and query_start.numel() == reqs + 1, "query_start must have one entry more than seq_lens")
         return self._make("prompt", reqs, query_start, seq_lens, None)
@@ -454,8 +482,8 @@ class AttnPlan:
     def update_prefix(self, seq_lens: torch.Tensor, prefix_len: torch.Tensor) -> "AttnPlan":
         """One query token per request, seq_lens[r] (int32 [R]) keys each, the first
         prefix_len (int32 [1]) of them the same for all."""
-        _cuda(seq_lens, "seq_lens", torch.int32)
-        _cuda(prefix_len, "prefix_len", torch.int32)
+        _need(seq_lens, "seq_lens", torch.int32, self.dev)
+        _need(prefix_len, "prefix_len", torch.int32, self.dev)
         _check(self.window == 0, "a shared prefix is read without a window")
         _check(prefix_len.numel() == 1, "prefix_len must hold one int32")
         reqs = seq_lens.numel()
@@ -463,27 +491,38 @@ class AttnPlan:
         return self._make("prefix", reqs, None, seq_lens, prefix_len)
 
 
+def _heads(t: torch.Tensor, name: str, plan: AttnPlan) -> None:
+    shape = t.shape
+    if t.dtype is not BF16 or t.get_device() != plan.dev:
+        raise ValueError(f"{name} must be a bfloat16 tensor on cuda:{plan.dev}, got {t.dtype} on {t.device}")
+    if len(shape) != 3 or shape[1] != plan.nq or shape[2] != plan.head_dim or (t.stride(2) != 1 and t.numel()):
+        raise ValueError(f"{name} must be [tokens, {plan.nq}, {plan.head_dim}], heads dense, got {tuple(shape)}")
+
+
 def _attn_paged(kind, q, k_cache, v_cache, block_table, plan, scale, out, error, wait_ns):
-    _check(plan.kind == kind, f"the plan was made for {plan.kind!r}, not {kind!r}")
-    nq, nkv, D = plan.nq, plan.nkv, plan.head_dim
-    for t, nm in ((q, "q"), (out, "out")):
-        _check(t.is_cuda and t.dtype == BF16, f"{nm} must be a CUDA bfloat16 tensor")
-        _check(t.dim() == 3 and t.shape[1] == nq and t.shape[2] == D and (t.stride(2) == 1 or t.numel() == 0),
-               f"{nm} must be [tokens, {nq}, {D}], heads dense")
+    if plan.kind != kind:
+        raise ValueError(f"the plan was made for {plan.kind!r}, not {kind!r}")
+    nq, nkv, D, dev = plan.nq, plan.nkv, plan.head_dim, plan.dev
+    _heads(q, "q", plan)
+    _heads(out, "out", plan)
     tokens = q.shape[0]
-    _check(out.shape[0] >= tokens, "out must have a row per token")
-    _check(tokens <= plan.max_tokens, f"{tokens} tokens in a plan for {plan.max_tokens}")
-    _cuda(k_cache, "k_cache", BF16)
-    _cuda(v_cache, "v_cache", BF16)
-    _check(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[1] == nkv and
-           k_cache.shape[3] == D, f"caches must be [blocks, {nkv}, block_size, {D}]")
-    _block_table(block_table, plan.reqs)
-    _error_word(error)
-    _same_device(plan.device, q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, out=out, error=error)
-    _call_on(plan.device, "spark_attn_paged", _p(q), q.stride(0), q.stride(1), tokens, _p(k_cache), _p(v_cache),
-             k_cache.shape[0], k_cache.shape[2], _p(block_table), block_table.stride(0), block_table.shape[1],
-             plan.max_tokens, plan.max_reqs, nq, nkv, D, plan.window, float(scale), _p(plan.buf), _p(plan.part_o),
-             _p(plan.part_ml), _p(out), out.stride(0), out.stride(1), _p(error), int(wait_ns))
+    if out.shape[0] < tokens or tokens > plan.max_tokens:
+        raise ValueError(f"{tokens} tokens: out has {out.shape[0]} rows, the plan room for {plan.max_tokens}")
+    _need(k_cache, "k_cache", BF16, dev)
+    _need(v_cache, "v_cache", BF16, dev)
+    ks = k_cache.shape
+    if len(ks) != 4 or v_cache.shape != ks or ks[1] != nkv or ks[3] != D:
+        raise ValueError(f"caches must be [blocks, {nkv}, block_size, {D}]")
+    _block_table(block_table, plan.reqs, dev)
+    _need(error, "error", torch.int32, dev)
+    if error.numel() < 1:
+        raise ValueError("error must hold one int32")
+    qt, qh, _ = q.stride()
+    ot, oh, _ = out.stride()
+    _launch(dev, "spark_attn_paged", q.data_ptr(), qt, qh, tokens, k_cache.data_ptr(), v_cache.data_ptr(), ks[0],
+            ks[2], block_table.data_ptr(), block_table.stride(0), block_table.shape[1], plan.max_tokens,
+            plan.max_reqs, nq, nkv, D, plan.window, scale, plan.buf.data_ptr(), plan.part_o.data_ptr(),
+            plan.part_ml.data_ptr(), out.data_ptr(), ot, oh, error.data_ptr(), wait_ns)
     return out
 
 
