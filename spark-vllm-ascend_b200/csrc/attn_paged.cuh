@@ -31,9 +31,9 @@
 // Three ways through one loop:
 //   head_dim 128, many rows: half h has its own 128 rows, S_h, O_h; every K / V chunk is
 //     used by both, and half 1's products run while half 0's softmax does;
-//   head_dim 128, few rows (up to 128: single tokens): both halves have the same rows and
-//     take alternate key tiles, each with its own m, l, O; they are merged through the Q
-//     buffer at the end;
+//   head_dim 128, few rows (up to 128: single tokens) and two key tiles or more: both halves
+//     have the same rows and take alternate key tiles, each with its own m, l, O, and leave a
+//     part each to be joined;
 //   head_dim 256: 128 rows, S0 and S1 take alternate key tiles of one softmax, O0 O1 are
 //     the two column halves of one sum.
 // In all of them the scores of tile t + 1 (or + 2) are computed while the softmax of tile t
@@ -75,11 +75,12 @@ constexpr int kOffRing = 64 * 1024;
 constexpr int kOffX = kOffRing + kStages * kChunk;  // row values shared by a half's warpgroups: [4][128]
 constexpr int kOffBar = kOffX + 4 * 128 * 4;
 constexpr int kBarFull = 0, kBarEmpty = kBarFull + kStages, kBarQFull = kBarEmpty + kStages,
-              kBarQEmpty = kBarQFull + 1, kBarS = kBarQEmpty + 1, kBarP = kBarS + 2, kBarP2 = kBarP + 2, kBarO = kBarP2 + 2,
-              kBarPV = kBarO + 2, kBarMerge = kBarPV + 2, kBarX = kBarMerge + 1, kBarDrain = kBarX + 8, kNumBars = kBarDrain + 1;
+              kBarQEmpty = kBarQFull + 2, kBarS = kBarQEmpty + 2, kBarP = kBarS + 2, kBarP2 = kBarP + 2,
+              kBarO = kBarP2 + 2, kBarPV = kBarO + 2, kBarX = kBarPV + 2, kBarDrain = kBarX + 8,
+              kNumBars = kBarDrain + 1;
 constexpr int kOffMisc = kOffBar + 8 * kNumBars;  // tensor-memory base, abort flag, drained flag
-constexpr int kOffItem = (kOffMisc + 16 + 15) / 16 * 16;  // the current item and its kv head
-constexpr int kSmemBytes = kOffItem + 64;
+constexpr int kOffItem = (kOffMisc + 16 + 15) / 16 * 16;  // two items and their kv heads, 64 bytes each
+constexpr int kSmemBytes = kOffItem + 2 * 64;
 constexpr int kTmemCols = 512;
 constexpr int kColS = 0, kColO = 256;
 constexpr unsigned long long kWaitNs = 500ull * 1000 * 1000;
@@ -109,10 +110,21 @@ __device__ __forceinline__ unsigned long long now_ns() {
   return t;
 }
 
-// Wait for the phase of `parity`; false: limit_ns ran out or another role gave up.  The
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ldsf(uint32_t addr) { return __uint_as_float(lds32(addr)); }
+__device__ __forceinline__ void stsf(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// Wait for the phase of `parity`; false: limit_ns ran out or another role gave up (abort: the
+// shared address of its flag, or 0).  The
 // clock and the flag are looked at every 16th try only.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, unsigned long long limit_ns,
-                                         const volatile int* abort) {
+                                         uint32_t abort) {
   unsigned long long t0 = 0;
   for (uint32_t spin = 1;; spin++) {
     uint32_t done;
@@ -123,12 +135,21 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, unsigned
         : "memory");
     if (done) return true;
     if ((spin & 15u) == 0) {
-      if (abort && *abort) return false;
+      if (abort && lds32(abort)) return false;
       const unsigned long long t = now_ns();
       if (t0 == 0) t0 = t;
       else if (t - t0 >= limit_ns) return false;
     }
   }
+}
+// one look
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{.reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}"
+               : "=r"(done)
+               : "r"(bar), "r"(parity)
+               : "memory");
+  return done != 0;
 }
 __device__ __forceinline__ void bar_init(uint32_t bar, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
@@ -310,8 +331,8 @@ __device__ __forceinline__ int warp_min_i(int v) {
 
 // The CTA's i-th work index (item x kv head): forward and backward through the CTAs in
 // turn, so that a CTA that got a long item of one pass gets a short one of the next.
-__device__ __forceinline__ int64_t work_index(int pass) {
-  return (int64_t)pass * gridDim.x + ((pass & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+__device__ __forceinline__ uint32_t work_index(uint32_t pass) {
+  return pass * gridDim.x + ((pass & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
 struct TcArgs {
@@ -321,8 +342,9 @@ struct TcArgs {
   unsigned long long limit_ns;
 };
 
-// Position of V tile t of n in the item's sequence of K / V tiles: d K tiles lead, then
-// V_t, K_{t+d} alternate.
+// Positions of K tile t and V tile t of n in the item's sequence of K / V tiles: d K tiles
+// lead, then V_t, K_{t+d} alternate.
+__device__ __forceinline__ int k_index(int t, int d) { return t < d ? t : 2 * t - d + 1; }
 __device__ __forceinline__ int v_index(int t, int n, int d) {
   const int lead = d < n ? d : n, past = t - (n - lead);
   return lead + 2 * t - (past > 0 ? past : 0);
@@ -347,13 +369,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const uint32_t bars = base + kOffBar;
   const uint32_t tslot = base + kOffMisc;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + kOffMisc + 4);
+  const uint32_t abort_flag = base + kOffMisc + 4;
   volatile int* drained_flag = reinterpret_cast<volatile int*>(gbase + kOffMisc + 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
   auto fail = [&]() {
     atomicOr(p.error, 1);
-    *abort_flag = 1;
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(abort_flag), "r"(1) : "memory");
   };
 
   if (tid == 0) {
@@ -361,19 +383,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(bar(kBarFull + s), 1);
       bar_init(bar(kBarEmpty + s), 1);
     }
-    bar_init(bar(kBarQFull), 1);
-    bar_init(bar(kBarQEmpty), 1 + kSoftmaxWarps);  // the last score product's commit, the softmax warps
     for (int h = 0; h < 2; h++) {
+      bar_init(bar(kBarQFull + h), 1);
+      bar_init(bar(kBarQEmpty + h), 1 + kSoftmaxWarps);  // the last score product's commit, the softmax warps
       bar_init(bar(kBarS + h), 1);
       bar_init(bar(kBarP + h), 8);
       bar_init(bar(kBarP2 + h), 8);
       bar_init(bar(kBarO + h), 1);
       bar_init(bar(kBarPV + h), 1);
     }
-    bar_init(bar(kBarMerge), 8);
     for (int i = 0; i < 8; i++) bar_init(bar(kBarX + i), D == 128 ? 2 : 4);
     bar_init(bar(kBarDrain), 1);
-    *abort_flag = 0;
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(abort_flag), "r"(0) : "memory");
     *drained_flag = 1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -387,10 +408,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tslot) : "memory");
   pdl_wait();
-  pdl_launch_dependents();  // (the next launch in the stream is combine_kernel, which waits)
   const Header* hdr = reinterpret_cast<const Header*>(p.plan);
   const Item* items = reinterpret_cast<const Item*>(p.plan + p.lay.items);
-  const int64_t nwork = (int64_t)hdr->items * p.nkv;
+  const uint32_t nwork = (uint32_t)hdr->items * (uint32_t)p.nkv, room = (uint32_t)p.lay.max_items * (uint32_t)p.nkv;
   const int g = p.nq / p.nkv;
 
   // (each warpgroup changes its share inside its own branch, where the register allocator
@@ -403,10 +423,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       const int pr = args.piece, pp = kKeyTile / pr;
       const int64_t rows_total = p.num_blocks * p.nkv * p.bs;
-      for (int pass = 0; ok; pass++) {
-        const int64_t w = work_index(pass);
+      for (uint32_t pass = 0; ok; pass++) {
+        const uint32_t w = work_index(pass);
+        if (w >= room) break;
+        const Item it = items[w / p.nkv];  // (its load does not wait for the number of items)
         if (w >= nwork) break;
-        const Item it = items[w / p.nkv];
         const int kvh = (int)(w % p.nkv);
         const int n = it.nkt;
         if (n == 0) continue;
@@ -461,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // every issued copy lands before the CTA can give its shared memory up
       bool drained = true;
       for (uint32_t i = ring > (uint32_t)kStages ? ring - kStages : 0; i < ring; i++)
-        drained &= bar_wait(bar(kBarFull + i % kStages), (i / kStages) & 1, kDrainNs, nullptr);
+        drained &= bar_wait(bar(kBarFull + i % kStages), (i / kStages) & 1, kDrainNs, 0);
       if (!drained && lane == 0) {
         atomicOr(p.error, 2);
         *drained_flag = 0;
@@ -470,47 +491,60 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == kQWarp) {
       // ---------------------------------------------------------------- Q
       if (lane == 0) {
-        uint32_t qi = 0;
-        bool ok = true;
+        uint32_t qi = 0, loaded = 0;  // items described; slots whose latest phase is a load of Q
+        bool ok = true, prev_whole = false;
         const uint32_t box = (uint32_t)(g * p.lay.half_tok) * 128u;
-        Item* slot = reinterpret_cast<Item*>(gbase + kOffItem);
-        int* slot_kvh = reinterpret_cast<int*>(gbase + kOffItem + sizeof(Item));
-        for (int pass = 0; ok; pass++) {
-          const int64_t w = work_index(pass);
-          const bool have = w < nwork;
+        // item i is over with its slot (i & 1): read by all, its score products done
+        auto over = [&](uint32_t i) { return bar_wait(bar(kBarQEmpty + (i & 1)), (i >> 1) & 1, limit_ns, abort_flag); };
+        for (uint32_t pass = 0;; pass++, qi++) {
+          const uint32_t w = work_index(pass);
           Item it;
           int kvh = 0;
-          if (have) {  // (read before the wait, written after it)
+          if (w < room) {
             it = items[w / p.nkv];
             kvh = (int)(w % p.nkv);
           }
-          if (!bar_wait(bar(kBarQEmpty), (qi & 1) ^ 1, limit_ns, abort_flag)) {
+          const bool have = w < nwork;
+          // Items that fill the Q buffer wait for the one before; those of few rows take a
+          // half of it in turn
+          const bool whole = have && it.nkt > 0 && (D == 256 || !(it.flags & kFlagFew));
+          if ((qi >= 2 && !over(qi - 2)) || (qi >= 1 && (whole || prev_whole) && !over(qi - 1))) {
             ok = false;
             break;
           }
-          qi++;
+          prev_whole = whole;
+          const uint32_t q = qi & 1, full = bar(kBarQFull + q);
+          loaded &= ~(1u << q);  // (the slot's last load was used: its item is over)
+          Item* slot = reinterpret_cast<Item*>(gbase + kOffItem + 64 * q);
           if (!have) {
             slot->nkt = -1;
-            bar_arrive(bar(kBarQFull));
+            bar_arrive(full);
             break;
           }
           *slot = it;
-          *slot_kvh = kvh;
+          *reinterpret_cast<int*>(gbase + kOffItem + 64 * q + sizeof(Item)) = kvh;
           if (it.nkt == 0) {
-            bar_arrive(bar(kBarQFull));
+            bar_arrive(full);
             continue;
           }
-          const int halves = D == 128 && !(it.flags & kFlagFew) ? 2 : 1;
-          bar_expect_tx(bar(kBarQFull), box * (uint32_t)(halves * (D / 64)));
+          const int halves = D == 128 && whole ? 2 : 1;
+          const uint32_t dst = base + (whole ? 0u : q * kChunk);
+          bar_expect_tx(full, box * (uint32_t)(halves * (D / 64)));
           for (int h = 0; h < halves; h++)
             for (int c = 0; c < D / 64; c++)
-              tma_3d(base + (uint32_t)(h * kChunk + c * kSub), &tmq, c * 64, kvh * g, it.tok0 + h * p.lay.half_tok,
-                     bar(kBarQFull));
+              tma_3d(dst + (uint32_t)(h * kChunk + c * kSub), &tmq, c * 64, kvh * g, it.tok0 + h * p.lay.half_tok, full);
+          loaded |= 1u << q;
         }
         if (!ok) fail();
-        if (qi > 0 && !bar_wait(bar(kBarQFull), (qi - 1) & 1, kDrainNs, nullptr)) {
-          atomicOr(p.error, 2);
-          *drained_flag = 0;
+        // a load still in flight is its slot's latest phase, that of the last item with this
+        // parity below qi (an older phase could not be told from a newer one)
+        for (uint32_t q = 0; q < 2; q++) {
+          if (!(loaded >> q & 1)) continue;
+          const uint32_t i = qi - 1 - ((qi - 1 - q) & 1);
+          if (!bar_wait(bar(kBarQFull + q), (i >> 1) & 1, kDrainNs, 0)) {
+            atomicOr(p.error, 2);
+            *drained_flag = 0;
+          }
         }
       }
       __syncwarp();
@@ -520,11 +554,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       // values in uniform registers; one lane, always the same, issues.  Issued from a
       // one-lane branch instead, an MMA took about 80 cycles to hand over.)
       {
-        uint32_t ring = 0, qi = 0, np[2] = {0, 0};
+        uint32_t ring = 0, qi = 0, np[2] = {0, 0};  // ring: first chunk of the item
         bool ok = true;
         auto wait = [&](int i, uint32_t parity) -> bool {
           return __all_sync(0xffffffffu, bar_wait(bar(i), parity, limit_ns, abort_flag));
         };
+        auto ready = [&](int i, uint32_t parity) -> bool { return __all_sync(0xffffffffu, bar_test(bar(i), parity)); };
         auto full = [&](uint32_t r) -> bool {
           return wait(kBarFull + r % kStages, (r / kStages) & 1);
         };
@@ -580,24 +615,46 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (NC == 2) f = f && full(r + 1);
           return f;
         };
-        const Item* slot = reinterpret_cast<const Item*>(gbase + kOffItem);
-        while (ok) {
-          ok = wait(kBarQFull, qi++ & 1);
-          if (!ok) break;
-          const int n = __shfl_sync(0xffffffffu, slot->nkt, 0);
-          const bool few = D == 128 && (__shfl_sync(0xffffffffu, slot->flags, 0) & kFlagFew);
+        // tiles and mode of the item in slot i & 1
+        auto describe = [&](uint32_t i, int& tiles, bool& alternate) {
+          const Item* slot = reinterpret_cast<const Item*>(gbase + kOffItem + 64 * (i & 1));
+          tiles = __shfl_sync(0xffffffffu, slot->nkt, 0);
+          alternate = D == 256 || (__shfl_sync(0xffffffffu, slot->flags, 0) & kFlagFew);
+        };
+        // Alternating tiles: the scores of tile t of item i (first chunk r), into buffer b
+        auto alt_scores = [&](uint32_t i, int t, int n, int b, uint32_t r) {
+          const uint32_t rk = r + (uint32_t)(NC * k_index(t, 2));
+          fence_after();
+          scores(b, D == 256 ? 0 : (int)(i & 1), rk);
+          release(rk);
+          if (t + 1 == n) announce(kBarQEmpty + (i & 1));
+        };
+        int early = 0;      // score tiles of this item that were issued behind the last one's
+        uint32_t par = 0;   // score buffer of the item's first alternating tile
+        // What was read of the next item ahead of its turn is kept: once its scores are issued
+        // the slot may move on, and its phase could no longer be told from the next but one.
+        bool known = false, next_alt = false;
+        int next_n = 0;
+        for (;; qi++) {
+          int n = next_n;
+          bool alternate = next_alt;
+          if (!known) {
+            if (!(ok = wait(kBarQFull + (qi & 1), (qi >> 1) & 1))) break;
+            describe(qi, n, alternate);
+          }
+          known = false;
           if (n < 0) break;
           if (n == 0) {
-            if (lane == 0) bar_arrive(bar(kBarQEmpty));
+            if (lane == 0) bar_arrive(bar(kBarQEmpty + (qi & 1)));
             continue;
           }
-          if (D == 128 && !few) {
+          if (!alternate) {
             if (!(ok = full(ring))) break;
             fence_after();
             scores(0, 0, ring);
             scores(1, 1, ring);
             release(ring);
-            if (n == 1) announce(kBarQEmpty);
+            if (n == 1) announce(kBarQEmpty + (qi & 1));
             ring++;
             for (int t = 0; t < n && ok; t++) {
               const uint32_t rv = ring, rk = ring + 1;
@@ -615,42 +672,52 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!ok) break;
               release(rv);
               if (more) release(rk);
-              if (t + 2 == n) announce(kBarQEmpty);
+              if (t + 2 == n) announce(kBarQEmpty + (qi & 1));
               ring += more ? 2 : 1;
             }
+            if (!ok) break;
           } else {
-            for (int t = 0; t < 2 && t < n; t++) {
-              if (!(ok = full_tile(ring))) break;
-              fence_after();
-              scores(t, 0, ring);
-              release(ring);
-              ring += NC;
+            for (int t = early; t < 2 && t < n && ok; t++) {
+              if (!(ok = full_tile(ring + NC * k_index(t, 2)))) break;
+              alt_scores(qi, t, n, (par + t) & 1, ring);
             }
             if (!ok) break;
-            if (n <= 2) announce(kBarQEmpty);
+            early = 0;
+            const uint32_t next_ring = ring + (uint32_t)(2 * NC * n);
             for (int t = 0; t < n; t++) {
-              const int h = t & 1;
-              if (!(ok = full_tile(ring) && sums(h, D == 128 ? h : 0, ring, D == 128 ? t > 1 : t > 0))) break;
-              if (D == 256) announce(kBarPV + h);
-              release(ring);
-              ring += NC;
+              const int b = (par + t) & 1;
+              const uint32_t rv = ring + (uint32_t)(NC * v_index(t, n, 2));
+              if (!(ok = full_tile(rv) && sums(b, D == 128 ? b : 0, rv, D == 128 ? t > 1 : t > 0))) break;
+              if (D == 256) announce(kBarPV + b);
+              if (D == 256 ? t + 1 == n : t + 2 >= n) announce(kBarO + (D == 128 ? b : 0));
+              release(rv);
               if (t + 2 < n) {
-                if (!(ok = full_tile(ring))) break;
-                fence_after();
-                scores(h, 0, ring);
-                release(ring);
-                ring += NC;
-                if (t + 3 == n) announce(kBarQEmpty);
+                if (!(ok = full_tile(ring + NC * k_index(t + 2, 2)))) break;
+                alt_scores(qi, t + 2, n, b, ring);
+                continue;
+              }
+              // The next item's first scores fill the gap while this one's last softmax
+              // runs, if its Q and K are there already (nothing is waited for).
+              if (!known && ready(kBarQFull + ((qi + 1) & 1), ((qi + 1) >> 1) & 1)) {
+                describe(qi + 1, next_n, next_alt);
+                known = true;
+              }
+              for (; known && next_alt && early < t + 3 - n && early < next_n; early++) {
+                const uint32_t rk = next_ring + (uint32_t)(NC * k_index(early, 2));
+                if (!ready(kBarFull + rk % kStages, (rk / kStages) & 1) ||
+                    (NC == 2 && !ready(kBarFull + (rk + 1) % kStages, ((rk + 1) / kStages) & 1)))
+                  break;
+                alt_scores(qi + 1, early, next_n, (par + n + early) & 1, next_ring);
               }
             }
             if (!ok) break;
-            announce(kBarO);  // after the whole item: the merge may then overwrite Q
-            if (D == 128 && n > 1) announce(kBarO + 1);
+            par = (par + n) & 1;
+            ring = next_ring;
           }
         }
         if (!ok && lane == 0) fail();
         announce(kBarDrain);  // tracks every MMA issued before it
-        if (!bar_wait(bar(kBarDrain), 0, kDrainNs, nullptr) && lane == 0) {
+        if (!bar_wait(bar(kBarDrain), 0, kDrainNs, 0) && lane == 0) {
           atomicOr(p.error, 2);
           *drained_flag = 0;
         }
@@ -667,16 +734,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const int* lens = reinterpret_cast<const int*>(p.plan + p.lay.lens);
     const float c = p.scale * kLog2e;
-    const u64 c2 = pack2(c, c);
-    float* xs = reinterpret_cast<float*>(gbase + kOffX) + h * SP * 128 + r;  // [warpgroup][row]
-    float* o_s = reinterpret_cast<float*>(gbase);  // few rows: half 1's sums, [column][row]
+    const uint32_t xs = base + kOffX + (uint32_t)(h * SP * 128 + r) * 4;  // [warpgroup][row]
     const int xbar = kBarX + h * 4 + (warp & 3);
-    uint32_t ns[2] = {0, 0}, no = 0, nm = 0, npv[2] = {0, 0}, ring0 = 0, qi = 0, nx = 0;
+    uint32_t ns[2] = {0, 0}, no = 0, npv[2] = {0, 0}, ring0 = 0, qi = 0, nx = 0, par = 0;
     bool ok = true, unread = false;
     auto wait = [&](int i, uint32_t parity) {
       return __all_sync(0xffffffffu, bar_wait(bar(i), parity, limit_ns, abort_flag));
     };
-    // xs[128 j] = warpgroup j's value, for all j.  The next values overwrite these: within an
+    // Warpgroup j's value of this row is at xs + 512 j.  The next values overwrite these: within an
     // item they follow the scores of the next tile, which every partner's probabilities
     // precede; behind the item's last exchange each warp reports that it has read them
     // (unread: that report is still to be awaited).
@@ -685,42 +750,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait(xbar, nx++ & 1)) return false;
         unread = false;
       }
-      xs[128 * sp] = v;
+      stsf(xs + 512 * sp, v);
       __syncwarp();
       if (lane == 0) bar_arrive(bar(xbar));
       return wait(xbar, nx++ & 1);
     };
-    const int local_row = r / g, head_row = r % g;
-    const bool row_used = r < g * p.lay.half_tok;
-    while (ok) {
-      if (!(ok = wait(kBarQFull, qi++ & 1))) break;
-      const Item it = *reinterpret_cast<const Item*>(gbase + kOffItem);
-      const int kvh = *reinterpret_cast<const int*>(gbase + kOffItem + sizeof(Item));
+    for (;; qi++) {
+      const int q = qi & 1;
+      if (!(ok = wait(kBarQFull + q, (qi >> 1) & 1))) break;
+      const Item it = *reinterpret_cast<const Item*>(gbase + kOffItem + 64 * q);
+      const int kvh = *reinterpret_cast<const int*>(gbase + kOffItem + 64 * q + sizeof(Item));
       const int n = it.nkt;
       if (n < 0) break;
+      __syncwarp();
+      if (lane == 0) bar_arrive(bar(kBarQEmpty + q));  // this warp is done with the slot
       const bool few = D == 128 && (it.flags & kFlagFew), alt = D == 256 || few;
-      const int local = local_row + (D == 128 && !few ? h * p.lay.half_tok : 0);
-      const int tok = it.tok0 + local, head = kvh * g + head_row;
-      const bool valid = row_used && local < it.ntok && tok < p.tokens;
+      // alternating tiles: the item's tile t is in score buffer (par + t) & 1; few rows: this
+      // half has the tiles of its own buffer, t0, t0 + 2 ..
+      const int t0 = few ? (int)(h ^ par) : 0;
+      const int local = r / g + (D == 128 && !few ? h * p.lay.half_tok : 0);  // token of the item
+      const bool valid = r < g * p.lay.half_tok && local < it.ntok && it.tok0 + local < p.tokens;
       const int2 kk = valid ? row_keys(it, lens, p.window, local) : make_int2(0, 0);
       const bool any_valid = __any_sync(0xffffffffu, valid);
       // keys that some row (lo0, hi1) / every row (lo1, hi0) of the warp sees
       const int lo0 = warp_min_i(valid ? kk.x : INT_MAX), lo1 = -warp_min_i(valid ? -kk.x : INT_MAX);
       const int hi0 = warp_min_i(valid ? kk.y : INT_MAX), hi1 = -warp_min_i(valid ? -kk.y : INT_MAX);
-      // head_dim 256: the sums of tile t are done.  Even and odd tiles have a barrier each:
-      // a parity tells a phase from its neighbours only, and when the sums of tile t are
-      // asked for (by the softmax of tile t + 1) those of tile t - 2 were announced before
-      // the scores of tile t, and those of tile t + 2 cannot have begun.
-      auto sums_done = [&](int t) { return wait(kBarPV + (t & 1), (npv[t & 1] + (uint32_t)(t >> 1)) & 1); };
+      // head_dim 256: the sums of tile t are done.  The two score buffers' tiles have a
+      // barrier each: a parity tells a phase from its neighbours only, and when the sums of
+      // tile t are asked for (by the softmax of tile t + 1) those of tile t - 2 were announced
+      // before the scores of tile t, and those of tile t + 2 cannot have begun.
+      auto sums_done = [&](int t) {
+        const uint32_t b = (par + t) & 1;
+        return wait(kBarPV + b, (npv[b] + (uint32_t)(t >> 1)) & 1);
+      };
       float m = -INFINITY, l = 0.0f;
-      // this warp is done with the item slot, and with Q's buffer unless sums pass through it
-      if (n == 0 || !few || (h == 1 && n == 1)) {
-        __syncwarp();
-        if (lane == 0) bar_arrive(bar(kBarQEmpty));
-      }
       const uint32_t ob = lanes + kColO + (D == 128 ? h * 128 : 0) + sp * 64;
-      for (int t = few ? h : 0; t < n; t += few ? 2 : 1) {
-        const int b = D == 256 ? (t & 1) : h;  // score buffer
+      for (int t = t0; t < n; t += few ? 2 : 1) {
+        const int b = D == 256 ? (int)((par + t) & 1) : h;  // score buffer
         const bool first = few ? t < 2 : t == 0;
         const uint32_t sb = lanes + kColS + b * 128;
         if (!(ok = wait(kBarS + b, ns[b]++ & 1))) break;
@@ -781,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (!(ok = exchange(mn))) break;
 #pragma unroll
-          for (int j = 0; j < SP; j++) mn = fmaxf(mn, xs[128 * j]);
+          for (int j = 0; j < SP; j++) mn = fmaxf(mn, ldsf(xs + 512 * j));
           mn = fmaxf(m, mn);
           if (first) {
             m = mn;
@@ -803,7 +869,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           const float neg = m == -INFINITY ? 0.0f : -m * c;
-          const u64 neg2 = pack2(neg, neg);
+          const u64 neg2 = pack2(neg, neg), c2 = pack2(c, c);
           u64 sum[2] = {0, 0};
 #pragma unroll
           for (int q = 0; q < NQ; q++) {
@@ -830,16 +896,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       ring0 += (uint32_t)(2 * NC * n);
-      npv[0] += (uint32_t)((n + 1) >> 1);
-      npv[1] += (uint32_t)(n >> 1);
+      npv[par] += (uint32_t)((n + 1) >> 1);
+      npv[par ^ 1] += (uint32_t)(n >> 1);
+      if (alt) par = (par + n) & 1;
       // -------------------------------------------------------------- epilogue
-      const int mine = few ? (n + 1 - h) / 2 : n;  // this half's tiles
+      const int mine = few ? (n + 1 - t0) / 2 : n;  // this half's tiles
       if (mine > 0) {
         if (any_valid) {  // the row's sum over all columns, added in warpgroup order
           if (!(ok = exchange(l))) break;
           l = 0.0f;
 #pragma unroll
-          for (int j = 0; j < SP; j++) l += xs[128 * j];
+          for (int j = 0; j < SP; j++) l += ldsf(xs + 512 * j);
           __syncwarp();
           if (lane == 0) bar_arrive(bar(xbar));
           unread = true;
@@ -847,59 +914,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = wait(kBarO + h, no++ & 1))) break;
         fence_after();
       }
-      if (few && h == 1) {  // hand the odd tiles' sums over
-        if (mine > 0) {
-          if (any_valid) {
-#pragma unroll 1
-            for (int i = 0; i < 4; i++) {
-              float o[16];
-              tm_load16(ob + 16 * i, o);
-#pragma unroll
-              for (int j = 0; j < 16; j++) o_s[(sp * 64 + 16 * i + j) * 128 + r] = o[j];
-            }
-            if (!(ok = wait(xbar, nx++ & 1))) break;
-            unread = false;
-            if (sp == 0) {
-              xs[0] = m;
-              xs[128] = l;
-            }
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (Q is loaded over it next)
-          __syncwarp();
-          if (lane == 0) {
-            bar_arrive(bar(kBarMerge));
-            bar_arrive(bar(kBarQEmpty));
-          }
-        }
-        continue;
-      }
-      float f0 = 1.0f, f1 = 0.0f;
-      const bool merge = few && n > 1;
-      if (merge) {
-        if (!(ok = wait(kBarMerge, nm++ & 1))) break;
-        if (any_valid) {
-          const float m1 = xs[SP * 128], l1 = xs[SP * 128 + 128];
-          const float M = fmaxf(m, m1);
-          if (M != -INFINITY) {
-            f0 = ex2((m - M) * c);
-            f1 = ex2((m1 - M) * c);
-          }
-          l = l * f0 + l1 * f1;
-          m = M;
-        }
-      }
       if (any_valid) {
+        const int head_row = r % g, tok = it.tok0 + local, head = kvh * g + head_row;
         const float inv = 1.0f / l;
-        const int64_t prow = (int64_t)(it.part + local * g + head_row) * p.nkv + kvh;
+        // (few rows: the even tiles' part, then the odd ones')
+        const int64_t prow = (int64_t)(it.part + (t0 * it.ntok + local) * g + head_row) * p.nkv + kvh;
 #pragma unroll 1
         for (int i = 0; i < 4; i++) {
           const int col = sp * 64 + 16 * i;
           float o[16];
-          if (n > 0) tm_load16(ob + 16 * i, o);
-          if (merge) {
-#pragma unroll
-            for (int j = 0; j < 16; j++) o[j] = o[j] * f0 + o_s[(col + j) * 128 + r] * f1;
-          }
+          if (mine > 0) tm_load16(ob + 16 * i, o);
           if (valid && it.part < 0) {
             uint32_t v[8];
 #pragma unroll
@@ -914,11 +938,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();  // (the next load is the whole warp's)
         }
         if (valid && it.part >= 0 && sp == 0) p.part_ml[prow] = make_float2(m * c, l);
-      }
-      if (few && n > 0) {  // Q's buffer may be loaded once all warps have read the hand-over
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) bar_arrive(bar(kBarQEmpty));
       }
     }
     if (!ok) fail();

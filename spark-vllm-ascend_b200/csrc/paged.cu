@@ -42,8 +42,9 @@ static int attn_launch(const paged::AttnArgs& p, int64_t wait_ns, cudaStream_t s
   if (st) return st;
   // one row of a join per warp and pass; the device knows how many there are
   const int64_t join_rows = (int64_t)p.lay.max_entries * p.nkv * std::min(p.lay.tile_tok, p.tokens) * g;
-  const int cgrid = (int)std::min<int64_t>((join_rows + 7) / 8, 4LL * num_sms());
-  return launch(paged::combine_kernel<D>, dim3(cgrid), dim3(256), 0, stream, p);
+  const int per_cta = paged::kJoinThreads / 32;
+  const int cgrid = (int)std::min<int64_t>((join_rows + per_cta - 1) / per_cta, 4LL * num_sms());
+  return launch(paged::combine_kernel<D>, dim3(cgrid), dim3(paged::kJoinThreads), 0, stream, p);
 }
 
 extern "C" {
@@ -110,7 +111,9 @@ static int check_attn_shape(int max_tokens, int max_reqs, int nq, int nkv, int h
       (head_dim != 128 && head_dim != 256))
     return SPARK_ERR_UNSUPPORTED_SHAPE;
   // tile, item and partial-row counts are 32-bit
-  if (max_tokens > (1 << 22) || max_reqs > (1 << 16) || nkv > 4096) return SPARK_ERR_TOO_LARGE;
+  if (max_tokens > (1 << 22) || max_reqs > (1 << 16) || nkv > 4096 ||
+      (int64_t)paged::layout_of(max_tokens, max_reqs, nq, nkv, head_dim).max_items * nkv > (1 << 30))
+    return SPARK_ERR_TOO_LARGE;
   return SPARK_OK;
 }
 

@@ -376,7 +376,7 @@ struct alignas(16) Item {
   int part;         // first partial row, or -1: the part is the whole tile
   int pad;
 };
-constexpr int kFlagFew = 1;   // the tokens fit half a tile: the two halves take alternate key tiles
+constexpr int kFlagFew = 1;   // the tokens fit half a tile: the two halves take alternate key tiles, a part each
 constexpr int kFlagLens = 2;  // row limits are the requests' lengths (shared prefix), not causal
 static_assert(sizeof(Item) == 48, "items are three 16-byte words");
 
@@ -406,9 +406,9 @@ __host__ __device__ inline Layout layout_of(int T, int R, int nq, int nkv, int D
   l.max_tiles = tk / l.tile_tok + R + 1;
   l.budget = 4 * kNumSMs / nkv + 1;
   l.max_items = l.max_tiles + l.budget;
-  l.max_entries = R > l.budget ? R : l.budget;
+  l.max_entries = R + l.budget;
   const int64_t rows = l.tile_tok < tk ? l.tile_tok : tk;
-  l.part_rows = (int)((2 * (int64_t)l.budget * rows + 2 * (int64_t)R) * g);
+  l.part_rows = (int)((2 * (int64_t)l.budget * rows + 4 * (int64_t)R) * g);
   int64_t at = 0;  // every array starts on a 16-byte boundary
   auto take = [&at](int64_t bytes) {
     const int64_t o = at;
@@ -456,7 +456,7 @@ __device__ __forceinline__ Tile prompt_tile(const AttnPlanArgs& p, int q0, int n
   t.klo = lo < 0 ? 0 : lo;
   t.key0 = t.klo / kKeyTile * kKeyTile;
   t.nkt = t.khi > t.klo ? (t.khi - t.key0 + kKeyTile - 1) / kKeyTile : 0;
-  t.flags = p.D == 128 && t.ntok <= p.lay.half_tok ? kFlagFew : 0;
+  t.flags = p.D == 128 && t.ntok <= p.lay.half_tok && t.nkt > 1 ? kFlagFew : 0;
   return t;
 }
 
@@ -478,15 +478,15 @@ __device__ __forceinline__ Tile prefix_tile(const AttnPlanArgs& p, const int* le
   }
   t.key0 = t.klo / kKeyTile * kKeyTile;
   t.nkt = t.khi > t.klo ? (t.khi - t.key0 + kKeyTile - 1) / kKeyTile : 0;
-  if (p.D == 128 && t.ntok <= p.lay.half_tok) t.flags |= kFlagFew;
+  if (p.D == 128 && t.ntok <= p.lay.half_tok && t.nkt > 1) t.flags |= kFlagFew;
   return t;
 }
 
 // Cost of a part in quarters of a key tile of many rows: the tiles (alternating halves take
 // two at a time), what an item costs around them, and for a part that is joined the fp32
 // sums of its rows.  Measured with the attention kernel: see there.
-__host__ __device__ inline int part_cost(int flags, int parts, int tiles, int ntok) {
-  return tiles * ((flags & kFlagFew) ? 2 : 4) + 6 + (parts > 1 && !(flags & kFlagFew) ? 6 : 0);
+__host__ __device__ inline int part_cost(int flags, int parts, int tiles, int rows) {
+  return tiles * ((flags & kFlagFew) ? 2 : 4) + 8 + (parts > 1 ? rows / 32 : 0);
 }
 constexpr int kPriceBins = 256;
 __device__ __forceinline__ int price_bin(int cost, int top) {
@@ -556,36 +556,49 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
     nt = (int)sum;
   }
   __syncthreads();
+  bool allow_few = true;
   auto tile_at = [&](int i) {
     if (prefix_kind) return prefix_tile(p, lens, prefix, npre, i);
     const int2 t = tiles[i];
     const int q0 = p.query_start[t.x];
-    return prompt_tile(p, q0, p.query_start[t.x + 1] - q0, lens[t.x], t.x, t.y);
+    Tile tile = prompt_tile(p, q0, p.query_start[t.x + 1] - q0, lens[t.x], t.x, t.y);
+    if (!allow_few) tile.flags = 0;
+    return tile;
   };
-  int longest = 0;
+  const int g = p.nq / p.nkv;
+  int longest = 0, few_rows = 0;
   for (int i = tid; i < nt; i += kAttnPlanThreads) {
     if (!prefix_kind) {
       const int r = find_request(starts, R, i);
       tiles[i] = make_int2(r, i - starts[r]);
     }
-    const int k = tile_at(i).nkt;
-    longest = k > longest ? k : longest;
+    const Tile t = tile_at(i);
+    longest = t.nkt > longest ? t.nkt : longest;
+    if (t.flags & kFlagFew) few_rows += 2 * t.ntok * g;
   }
-  for (int o = 16; o >= 1; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-  if ((tid & 31) == 0) ws[tid >> 5] = longest;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  few_rows = __reduce_add_sync(0xffffffffu, few_rows);
+  if ((tid & 31) == 0) {
+    ws[tid >> 5] = longest;
+    ws2[tid >> 5][0] = few_rows;
+  }
   __syncthreads();
-  for (int w = 0; w < kAttnPlanThreads / 32; w++) longest = max(longest, ws[w]);
+  longest = __reduce_max_sync(0xffffffffu, ws[tid & 31]);
+  long long few_all = 0;
+  for (int w = 0; w < kAttnPlanThreads / 32; w++) few_all += ws2[w][0];
+  __syncthreads();
+  // many requests of some tokens each: enough tiles without, and their parts would not fit
+  if (!prefix_kind && few_all > p.lay.part_rows / 2) allow_few = false;
   // How fine to cut: warp w prices "the longest tile in kCuts[w] parts, the others in parts
   // no longer than those" by dealing the parts out as the attention kernel will.  (A batch of
   // more than 8192 tiles balances without.)
-  const int g = p.nq / p.nkv;
   int cut = longest > 0 ? longest : 1;
   if (nt <= 8192 && longest > 1) {
     const int w = tid >> 5, lane = tid & 31;
     const int c = (longest + kCuts[w] - 1) / kCuts[w];
     int* h = price + w * (kPriceBins + 1);
     for (int b = lane; b <= kPriceBins; b += 32) h[b] = 0;
-    const int top = part_cost(0, 2, c, p.lay.tile_tok);  // (no part costs more)
+    const int top = part_cost(0, 2, c, p.lay.tile_tok * g);  // (no part costs more)
     __syncwarp();
     int extra = 0, rows = 0;
     for (int i = lane; i < nt; i += 32) {
@@ -593,10 +606,11 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
       const int np = (t.nkt + c - 1) / c;
       if (np == 0) continue;
       extra += np - 1;
-      if (np > 1 || prefix_kind) rows += np * t.ntok * g;
+      const int each = (t.flags & kFlagFew) ? 2 : 1;
+      if (np > 1 || prefix_kind || each == 2) rows += each * np * t.ntok * g;
       const int lo = t.nkt / np, more = t.nkt - lo * np;  // `more` parts have one tile more
       const int joined = prefix_kind ? 2 : np;
-      const int c0 = part_cost(t.flags, joined, lo, t.ntok), c1 = part_cost(t.flags, joined, lo + 1, t.ntok);
+      const int c0 = part_cost(t.flags, joined, lo, t.ntok * g), c1 = part_cost(t.flags, joined, lo + 1, t.ntok * g);
       if (np > more) atomicAdd(&h[price_bin(c0, top)], (np - more) * p.nkv);
       if (more) atomicAdd(&h[price_bin(c1, top)], more * p.nkv);
     }
@@ -658,23 +672,24 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
   // matter to any result)
   for (int b = tid; b < kBins; b += kAttnPlanThreads) hist[b] = 0;
   __syncthreads();
-  const int top = part_cost(0, 2, cut, p.lay.tile_tok);
+  const int top = part_cost(0, 2, cut, p.lay.tile_tok * g);
   auto bin_of = [&](const Tile& t, int joined, int keys) {
-    return kBins - 1 - (int)((long long)min(part_cost(t.flags, joined, keys, t.ntok), top) * (kBins - 1) / top);
+    return kBins - 1 - (int)((long long)min(part_cost(t.flags, joined, keys, t.ntok * g), top) * (kBins - 1) / top);
   };
   for (int pass = 0; pass < 2; pass++) {
     for (int i = tid; i < nt; i += kAttnPlanThreads) {
       const Tile t = tile_at(i);
       int np = (t.nkt + cut - 1) / cut;
       if (np == 0 && !prefix_kind) np = 1;  // rows without keys are written as zeros
-      const bool parts = np > 1 || prefix_kind;
+      const int each = (t.flags & kFlagFew) ? 2 : 1;
+      const bool parts = np > 1 || prefix_kind || each == 2;
       int base = -1;
       if (pass == 1) {
-        if (parts) base = atomicAdd(&rows_s, np * t.ntok * g);
-        bases[i] = make_int2(base, np);
+        if (parts) base = atomicAdd(&rows_s, each * np * t.ntok * g);
+        bases[i] = make_int2(base, each * np);
         if (parts && !prefix_kind) {
           const int e = atomicAdd(&entries_s, 1);
-          entries[e] = {t.tok0, t.ntok, base, np, t.ntok * g, 0, 0, 0};
+          entries[e] = {t.tok0, t.ntok, base, each * np, t.ntok * g, 0, 0, 0};
           atomicMax(&join_s, t.ntok * g);
         }
       }
@@ -689,7 +704,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
           it.klo = a ? it.key0 : t.klo;
           it.khi = k + 1 < np ? t.key0 + b * kKeyTile : t.khi;
           it.len = t.len, it.flags = t.flags;
-          it.part = parts ? base + k * t.ntok * g : -1;
+          it.part = parts ? base + k * each * t.ntok * g : -1;
           it.pad = 0;
           items[slot] = it;
         }
@@ -759,16 +774,18 @@ __device__ __forceinline__ int2 row_keys(const Item& it, const int* lens, int wi
 // the parts in list order whatever order they were computed in.  A row without any key is
 // zero.  One warp per row: lanes hold 32 parts' (m, l) at a time, then the warp adds the
 // parts' sums, four in flight.
+constexpr int kJoinThreads = 256;
+
 template <int D>
-__global__ void __launch_bounds__(256) combine_kernel(AttnArgs p) {
+__global__ void __launch_bounds__(kJoinThreads) combine_kernel(AttnArgs p) {
   constexpr int E = D / 32;  // elements of a lane, contiguous
   pdl_wait();
   const Header* hdr = reinterpret_cast<const Header*>(p.plan);
   const Entry* entries = reinterpret_cast<const Entry*>(p.plan + p.lay.entries);
   const int g = p.nq / p.nkv, lane = threadIdx.x & 31;
   const int n = hdr->entries, jr = hdr->join_rows;
-  const int64_t total = (int64_t)n * p.nkv * jr, step = (int64_t)gridDim.x * 8;
-  for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += step) {
+  const int64_t total = (int64_t)n * p.nkv * jr, step = (int64_t)gridDim.x * (kJoinThreads / 32);
+  for (int64_t w = (int64_t)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5); w < total; w += step) {
     const int row = (int)(w % jr);
     const int64_t x = w / jr;
     const int kvh = (int)(x % p.nkv);
