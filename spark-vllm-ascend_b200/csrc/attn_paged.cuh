@@ -63,8 +63,10 @@ namespace paged {
 namespace tc {
 
 constexpr int kThreads = 640;
-// registers: 96 a thread at launch; warps 16-19 give up 32 each, the softmax warps take 8
-// (4 x 104 + 64 = 5 x 96)
+// registers: 96 a thread at launch; for head_dim 128 warps 16-19 give up 32 each and the
+// softmax warps take 8 (4 x 104 + 64 = 5 x 96): a spill in the softmax loop costs the shared
+// memory bandwidth that the MMAs live on (150 bytes: a third more time).  For head_dim 256 a
+// softmax thread has half as many scores and 96 do.
 constexpr int kRegsLaunch = 96, kRegsSoftmax = 104, kRegsRest = 64;
 constexpr int kSoftmaxWarps = 16;
 constexpr int kProducerWarp = 16, kMmaWarp = 17, kQWarp = 18;
@@ -289,15 +291,16 @@ __device__ __forceinline__ u64 ex2_poly(u64 x2) {
   return pack2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(n) << 23)),
                __uint_as_float(__float_as_uint(b) + (__float_as_uint(k) << 23)));
 }
-// p = 2^(s c + neg) of 32 scores: sums in fp32, the bf16 pairs to pk.  kPoly of 16 pairs go
-// through ex2_poly.
+// p = 2^(s c + neg) of 16 scores: sums in fp32, the bf16 pairs to tensor memory.  kPoly of the
+// 8 pairs go through ex2_poly.
 template <int kPoly>
-__device__ __forceinline__ void probs32(const float* s, u64 c2, u64 neg2, u64 (&sum)[2], uint32_t (&pk)[16]) {
+__device__ __forceinline__ void probs16(const float* s, u64 c2, u64 neg2, u64 (&sum)[2], uint32_t addr) {
+  uint32_t pk[8];
 #pragma unroll
-  for (int i = 0; i < 16; i++) {
+  for (int i = 0; i < 8; i++) {
     u64 x2 = fma2(pack2(s[2 * i], s[2 * i + 1]), c2, neg2);
     float x, y;
-    if ((i * kPoly) / 16 != ((i + 1) * kPoly) / 16) {  // (kPoly pairs, evenly spread)
+    if ((i * kPoly) / 8 != ((i + 1) * kPoly) / 8) {  // (kPoly pairs, evenly spread)
       x2 = ex2_poly(x2);
       unpack2(x2, x, y);
     } else {
@@ -309,8 +312,11 @@ __device__ __forceinline__ void probs32(const float* s, u64 c2, u64 neg2, u64 (&
     sum[i & 1] = add2(sum[i & 1], x2);
     pk[i] = pack_bf16(x, y);
   }
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(pk[0]), "r"(pk[1]),
+               "r"(pk[2]), "r"(pk[3]), "r"(pk[4]), "r"(pk[5]), "r"(pk[6]), "r"(pk[7]), "r"(addr)
+               : "memory");
 }
-constexpr int kPolyPairs = 4;
+constexpr int kPolyPairs = 2;
 
 // 32 bytes (wide) or two times 16 to global memory
 __device__ __forceinline__ void store32(void* dst, const uint32_t* v, bool wide) {
@@ -416,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // (each warpgroup changes its share inside its own branch, where the register allocator
   // can tell which share holds)
   if (warp >= kSoftmaxWarps) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+    if (D == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
     if (warp == kProducerWarp) {
       // ---------------------------------------------------------------- K / V producer
       uint32_t ring = 0;
@@ -725,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    if (D == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ---------------------------------------------------------------- softmax and epilogue
     // SP warpgroups share the rows of a half (a thread of each owns the same row), 128 / SP
     // score columns and 64 sum columns each
@@ -873,11 +879,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           u64 sum[2] = {0, 0};
 #pragma unroll
           for (int q = 0; q < NQ; q++) {
-            uint32_t pk[16];
             if (q > 0) load(q);
-            if (edge) probs32<0>(s, c2, neg2, sum, pk);
-            else probs32<kPolyPairs>(s, c2, neg2, sum, pk);
-            tm_store16(sb + 64 * q + 32 * sp, pk);
+            const uint32_t pb = sb + 64 * q + 32 * sp;
+            if (edge) {
+              probs16<0>(s, c2, neg2, sum, pb);
+              probs16<0>(s + 16, c2, neg2, sum, pb + 8);
+            } else {
+              probs16<kPolyPairs>(s, c2, neg2, sum, pb);
+              probs16<kPolyPairs>(s + 16, c2, neg2, sum, pb + 8);
+            }
             announce(D == 128 ? q : sp >> 1);
           }
           float s0, s1;

@@ -33,7 +33,7 @@ static int attn_launch(const paged::AttnArgs& p, int64_t wait_ns, cudaStream_t s
   static const bool split_ok = [] {
     cudaFuncAttributes fa;
     return cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(&paged::tc::attn_kernel<D>)) == cudaSuccess &&
-           fa.numRegs >= paged::tc::kRegsLaunch;
+           (D != 128 || fa.numRegs >= paged::tc::kRegsLaunch);
   }();
   if (!split_ok) return SPARK_ERR_LAUNCH;
   const int grid = (int)std::min<int64_t>((int64_t)p.lay.max_items * p.nkv, num_sms());
