@@ -189,14 +189,23 @@ class BatchDecodeEngine:
     def set_positions(self, pos) -> None:
         self.pos.copy_(torch.as_tensor(pos, dtype=torch.int64).reshape(self.batch))
 
-    def prefill(self, prompts, chunk: int = 2048) -> torch.Tensor:
+    def prefill(self, prompts, chunk: int = 2048, packed: bool = False) -> torch.Tensor:
         """Prefill each sequence's prompt (``spark_b200.prefill``: tensor-core GEMMs over the
-        Q4_0 weights, causal attention, K / V into the sequence's own blocks).  Returns the first
-        generated token of every sequence (int32 [B])."""
-        from .prefill import prefill
+        Q4_0 weights, causal attention, K / V into the sequence's own blocks).  ``packed``: all
+        prompts in one batch of rows (``prefill_packed``; ``chunk`` rows per sequence at a time),
+        else one after the other.  Returns the first generated token of every sequence
+        (int32 [B])."""
+        from .prefill import prefill, prefill_packed
         if len(prompts) != self.batch:
             raise ValueError(f"{len(prompts)} prompts for batch {self.batch}")
         self.reset_counters()
+        if packed:
+            self.logits.copy_(prefill_packed(self, prompts, self.block_tables, chunk * self.batch))
+            self.token.copy_(torch.argmax(self.logits.float(), dim=-1))
+            self.pos.copy_(torch.tensor([len(p) for p in prompts], dtype=torch.int64))
+            self.step_idx.zero_()
+            self.key.zero_()
+            return self.token.clone()
         for b, p in enumerate(prompts):
             prefill(_SeqView(self, b), torch.as_tensor(p), chunk)
         self.step_idx.zero_()
@@ -219,9 +228,9 @@ class BatchDecodeEngine:
             self.step()
         return self.token.clone()
 
-    def generate(self, prompts, max_new_tokens: int, stepwise: bool = False) -> list[list[int]]:
+    def generate(self, prompts, max_new_tokens: int, stepwise: bool = False, packed: bool = False) -> list[list[int]]:
         """Greedy decode of every sequence; returns the generated ids per sequence."""
-        first = self.prefill_stepwise(prompts) if stepwise else self.prefill(prompts)
+        first = self.prefill_stepwise(prompts) if stepwise else self.prefill(prompts, packed=packed)
         self.step_idx.zero_()
         for _ in range(max_new_tokens - 1):
             self.step()

@@ -12,6 +12,9 @@ torch or CUDA.  ``register()`` then wires, lazily:
   (paged split-KV decode attention over BF16 K / V, 128-token pages stored one
   (block, kv head) page contiguous).
 
+Set ``SPARK_B200_PAGED_ATTENTION=1`` to run prompts, mixed batches and common prefixes on
+the paged attention kernel (plugin/attention.py).
+
 Set ``SPARK_B200_PLUGIN_DISABLE=1`` to make ``register()`` stand down (the reference's
 override switch, inverted: this plugin adds kernels, not a model architecture).
 """

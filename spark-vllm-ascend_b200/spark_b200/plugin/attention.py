@@ -19,12 +19,19 @@ metadata to the sm_100a kernels:
   positions, the current one included, as the reference's kernel does (it masks below
   len - 513 for its 512-window layers, kernels/attention.py:124-127);
 * prefill (query length > 1) is not on the decode hot path: causal attention in torch
-  over the request's gathered pages, on the GPU.
+  over the request's gathered pages, on the GPU;
+* with ``SPARK_B200_PAGED_ATTENTION=1`` every step that is not all single tokens (prompts,
+  chunks, mixed batches) runs the paged attention kernel instead (``ops.attn_prompt_out``:
+  one launch for all requests, reading the pages in place, no host copy of the lengths), and
+  the backend asks vLLM for cascade attention, so that decode batches with a common prefix
+  read it once (``ops.attn_shared_prefix_out``).  Off by default: its outputs differ from
+  the torch path's in the last bf16 bit.
 """
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
+import os
+from dataclasses import dataclass, field
 from typing import ClassVar
 
 import ctypes
@@ -37,7 +44,12 @@ from .. import ops
 
 BLOCK_SIZE = 128
 HEAD_SIZE = 128
+PAGED_ENV = "SPARK_B200_PAGED_ATTENTION"
 HEAD_SIZES = (128, 256)  # 256: the persistent kernel's attention stage (the Spark model)
+
+
+def paged_attention() -> bool:
+    return os.environ.get(PAGED_ENV, "").strip().lower() in ("1", "true", "yes", "on")
 
 
 def choose_splits(max_model_len: int) -> int:
@@ -63,6 +75,9 @@ class SparkAttentionMetadata:
     slot_mapping: torch.Tensor  # int64 [num_tokens]
     splits: int
     max_split_tokens: int
+    prefix_len: torch.Tensor | None = None  # int32 [1]: positions all requests share (cascade)
+    plans: dict = field(default_factory=dict)  # this step's attention work lists, per head layout and window
+    plan_pool: dict = field(default_factory=dict)  # their buffers, kept by the builder from step to step
 
     @property
     def is_decode(self) -> bool:
@@ -77,11 +92,25 @@ class SparkAttentionMetadataBuilder(AttentionMetadataBuilder[SparkAttentionMetad
         max_len = vllm_config.model_config.max_model_len if vllm_config is not None else 4096
         self.splits = choose_splits(max_len)
         self.max_split_tokens = split_tokens(max_len, self.splits)
+        self.plan_pool: dict = {}
+
+    def use_cascade_attention(self, common_prefix_len: int, query_lens, num_query_heads: int, num_kv_heads: int,
+                              use_alibi: bool, use_sliding_window: bool, use_local_attention: bool, num_sms: int,
+                              dcp_world_size: int) -> bool:
+        """Single-token decode of two requests or more behind at least a page in common (the
+        per-request path launches once per request and reads the prefix each time)."""
+        return (paged_attention() and common_prefix_len >= BLOCK_SIZE and len(query_lens) > 1 and
+                all(int(n) == 1 for n in query_lens) and not (use_alibi or use_sliding_window or use_local_attention)
+                and dcp_world_size == 1)
 
     def build(self, common_prefix_len: int, common_attn_metadata: CommonAttentionMetadata,
               fast_build: bool = False) -> SparkAttentionMetadata:
         cm = common_attn_metadata
+        prefix = None
+        if common_prefix_len > 0:
+            prefix = torch.full((1,), common_prefix_len, dtype=torch.int32, device=cm.seq_lens.device)
         return SparkAttentionMetadata(
+            prefix_len=prefix, plan_pool=self.plan_pool if hasattr(self, "plan_pool") else {},
             num_actual_tokens=cm.num_actual_tokens, num_reqs=cm.num_reqs, max_query_len=cm.max_query_len,
             max_seq_len=cm.max_seq_len, query_start_loc=cm.query_start_loc, query_start_loc_cpu=cm.query_start_loc_cpu,
             seq_lens=cm.seq_lens, block_table=cm.block_table_tensor, slot_mapping=cm.slot_mapping,
@@ -115,6 +144,8 @@ class SparkAttentionImpl(AttentionImpl[SparkAttentionMetadata]):
         self.window = sliding_window + 1 if sliding_window is not None else 0
         self._ws: dict = {}
         self._step = None
+        self._paged = paged_attention()
+        self._error: dict = {}
 
     def _workspace(self, splits: int, device) -> tuple:
         key = (splits, device)
@@ -141,6 +172,8 @@ class SparkAttentionImpl(AttentionImpl[SparkAttentionMetadata]):
         if self.kv_sharing_target_layer_name is None and key is not None:
             ops.kv_store_(key[:t].view(t, nkv, d), value[:t].view(t, nkv, d), md.slot_mapping[:t], k_cache, v_cache)
         out = output[:t].view(t, nq, d)
+        if self._paged and (not md.is_decode or (md.prefix_len is not None and not self.window)):
+            return self._paged_attention(q, k_cache, v_cache, md, out, output)
         if md.is_decode and (d != HEAD_SIZE or self.window):
             return self._decode_step(q, key, value, k_cache, v_cache, md, out, output)
         if md.is_decode:
@@ -151,6 +184,33 @@ class SparkAttentionImpl(AttentionImpl[SparkAttentionMetadata]):
                                     error=err)
             return output
         return self._prefill(q, k_cache, v_cache, md, out, output)
+
+    def _plan(self, md, device):
+        """This step's work list: made by the first layer of a head layout and window, used
+        by the others."""
+        key = (self.num_heads, self.num_kv_heads, self.head_size, self.window)
+        plan = md.plans.get(key)
+        if plan is None:
+            tokens, reqs = max(md.num_actual_tokens, md.num_reqs), md.num_reqs
+            plan = md.plan_pool.get(key)
+            if plan is None or plan.max_tokens < tokens or plan.max_reqs < reqs:
+                room = lambda n: 1 << max(n - 1, 63).bit_length()  # noqa: E731
+                plan = md.plan_pool[key] = ops.AttnPlan(room(tokens), room(reqs), *key[:3], device, self.window)
+            if md.is_decode and md.prefix_len is not None and not self.window:
+                plan.update_prefix(md.seq_lens[:reqs], md.prefix_len)
+            else:
+                plan.update(md.query_start_loc[:reqs + 1], md.seq_lens[:reqs])
+            md.plans[key] = plan
+        return plan
+
+    def _paged_attention(self, q, k_cache, v_cache, md, out, output):
+        err = self._error.get(q.device)
+        if err is None:
+            err = self._error[q.device] = torch.zeros(1, dtype=torch.int32, device=q.device)
+        plan = self._plan(md, q.device)
+        attend = ops.attn_prompt_out if plan.kind == "prompt" else ops.attn_shared_prefix_out
+        attend(q, k_cache, v_cache, md.block_table, plan, self.scale, out, err)
+        return output
 
     def _step_state(self, md, device):
         """Persistent buffers of the one-stage step-kernel program (fixed pointers, so a

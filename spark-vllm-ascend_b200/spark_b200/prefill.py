@@ -19,6 +19,13 @@ SiLU / GELU-table arithmetic).  Results agree with token-by-token decode within 
 rounding, not bit for bit (the GEMM summation order is the tensor cores').  After
 ``prefill`` the engine holds the prompt's K / V, ``pos`` = prompt length and ``token`` =
 the first generated token.
+
+``prefill_packed`` takes prompts of any lengths together: their tokens are packed into one
+batch of rows (each weight is then read once for all), positions and cache slots come from
+``ops.paged_plan_out``, rotation and the paged store are one kernel
+(``ops.qk_norm_rope_store_rows``) and attention reads the pages in place
+(``ops.attn_prompt_out``): no gathered copy of the context, no mask, no host round trip per
+prompt.  ``prefill(..., attn="paged")`` is the same path for one prompt.
 """
 from __future__ import annotations
 
@@ -82,6 +89,34 @@ class _Q4Linear:
             raise RuntimeError(f"spark_q4_gemm_tc: a wait inside the kernel ran out (status {e})")
 
 
+def _projections(eng, gemm: str):
+    """(status word owner or None, per layer the qkv / o / gate_up / down products)."""
+    w = eng.w
+    if gemm not in ("q4", "bf16"):
+        raise ValueError(f"gemm must be 'q4' or 'bf16', not {gemm!r}")
+    if gemm == "q4":
+        q4 = _Q4Linear(eng.device)
+        return q4, [((lambda x, m=l.qkv: q4(x, m)), (lambda x, m=l.o: q4(x, m)), (lambda x, m=l.gate_up: q4(x, m)),
+                     (lambda x, m=l.down: q4(x, m))) for l in w.layers]
+    return None, [tuple((lambda x, wt=wt: x @ wt.t()) for wt in ws) for ws in _bf16_weights(eng)]
+
+
+def _head_logits(eng, x: torch.Tensor) -> torch.Tensor:
+    """LM-head logits bf16 [n, vocab] of normalised rows x [n, h]."""
+    cfg, w, n = eng.cfg, eng.w, x.shape[0]
+    logits = torch.empty((n, cfg.vocab_size), dtype=BF16, device=x.device)
+    if getattr(w, "head_q6", None) is not None:  # Q6_K head: bf16 row chunks and matmul
+        rows = 16384
+        for r0 in range(0, cfg.vocab_size, rows):
+            r1 = min(cfg.vocab_size, r0 + rows)
+            wt = ops.q6k_dequantize(w.head_q6[r0:r1].contiguous()).view(r1 - r0, cfg.hidden_size).to(BF16)
+            logits[:, r0:r1] = x @ wt.t()
+    else:  # few positions: the decode path's Q4_0 GEMV, not a dequantized copy of the head
+        for r0 in range(0, n, 8):
+            ops.q4_gemv_out(x[r0:r0 + 8], w.head.qs, w.head.d, logits[r0:r0 + 8])
+    return logits
+
+
 def _gather(cache: torch.Tensor, table: torch.Tensor, n: int, bs: int) -> torch.Tensor:
     """Positions [0, n) of one layer's paged cache [blocks, nkv, bs, D] -> [nkv, n, D]."""
     pos = torch.arange(n, device=cache.device)
@@ -89,10 +124,13 @@ def _gather(cache: torch.Tensor, table: torch.Tensor, n: int, bs: int) -> torch.
 
 
 @torch.no_grad()
-def prefill(eng, prompt: torch.Tensor, chunk: int = 2048, gemm: str = "q4") -> torch.Tensor:
+def prefill(eng, prompt: torch.Tensor, chunk: int = 2048, gemm: str = "q4", attn: str = "sdpa") -> torch.Tensor:
     """Fill ``eng``'s KV cache with ``prompt`` (int32 [P]) from position 0 and set the
     first generated token; returns it (int32 [1]).  ``gemm``: "q4" (tensor-core GEMMs
-    over the Q4_0 planes) or "bf16" (cuBLAS over a cached bf16 dequantization)."""
+    over the Q4_0 planes) or "bf16" (cuBLAS over a cached bf16 dequantization).  ``attn``:
+    "sdpa" (torch's attention over gathered keys) or "paged" (``prefill_packed``)."""
+    if attn not in ("sdpa", "paged"):
+        raise ValueError(f"attn must be 'sdpa' or 'paged', not {attn!r}")
     cfg, w = eng.cfg, eng.w
     dev = eng.device
     prompt = torch.as_tensor(prompt, dtype=torch.int64).to(dev)
@@ -103,14 +141,11 @@ def prefill(eng, prompt: torch.Tensor, chunk: int = 2048, gemm: str = "q4") -> t
                             cfg.head_dim, cfg.block_size)
     nh, eps, scale = nq + 2 * nkv, cfg.rms_norm_eps, cfg.attn_scale
     table = eng.block_table
-    if gemm not in ("q4", "bf16"):
-        raise ValueError(f"gemm must be 'q4' or 'bf16', not {gemm!r}")
-    if gemm == "q4":
-        q4 = _Q4Linear(dev)
-        mats = [((lambda x, m=l.qkv: q4(x, m)), (lambda x, m=l.o: q4(x, m)), (lambda x, m=l.gate_up: q4(x, m)),
-                 (lambda x, m=l.down: q4(x, m))) for l in w.layers]
-    else:
-        mats = [tuple((lambda x, wt=wt: x @ wt.t()) for wt in ws) for ws in _bf16_weights(eng)]
+    if attn == "paged":
+        eng.reset(0)
+        logits = prefill_packed(eng, [prompt], table.view(1, -1), chunk, gemm)[0]
+        return _finish(eng, logits, P)
+    q4, mats = _projections(eng, gemm)
     heads = torch.arange(nkv, device=dev)
     eng.reset(0)
     a_last = b_last = None
@@ -160,24 +195,98 @@ def prefill(eng, prompt: torch.Tensor, chunk: int = 2048, gemm: str = "q4") -> t
         a_last, b_last = a[-1:], b[-1:]
     # LM head of the last position, greedy
     _, x = ops.add_rmsnorm_rows(a_last, b_last, w.final_norm, eps)
-    logits = torch.empty(cfg.vocab_size, dtype=BF16, device=dev)
-    if getattr(w, "head_q6", None) is not None:  # Q6_K head: bf16 row chunks and matmul
-        rows = 16384
-        for r0 in range(0, cfg.vocab_size, rows):
-            r1 = min(cfg.vocab_size, r0 + rows)
-            wt = ops.q6k_dequantize(w.head_q6[r0:r1].contiguous()).view(r1 - r0, h).to(BF16)
-            logits[r0:r1] = (x @ wt.t())[0]
-    else:  # one position: the decode path's Q4_0 GEMV, not a dequantized copy of the head
-        ops.q4_gemv_out(x, w.head.qs, w.head.d, logits)
+    logits = _head_logits(eng, x)[0]
+    if q4 is not None:
+        q4.check()
+    return _finish(eng, logits, P)
+
+
+def _finish(eng, logits: torch.Tensor, P: int) -> torch.Tensor:
+    """Engine state behind a prompt of P tokens: logits, first token, position."""
     eng.logits.copy_(logits)
     tok = torch.argmax(logits.float()).to(torch.int32).reshape(1)
-    if gemm == "q4":
-        q4.check()
     eng.token.copy_(tok)
     eng.pos.fill_(P)
     eng.step_idx.zero_()
     eng.key.zero_()
     return tok.clone()
+
+
+def _next_rows(left: list[int], chunk: int) -> list[int]:
+    """Tokens each prompt gives to the next batch of at most ``chunk`` rows, in order."""
+    take = []
+    for n in left:
+        take.append(min(n, chunk))
+        chunk -= take[-1]
+    return take
+
+
+@torch.no_grad()
+def prefill_packed(eng, prompts, block_tables: torch.Tensor, chunk: int = 8192, gemm: str = "q4") -> torch.Tensor:
+    """Prefill ``prompts`` (sequences of token ids, any lengths from 1) from position 0 into
+    the pages of ``block_tables`` (int32 [R, pages], complete) of ``eng``'s caches, ``chunk``
+    rows at a time; returns the last positions' logits, bf16 [R, vocab].  Sets no engine
+    state: ``DecodeEngine.prefill_batched(attn="paged")`` and
+    ``BatchDecodeEngine.prefill(packed=True)`` do."""
+    cfg, w, dev = eng.cfg, eng.w, eng.device
+    h, nq, nkv, D, bs = cfg.hidden_size, cfg.num_q_heads, cfg.num_kv_heads, cfg.head_dim, cfg.block_size
+    nh, eps = nq + 2 * nkv, cfg.rms_norm_eps
+    prompts = [torch.as_tensor(p, dtype=torch.int64).reshape(-1).cpu() for p in prompts]
+    R, lens = len(prompts), [p.numel() for p in prompts]
+    if R == 0 or min(lens) == 0 or max(lens) > eng.max_seq_len:
+        raise ValueError(f"prompts of {lens} tokens (1 to max_seq_len {eng.max_seq_len} each)")
+    if chunk < 1 or block_tables.shape[0] != R:
+        raise ValueError("chunk must be positive and block_tables hold a row per prompt")
+    q4, mats = _projections(eng, gemm)
+    i32 = {"dtype": torch.int32, "device": dev}
+    rows_max = min(chunk, sum(lens))
+    err, counter = torch.zeros(1, **i32), torch.zeros(1, **i32)
+    start, seq = torch.empty(R + 1, **i32), torch.empty(R, **i32)
+    pos = torch.empty(rows_max, dtype=torch.int64, device=dev)
+    slots, x_last = torch.empty_like(pos), torch.empty((R, h), dtype=BF16, device=dev)
+    plans = {win: ops.AttnPlan(rows_max, R, nq, nkv, D, dev, win)
+             for win in {cfg.layer_window(li) for li in range(cfg.num_layers)}}
+    done = [0] * R
+    while done != lens:
+        new = _next_rows([n - d for n, d in zip(lens, done)], chunk)
+        T = sum(new)
+        ids = torch.cat([p[d:d + n] for p, d, n in zip(prompts, done, new)]).to(dev)
+        ops.paged_plan_out(torch.tensor(done, **i32), torch.tensor(new, **i32), block_tables, bs, start, seq, pos[:T],
+                           slots[:T], counter, err)
+        for plan in plans.values():
+            plan.update(start, seq)
+        a, b = w.embed[ids], None  # bf16 [T, h]
+        q, o = torch.empty((T, nq, D), dtype=BF16, device=dev), torch.empty((T, nq, D), dtype=BF16, device=dev)
+        for li, (lw, (w_qkv, w_o, w_gu, w_down)) in enumerate(zip(w.layers, mats)):
+            res, x = ops.add_rmsnorm_rows(a, b, lw.in_norm, eps)
+            y = w_qkv(x)
+            cs = w.layer_cos_sin(li) if hasattr(w, "layer_cos_sin") else w.cos_sin
+            ops.qk_norm_rope_store_rows(y, nq, nkv, D, None, None, eps, cs, pos[:T], slots[:T], eng.k_cache[li],
+                                        eng.v_cache[li], q, err)
+            ops.attn_prompt_out(q, eng.k_cache[li], eng.v_cache[li], block_tables, plans[cfg.layer_window(li)],
+                                cfg.attn_scale, o, err)
+            att = o
+            if cfg.attn_gate:
+                gate = torch.sigmoid(y[:, nh * D:nh * D + nq].float()).to(BF16)
+                att = (o.float() * gate.float()[:, :, None]).to(BF16)
+            resmid, x2 = ops.add_rmsnorm_rows(w_o(att.reshape(T, nq * D)), res, lw.post_norm, eps)
+            mid = ops.act_mul_rows(w_gu(x2), getattr(eng, "gelu", None) if cfg.hidden_act == "gelu" else None)
+            a, b = w_down(mid), resmid
+        end = 0
+        for r, n in enumerate(new):  # the last position of each prompt that ends in this batch
+            end += n
+            done[r] += n
+            if n and done[r] == lens[r]:
+                x_last[r:r + 1] = ops.add_rmsnorm_rows(a[end - 1:end], b[end - 1:end], w.final_norm, eps)[1]
+    logits = _head_logits(eng, x_last)
+    for plan in plans.values():
+        err.bitwise_or_(plan.error)
+    status = int(err.item())
+    if status:
+        raise RuntimeError(f"packed prefill: the paged operators report status {status}")
+    if q4 is not None:
+        q4.check()
+    return logits
 
 
 def main(argv=None):
@@ -193,28 +302,29 @@ def main(argv=None):
     ap.add_argument("--tokens", type=int, default=2048)
     ap.add_argument("--profile", action="store_true")
     ap.add_argument("--gemm", choices=["q4", "bf16"], default="q4")
+    ap.add_argument("--attn", choices=["sdpa", "paged"], default="sdpa")
     args = ap.parse_args(argv)
     cfg = spark_x26_config() if args.model == "spark-x26" else SparkConfig()
     w = SyntheticWeights(cfg, device="cuda", seed=0)
     eng = DecodeEngine(w, max_seq_len=args.tokens + 64, num_blocks=(args.tokens + 64) // 128 + 8, use_graph=False)
     prompt = torch.randint(0, cfg.vocab_size, (args.tokens,), generator=torch.Generator().manual_seed(0),
                            dtype=torch.int32)
-    eng.prefill_batched(prompt, gemm=args.gemm)
+    eng.prefill_batched(prompt, gemm=args.gemm, attn=args.attn)
     torch.cuda.synchronize()
     best = None
     for _ in range(3):
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record()
-        eng.prefill_batched(prompt, gemm=args.gemm)
+        eng.prefill_batched(prompt, gemm=args.gemm, attn=args.attn)
         e1.record()
         torch.cuda.synchronize()
         ms = e0.elapsed_time(e1)
         best = ms if best is None else min(best, ms)
-    print(json.dumps({"model": cfg.name, "tokens": args.tokens, "gemm": args.gemm, "ttft_ms": round(best, 3)}))
+    print(json.dumps({"model": cfg.name, "tokens": args.tokens, "gemm": args.gemm, "attn": args.attn, "ttft_ms": round(best, 3)}))
     if args.profile:
         from torch.profiler import ProfilerActivity, profile
         with profile(activities=[ProfilerActivity.CUDA]) as prof:
-            eng.prefill_batched(prompt, gemm=args.gemm)
+            eng.prefill_batched(prompt, gemm=args.gemm, attn=args.attn)
             torch.cuda.synchronize()
         print(prof.key_averages().table(sort_by="cuda_time_total", row_limit=12, max_name_column_width=70))
 

@@ -134,3 +134,25 @@ def test_paged_custom_ops_trace_on_meta_tensors():
     y = torch.ops.spark_b200.qk_norm_rope_store_rows(torch.empty((5, 1536), **bf), 8, 2, 128, None, None, 1e-6,
                                                      torch.empty((9, 128), **bf), p, p, c, c.clone(), e)
     assert y.shape == (5, 8, 128)
+
+
+def test_rows_of_a_packed_prefill_are_dealt_in_order():
+    from spark_b200.prefill import _next_rows
+    assert _next_rows([130, 1, 77], 40) == [40, 0, 0]
+    assert _next_rows([10, 1, 77], 40) == [10, 1, 29]
+    assert _next_rows([0, 0, 5], 40) == [0, 0, 5]
+
+
+def test_cascade_is_asked_for_only_where_it_serves(monkeypatch):
+    pytest.importorskip("vllm")
+    from spark_b200.plugin.attention import PAGED_ENV, SparkAttentionMetadataBuilder as B
+    b = B.__new__(B)
+    ask = lambda prefix=512, q=(1, 1, 1), **k: b.use_cascade_attention(  # noqa: E731
+        prefix, list(q), 32, 8, k.get("alibi", False), k.get("sliding", False), k.get("local", False), 148,
+        k.get("dcp", 1))
+    monkeypatch.delenv(PAGED_ENV, raising=False)
+    assert not ask()  # off unless switched on
+    monkeypatch.setenv(PAGED_ENV, "1")
+    assert ask()
+    assert not ask(prefix=127) and not ask(q=(1,)) and not ask(q=(1, 2)) and not ask(alibi=True)
+    assert not ask(sliding=True) and not ask(local=True) and not ask(dcp=2)
