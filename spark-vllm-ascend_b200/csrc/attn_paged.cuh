@@ -273,12 +273,13 @@ __device__ __forceinline__ float ex2(float x) {
 // 2^x of a pair by arithmetic alone, for the special-function unit's relief: x = n + f with
 // n the nearest integer (adding 1.5 2^23 leaves n in the low bits), 2^f a cubic on
 // [-1/2, 1/2] fitted here to the least maximal relative error (7.5e-5, against the 2^-8 of
-// the bf16 rounding that follows), n added to the exponent.  x <= 127; below -127 the
-// result is a denormal of no weight, not zero: tiles with masked keys do not come here.
+// the bf16 rounding that follows), n added to the exponent, which has to stay a normal
+// one: x <= 127, and what is below -125 (the cubic may be just under 1) becomes 2^-125, of
+// no weight but not zero: tiles with masked keys do not come here.
 __device__ __forceinline__ u64 ex2_poly(u64 x2) {
   float x, y;
   unpack2(x2, x, y);
-  x2 = pack2(fmaxf(x, -127.0f), fmaxf(y, -127.0f));
+  x2 = pack2(fmaxf(x, -125.0f), fmaxf(y, -125.0f));
   const u64 magic = pack2(12582912.0f, 12582912.0f), unmagic = pack2(-12582912.0f, -12582912.0f);
   const u64 t = add2(x2, magic);
   const u64 f = fma2(add2(t, unmagic), pack2(-1.0f, -1.0f), x2);
@@ -747,10 +748,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto wait = [&](int i, uint32_t parity) {
       return __all_sync(0xffffffffu, bar_wait(bar(i), parity, limit_ns, abort_flag));
     };
-    // Warpgroup j's value of this row is at xs + 512 j.  The next values overwrite these: within an
-    // item they follow the scores of the next tile, which every partner's probabilities
-    // precede; behind the item's last exchange each warp reports that it has read them
-    // (unread: that report is still to be awaited).
+    // Warpgroup j's value of this row is at xs + 512 j.  The next values may be written over
+    // these once all have read them.  head_dim 128, maxima: they follow the next scores of the
+    // same buffer, which every partner's probabilities precede.  head_dim 256, whose next
+    // scores are in the other buffer and may be there already, and an item's last exchange:
+    // each warp reports that it has read (unread: that report is still to be awaited).
     auto exchange = [&](float v) -> bool {
       if (unread) {
         if (!wait(xbar, nx++ & 1)) return false;
@@ -854,6 +856,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = exchange(mn))) break;
 #pragma unroll
           for (int j = 0; j < SP; j++) mn = fmaxf(mn, ldsf(xs + 512 * j));
+          if (D == 256) {
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar(xbar));
+            unread = true;
+          }
           mn = fmaxf(m, mn);
           if (first) {
             m = mn;
@@ -912,6 +919,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       // -------------------------------------------------------------- epilogue
       const int mine = few ? (n + 1 - t0) / 2 : n;  // this half's tiles
       if (mine > 0) {
+        if (!(ok = wait(kBarO + h, no++ & 1))) break;
+        fence_after();
+        // (only now: the products took every partner's last probabilities, so the maxima have
+        // been read)
         if (any_valid) {  // the row's sum over all columns, added in warpgroup order
           if (!(ok = exchange(l))) break;
           l = 0.0f;
@@ -921,8 +932,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) bar_arrive(bar(xbar));
           unread = true;
         }
-        if (!(ok = wait(kBarO + h, no++ & 1))) break;
-        fence_after();
       }
       if (any_valid) {
         const int head_row = r % g, tok = it.tok0 + local, head = kvh * g + head_row;

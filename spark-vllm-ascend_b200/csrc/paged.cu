@@ -111,8 +111,10 @@ static int check_attn_shape(int max_tokens, int max_reqs, int nq, int nkv, int h
       (head_dim != 128 && head_dim != 256))
     return SPARK_ERR_UNSUPPORTED_SHAPE;
   // tile, item and partial-row counts are 32-bit
-  if (max_tokens > (1 << 22) || max_reqs > (1 << 16) || nkv > 4096 ||
-      (int64_t)paged::layout_of(max_tokens, max_reqs, nq, nkv, head_dim).max_items * nkv > (1 << 30))
+  if (max_tokens > (1 << 22) || max_reqs > (1 << 16) || nkv > 4096) return SPARK_ERR_TOO_LARGE;
+  const paged::Layout l = paged::layout_of(max_tokens, max_reqs, nq, nkv, head_dim);
+  if ((int64_t)l.max_items * nkv > (1 << 30) ||
+      (int64_t)l.max_entries * nkv * l.tile_tok * (nq / nkv) > 0xffffffffLL)
     return SPARK_ERR_TOO_LARGE;
   return SPARK_OK;
 }

@@ -774,7 +774,7 @@ __device__ __forceinline__ int2 row_keys(const Item& it, const int* lens, int wi
 // the parts in list order whatever order they were computed in.  A row without any key is
 // zero.  One warp per row: lanes hold 32 parts' (m, l) at a time, then the warp adds the
 // parts' sums, four in flight.
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinFlight = 4;
 
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) combine_kernel(AttnArgs p) {
@@ -784,12 +784,12 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(AttnArgs p) {
   const Entry* entries = reinterpret_cast<const Entry*>(p.plan + p.lay.entries);
   const int g = p.nq / p.nkv, lane = threadIdx.x & 31;
   const int n = hdr->entries, jr = hdr->join_rows;
-  const int64_t total = (int64_t)n * p.nkv * jr, step = (int64_t)gridDim.x * (kJoinThreads / 32);
-  for (int64_t w = (int64_t)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5); w < total; w += step) {
-    const int row = (int)(w % jr);
-    const int64_t x = w / jr;
-    const int kvh = (int)(x % p.nkv);
-    const Entry en = entries[x / p.nkv];
+  // (entries x kv heads x rows: below 2^31, since part rows x kv heads are)
+  const uint32_t total = (uint32_t)n * p.nkv * jr, step = gridDim.x * (kJoinThreads / 32);
+  for (uint32_t w = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5); w < total; w += step) {
+    const uint32_t x = w / (uint32_t)jr, e = x / (uint32_t)p.nkv;
+    const int row = (int)(w - x * jr), kvh = (int)(x - e * p.nkv);
+    const Entry en = entries[e];
     const int tok = en.tok0 + row / g, head = kvh * g + row % g;
     if (row >= en.ntok * g || tok >= p.tokens) continue;
     const int parts = en.n_a + en.n_b;
@@ -812,10 +812,10 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(AttnArgs p) {
 #pragma unroll
       for (int e = 0; e < E; e++) o[e] *= a;
       const int m = parts - k0 < 32 ? parts - k0 : 32;
-      for (int k = 0; k < m; k += 4) {
-        float v[4][E], f[4];
+      for (int k = 0; k < m; k += kJoinFlight) {
+        float v[kJoinFlight][E], f[kJoinFlight];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < kJoinFlight; j++) {
           f[j] = __shfl_sync(0xffffffffu, wt, (k + j) & 31);
           const bool use = k + j < m && f[j] != 0.0f;
           const float4* src = reinterpret_cast<const float4*>(p.part_o + index(k0 + k + j) * D + lane * E);
@@ -827,7 +827,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(AttnArgs p) {
           if (!use) f[j] = 0.0f;
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+        for (int j = 0; j < kJoinFlight; j++)
 #pragma unroll
           for (int e = 0; e < E; e++) o[e] = __fmaf_rn(v[j][e], f[j], o[e]);
       }

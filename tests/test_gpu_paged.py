@@ -597,3 +597,148 @@ def test_paged_refusals(cuda):
         plan.update(torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"))
     with pytest.raises(ValueError):
         ops.AttnPlan(20, 1, nq, nkv, D, window=5).update_prefix(b["lens"], b["lens"])
+
+
+@pytest.mark.parametrize("D,nq,nkv", [(128, 8, 2), (256, 8, 2)])
+@pytest.mark.parametrize("ctx,new", [([0], [700]), ([2000, 900], [1, 3])])
+def test_attn_prompt_large_and_climbing_scores(cuda, D, nq, nkv, ctx, new):
+    """Scores up to 10^4 that climb along the keys, so that the softmax's reference moves at
+    every tile and by more than any single exponential could take.  q and k are small
+    integers: every score is exact in fp32 and the tolerance stays the rounding of p."""
+    import torch
+    from spark_b200 import ops
+    b = _batch(ctx, new, nq, nkv, D, 16, seed=31)
+    g = torch.Generator(device="cuda").manual_seed(32)
+    b["q"].copy_(torch.randint(0, 2, b["q"].shape, generator=g, device="cuda") * 512)
+    for r, m in enumerate(b["len"]):
+        at = torch.arange(m, device="cuda")
+        blk, off = b["table"][r, at // 16].long(), at % 16
+        k = torch.randint(-1, 2, (m, nkv, D), generator=g, device="cuda").float()
+        k[:, :, 0] = (at.float() / m * 200).round()[:, None]  # the climb
+        b["kc"][blk, :, off] = k.to(torch.bfloat16)
+    b["q"][:, :, 0] = 512
+    plan = ops.AttnPlan(b["q"].shape[0], len(ctx), nq, nkv, D).update(b["start"], b["lens"])
+    out = torch.full_like(b["q"], float("nan"))
+    ops.attn_prompt_out(b["q"], b["kc"], b["vc"], b["table"], plan, D ** -0.5, out, b["err"])
+    torch.cuda.synchronize()
+    assert int(b["err"]) == 0
+    ref, mag = _attn_ref(b, nq, nkv, D, D ** -0.5)
+    _close(out, ref, mag)
+
+
+def test_attn_prompt_pages_past_32_bit_offsets(cuda):
+    """Caches of more than 2^31 elements, the requests' pages at their far end."""
+    import torch
+    from spark_b200 import ops
+    nq, nkv, D, bs, n = 32, 8, 128, 128, 300
+    blocks = 17000  # x 2^17 elements a page
+    kc = torch.empty((blocks, nkv, bs, D), dtype=torch.bfloat16, device="cuda")
+    vc = torch.empty_like(kc)
+    assert kc.numel() > 1 << 31
+    g = torch.Generator(device="cuda").manual_seed(33)
+    ids = [blocks - 1, blocks - 5, blocks - 3, 2, blocks - 2, blocks - 4]
+    kc[ids], vc[ids] = (torch.randn((6, nkv, bs, D), generator=g, device="cuda").to(torch.bfloat16) for _ in "kv")
+    table = torch.tensor([ids[:3], ids[3:]], dtype=torch.int32, device="cuda")
+    i32 = {"dtype": torch.int32, "device": "cuda"}
+    start, lens = torch.tensor([0, n, n + 1], **i32), torch.tensor([n, 290], **i32)
+    qkv = torch.randn((n + 1, (nq + 2 * nkv) * D), generator=g, device="cuda").to(torch.bfloat16)
+    pos = torch.cat([torch.arange(n, device="cuda"), torch.tensor([289], device="cuda")])
+    slots = torch.cat([table[0].long()[pos[:n] // bs] * bs + pos[:n] % bs, table[1].long()[2:3] * bs + 289 - 2 * bs])
+    cs = torch.cat([torch.ones((400, 64)), torch.zeros((400, 64))], 1).to(torch.bfloat16).cuda()
+    q, err = torch.empty((n + 1, nq, D), dtype=torch.bfloat16, device="cuda"), torch.zeros(1, **i32)
+    ops.qk_norm_rope_store_rows(qkv, nq, nkv, D, None, None, 0.0, cs, pos, slots, kc, vc, q, err)
+    out = torch.zeros_like(q)
+    plan = ops.AttnPlan(n + 1, 2, nq, nkv, D).update(start, lens)
+    ops.attn_prompt_out(q, kc, vc, table, plan, D ** -0.5, out, err)
+    torch.cuda.synchronize()
+    assert int(err) == 0
+    b = {"q": q, "kc": kc, "vc": vc, "table": table, "new": [n, 1], "len": [n, 290], "bs": bs}
+    assert torch.equal(kc[ids[0], :, 5], qkv[5].view(-1, D)[nq:nq + nkv])
+    ref, mag = _attn_ref(b, nq, nkv, D, D ** -0.5)
+    _close(out, ref, mag)
+
+
+def test_attn_two_calls_at_once_with_a_plan_each(cuda):
+    """Two streams, two captured graphs, replayed together: equal to one after the other."""
+    import torch
+    from spark_b200 import ops
+    nq, nkv, D, bs = 32, 8, 128, 16
+    jobs = []
+    for seed, (ctx, new) in enumerate([([4000, 100], [1, 1]), ([0, 64], [300, 70])]):
+        b = _batch(ctx, new, nq, nkv, D, bs, seed=40 + seed)
+        plan = ops.AttnPlan(b["q"].shape[0], 2, nq, nkv, D)
+        out = torch.zeros_like(b["q"])
+
+        def step(b=b, plan=plan, out=out):
+            plan.update(b["start"], b["lens"])
+            ops.attn_prompt_out(b["q"], b["kc"], b["vc"], b["table"], plan, D ** -0.5, out, b["err"])
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        jobs.append((b, out, out.clone(), graph, torch.cuda.Stream()))
+    for _ in range(20):
+        for b, out, want, graph, stream in jobs:
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                out.zero_()
+                for _ in range(3):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for b, out, want, graph, stream in jobs:
+            assert torch.equal(out.view(torch.int16), want.view(torch.int16)) and int(b["err"]) == 0
+
+
+@pytest.mark.parametrize("D,nq,nkv", [(128, 32, 8), (256, 16, 4)])
+def test_attn_wait_that_runs_out_reports_and_recovers(cuda, D, nq, nkv):
+    """A wait limit of 0 makes the first unfinished wait give up: the kernel returns, the
+    caller's word says so (not 2: copies and products drained, tensor memory was freed), and
+    the next call is right."""
+    import torch
+    from spark_b200 import ops
+    b = _batch([3000, 0], [200, 600], nq, nkv, D, 128, seed=50)
+    plan = ops.AttnPlan(800, 2, nq, nkv, D).update(b["start"], b["lens"])
+    out = torch.zeros_like(b["q"])
+    ops.attn_prompt_out(b["q"], b["kc"], b["vc"], b["table"], plan, D ** -0.5, out, b["err"], wait_ns=0)
+    torch.cuda.synchronize()
+    assert int(b["err"]) == ops.ERR_WAIT
+    b["err"].zero_()
+    ops.attn_prompt_out(b["q"], b["kc"], b["vc"], b["table"], plan, D ** -0.5, out, b["err"])
+    torch.cuda.synchronize()
+    assert int(b["err"]) == 0
+    ref, mag = _attn_ref(b, nq, nkv, D, D ** -0.5)
+    _close(out, ref, mag)
+
+
+def test_paged_plan_in_a_graph_takes_pages_each_replay(cuda):
+    """free_head advanced in place, replay by replay."""
+    import torch
+    from spark_b200 import ops
+    i32 = {"dtype": torch.int32, "device": "cuda"}
+    R, bs = 3, 16
+    ctx, new = torch.zeros(R, **i32), torch.tensor([16, 5, 0], **i32)
+    table, free = torch.full((R, 4), -1, **i32), torch.arange(100, 140, **i32)
+    head, counter, err = torch.zeros(1, **i32), torch.zeros(1, **i32), torch.zeros(1, **i32)
+    start, lens = torch.zeros(R + 1, **i32), torch.zeros(R, **i32)
+    pos, slots = torch.zeros(21, dtype=torch.int64, device="cuda"), torch.zeros(21, dtype=torch.int64, device="cuda")
+
+    def step():
+        ops.paged_plan_out(ctx, new, table, bs, start, lens, pos, slots, counter, err, free_blocks=free,
+                           free_head=head)
+        ctx.copy_(lens)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    # 16 + 5 tokens, four times: 4 pages, and pages at 0, (5 10 15) none, 16 .. 20
+    assert int(err) == 0 and ctx.tolist() == [64, 20, 0] and int(head) == 6 and int(counter) == 0
+    assert table.tolist() == [[100, 102, 103, 104], [101, 105, -1, -1], [-1] * 4]
+    assert pos[16:].tolist() == [15, 16, 17, 18, 19] and slots[16:].tolist() == [101 * 16 + 15] + [
+        105 * 16 + i for i in range(4)]
