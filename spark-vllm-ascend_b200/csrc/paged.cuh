@@ -436,6 +436,7 @@ struct AttnPlanArgs {
 
 constexpr int kAttnPlanThreads = 1024;
 constexpr int kBins = 1024;
+constexpr int kPlanStarts = 1024, kPlanTiles = 1024;
 
 // Tile i of the batch: everything but how it is cut.
 struct Tile {
@@ -488,7 +489,7 @@ __device__ __forceinline__ Tile prefix_tile(const AttnPlanArgs& p, const int* le
 __host__ __device__ inline int part_cost(int flags, int parts, int tiles, int rows) {
   return tiles * ((flags & kFlagFew) ? 2 : 4) + 8 + (parts > 1 ? rows / 32 : 0);
 }
-constexpr int kPriceBins = 256;
+constexpr int kPriceBins = 128;
 __device__ __forceinline__ int price_bin(int cost, int top) {
   return min((int)((long long)cost * kPriceBins / (top + 1)), kPriceBins - 1);
 }
@@ -500,12 +501,15 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
   __shared__ int ws[kAttnPlanThreads / 32];
   __shared__ int hist[kBins];
   __shared__ int price[32 * (kPriceBins + 1)];
+  // of small batches: first tile per request, and (key tiles, flags | rows << 8) per tile
+  __shared__ int starts_s[kPlanStarts + 1];
+  __shared__ int2 brief_s[kPlanTiles];
   __shared__ int entries_s, rows_s, bad_s, join_s;
   const int tid = threadIdx.x, R = p.reqs;
   Header* hdr = reinterpret_cast<Header*>(p.plan);
   Item* items = reinterpret_cast<Item*>(p.plan + p.lay.items);
   Entry* entries = reinterpret_cast<Entry*>(p.plan + p.lay.entries);
-  int* starts = reinterpret_cast<int*>(p.plan + p.lay.starts);  // first tile of request r
+  int* starts = R <= kPlanStarts ? starts_s : reinterpret_cast<int*>(p.plan + p.lay.starts);  // first tile of request r
   int2* tiles = reinterpret_cast<int2*>(p.plan + p.lay.tiles);  // (request, tile of the request)
   int2* bases = reinterpret_cast<int2*>(p.plan + p.lay.bases);  // (first partial row, parts)
   int* lens = reinterpret_cast<int*>(p.plan + p.lay.lens);
@@ -573,6 +577,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
       tiles[i] = make_int2(r, i - starts[r]);
     }
     const Tile t = tile_at(i);
+    if (i < kPlanTiles) brief_s[i] = make_int2(t.nkt, t.flags | t.ntok * g << 8);
     longest = t.nkt > longest ? t.nkt : longest;
     if (t.flags & kFlagFew) few_rows += 2 * t.ntok * g;
   }
@@ -602,15 +607,22 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
     __syncwarp();
     int extra = 0, rows = 0;
     for (int i = lane; i < nt; i += 32) {
-      const Tile t = tile_at(i);
-      const int np = (t.nkt + c - 1) / c;
+      int nkt, flags, trows;
+      if (i < kPlanTiles) {
+        const int2 t = brief_s[i];
+        nkt = t.x, flags = allow_few ? t.y & 255 : t.y & 255 & ~kFlagFew, trows = t.y >> 8;
+      } else {
+        const Tile t = tile_at(i);
+        nkt = t.nkt, flags = t.flags, trows = t.ntok * g;
+      }
+      const int np = (nkt + c - 1) / c;
       if (np == 0) continue;
       extra += np - 1;
-      const int each = (t.flags & kFlagFew) ? 2 : 1;
-      if (np > 1 || prefix_kind || each == 2) rows += each * np * t.ntok * g;
-      const int lo = t.nkt / np, more = t.nkt - lo * np;  // `more` parts have one tile more
+      const int each = (flags & kFlagFew) ? 2 : 1;
+      if (np > 1 || prefix_kind || each == 2) rows += each * np * trows;
+      const int lo = nkt / np, more = nkt - lo * np;  // `more` parts have one tile more
       const int joined = prefix_kind ? 2 : np;
-      const int c0 = part_cost(t.flags, joined, lo, t.ntok * g), c1 = part_cost(t.flags, joined, lo + 1, t.ntok * g);
+      const int c0 = part_cost(flags, joined, lo, trows), c1 = part_cost(flags, joined, lo + 1, trows);
       if (np > more) atomicAdd(&h[price_bin(c0, top)], (np - more) * p.nkv);
       if (more) atomicAdd(&h[price_bin(c1, top)], more * p.nkv);
     }
@@ -632,25 +644,24 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
     for (int j = 0; j < kPriceBins / 32; j++) h[lane * (kPriceBins / 32) + j] = mine[j] + above;
     __syncwarp();
     const int parts = h[0];
-    // the load of some of the CTAs: lane = round, in the kernel's back-and-forth order
+    // the load of eight of the CTAs, four lanes each that take every fourth round, in the
+    // kernel's back-and-forth order
+    const int cta = (lane >> 2) * (kNumSMs - 1) / 7;
     int worst = 0;
-    for (int s = 0; s < 8; s++) {
-      const int cta = s * (kNumSMs - 1) / 7;
-      int load = 0;
-      for (int round = lane; (int64_t)round * kNumSMs < parts; round += 32) {
-        const int at = round * kNumSMs + ((round & 1) ? kNumSMs - 1 - cta : cta);
-        if (at >= parts) continue;
-        int lo = 0, hi = kPriceBins - 1;  // largest bin with more than `at` parts in and above it
-        while (lo < hi) {
-          const int m = (lo + hi + 1) >> 1;
-          if (h[m] > at) lo = m;
-          else hi = m - 1;
-        }
-        load += lo + 1;
+    for (int round = lane & 3; (int64_t)round * kNumSMs < parts; round += 4) {
+      const int at = round * kNumSMs + ((round & 1) ? kNumSMs - 1 - cta : cta);
+      if (at >= parts) continue;
+      int lo = 0, hi = kPriceBins - 1;  // largest bin with more than `at` parts in and above it
+      while (lo < hi) {
+        const int m = (lo + hi + 1) >> 1;
+        if (h[m] > at) lo = m;
+        else hi = m - 1;
       }
-      for (int o = 16; o >= 1; o >>= 1) load += __shfl_xor_sync(0xffffffffu, load, o);
-      worst = max(worst, load);
+      worst += lo + 1;
     }
+    worst += __shfl_xor_sync(0xffffffffu, worst, 1);
+    worst += __shfl_xor_sync(0xffffffffu, worst, 2);
+    worst = __reduce_max_sync(0xffffffffu, worst);
     // bins back to cost (rounded up); what does not fit the buffers is out
     const bool fits = extra <= p.lay.budget && rows <= p.lay.part_rows;
     const long long cost = fits ? (long long)worst * top : (1LL << 60);
@@ -676,24 +687,33 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
   auto bin_of = [&](const Tile& t, int joined, int keys) {
     return kBins - 1 - (int)((long long)min(part_cost(t.flags, joined, keys, t.ntok * g), top) * (kBins - 1) / top);
   };
+  // a group of 32, 4 or 1 lanes per tile, which share its parts
+  const int group = nt <= 32 ? 32 : nt <= 256 ? 4 : 1, sub = tid & (group - 1);
+  const int per = kAttnPlanThreads / group, turns = (nt + per - 1) / per;
   for (int pass = 0; pass < 2; pass++) {
-    for (int i = tid; i < nt; i += kAttnPlanThreads) {
-      const Tile t = tile_at(i);
-      int np = (t.nkt + cut - 1) / cut;
-      if (np == 0 && !prefix_kind) np = 1;  // rows without keys are written as zeros
-      const int each = (t.flags & kFlagFew) ? 2 : 1;
-      const bool parts = np > 1 || prefix_kind || each == 2;
-      int base = -1;
-      if (pass == 1) {
-        if (parts) base = atomicAdd(&rows_s, each * np * t.ntok * g);
-        bases[i] = make_int2(base, each * np);
-        if (parts && !prefix_kind) {
-          const int e = atomicAdd(&entries_s, 1);
-          entries[e] = {t.tok0, t.ntok, base, each * np, t.ntok * g, 0, 0, 0};
-          atomicMax(&join_s, t.ntok * g);
+    for (int turn = 0; turn < turns; turn++) {  // (uniform: the shuffle is the whole warp's)
+      const int i = turn * per + tid / group;
+      Tile t;
+      int np = 0, each = 1, base = -1;
+      bool parts = false;
+      if (i < nt) {
+        t = tile_at(i);
+        np = (t.nkt + cut - 1) / cut;
+        if (np == 0 && !prefix_kind) np = 1;  // rows without keys are written as zeros
+        each = (t.flags & kFlagFew) ? 2 : 1;
+        parts = np > 1 || prefix_kind || each == 2;
+        if (pass == 1 && sub == 0) {
+          if (parts) base = atomicAdd(&rows_s, each * np * t.ntok * g);
+          bases[i] = make_int2(base, each * np);
+          if (parts && !prefix_kind) {
+            const int e = atomicAdd(&entries_s, 1);
+            entries[e] = {t.tok0, t.ntok, base, each * np, t.ntok * g, 0, 0, 0};
+            atomicMax(&join_s, t.ntok * g);
+          }
         }
       }
-      for (int k = 0; k < np; k++) {
+      base = __shfl_sync(0xffffffffu, base, (tid & 31) & ~(group - 1));
+      for (int k = sub; k < np; k += group) {
         const int a = (int)((long long)k * t.nkt / np), b = (int)((long long)(k + 1) * t.nkt / np);
         const int slot = atomicAdd(&hist[bin_of(t, parts ? 2 : 1, b - a)], 1);
         if (pass == 1) {

@@ -437,8 +437,9 @@ class AttnPlan:
     ``update`` (packed prompts, chunks, single tokens) or ``update_prefix`` (one token per
     request behind a common prefix) makes the list from device tensors, without a host
     copy, once per step; every layer of that layout then uses it.  Both can be captured
-    into a CUDA graph.  Calls that may overlap on the device need a plan each: the plan and
-    the partial results are overwritten by the next one.  ``error`` int32 [1] collects what
+    into a CUDA graph, which holds the plan's addresses: the plan has to live as long as the
+    graph.  Calls that may overlap on the device need a plan each: the plan and the partial
+    results are overwritten by the next one.  ``error`` int32 [1] collects what
     ``update`` found (ERR_* bits)."""
 
     def __init__(self, max_tokens: int, max_reqs: int, nq: int, nkv: int, head_dim: int, device="cuda",

@@ -677,16 +677,17 @@ def test_attn_two_calls_at_once_with_a_plan_each(cuda):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             step()
-        jobs.append((b, out, out.clone(), graph, torch.cuda.Stream()))
+        # the graph holds the plan's addresses, not the plan: it is kept as long as the graph
+        jobs.append((b, out, out.clone(), graph, torch.cuda.Stream(), plan))
     for _ in range(20):
-        for b, out, want, graph, stream in jobs:
+        for b, out, want, graph, stream, _plan in jobs:
             stream.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(stream):
                 out.zero_()
                 for _ in range(3):
                     graph.replay()
         torch.cuda.synchronize()
-        for b, out, want, graph, stream in jobs:
+        for b, out, want, graph, stream, _plan in jobs:
             assert torch.equal(out.view(torch.int16), want.view(torch.int16)) and int(b["err"]) == 0
 
 
