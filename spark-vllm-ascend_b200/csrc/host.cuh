@@ -39,8 +39,11 @@ inline int set_smem(const void* kernel, size_t smem) {
   std::lock_guard<std::mutex> lock(g_smem_mu);
   for (int i = 0; i < g_smem_count; i++)
     if (g_smem_done[i].fn == kernel && g_smem_done[i].dev == dev && g_smem_done[i].bytes >= smem) return kOk;
-  // always request the maximum so one call serves every later size
-  const int max_bytes = 227 * 1024;
+  // always request the maximum (what the kernel's static part leaves of it) so one call
+  // serves every later size
+  cudaFuncAttributes fa;
+  if (cudaFuncGetAttributes(&fa, kernel) != cudaSuccess) return kErrLaunch;
+  const int max_bytes = 227 * 1024 - (int)fa.sharedSizeBytes;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, max_bytes) != cudaSuccess)
     return kErrLaunch;
   for (int i = 0; i < g_smem_count; i++)
