@@ -229,7 +229,7 @@ int spark_slot_mapping(int64_t num_tokens, int64_t max_tokens, const int32_t* qu
  *
  * The reference leaves these to vLLM's torch path (integration/model.py:50-62: query
  * length > 1) and maps slots for one request at a time (integration/slot_mapping.py:8-22).
- * `error` (int32 on the device, required) collects bits: 4 a negative length or
+ * `error` (int32 on the device, required) collects bits: 4 a length out of range or
  * descending starts, 8 the free list ran out, 16 a request longer than its block table
  * row, 32 more tokens than output rows, 64 a block table entry outside the cache, 128 a
  * position outside the rotation table, 256 a slot outside the cache; 1 and 2 as in
@@ -248,7 +248,7 @@ int spark_slot_mapping(int64_t num_tokens, int64_t max_tokens, const int32_t* qu
  * already, nothing is taken.  A batch that does not fit (bits 4, 8, 16, 32) comes out
  * empty -- all starts and lengths 0, all slots -1 -- and takes no page.  counter: int32,
  * zero before the first call, left zero; calls that may overlap need one each.
- * reqs <= 8192. */
+ * reqs <= 8192.  query_start and seq_lens must not be the inputs. */
 int spark_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int reqs, const int32_t* free_blocks,
                      int num_free, const int32_t* free_head, int32_t* free_head_out, int32_t* block_table,
                      int64_t table_stride, int table_width, int block_size, int rows, int32_t* query_start,

@@ -40,7 +40,9 @@
 // runs, and the issuing order makes every hazard on S, P and O an in-order one: the product
 // that overwrites S_h is issued after the one that reads P_h, and a commit that announces
 // S_h covers all earlier products, so the softmax may touch O_h as soon as it holds S_h
-// (head_dim 256: after a commit of its own).
+// (head_dim 256: after a commit of its own).  The product that adds to O_h is issued only
+// when every warp of the half has rescaled its columns of it, or read them out for the last
+// item.
 //
 // Stale memory: a K / V row at or past the request's length (or before the window) may hold
 // anything.  Scores are masked by selection, and V rows outside [klo, len) are zeroed in
@@ -240,17 +242,6 @@ __device__ __forceinline__ void tm_load16(uint32_t addr, float* v) {
                :
                : "memory");
 }
-__device__ __forceinline__ void tm_store32(uint32_t addr, const uint32_t* u) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(u[0]),
-      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
-      "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]),
-      "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]),
-      "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(addr)
-      : "memory");
-}
-
 __device__ __forceinline__ void tm_store16(uint32_t addr, const uint32_t* u) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(
@@ -394,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(bar(kBarQFull + h), 1);
       bar_init(bar(kBarQEmpty + h), 1 + kSoftmaxWarps);  // the last score product's commit, the softmax warps
       bar_init(bar(kBarS + h), 1);
-      bar_init(bar(kBarP + h), 8);
+      bar_init(bar(kBarP + h), D == 128 ? 8 : 16);
       bar_init(bar(kBarP2 + h), 8);
       bar_init(bar(kBarO + h), 1);
       bar_init(bar(kBarPV + h), 1);
@@ -791,7 +782,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t b = (par + t) & 1;
         return wait(kBarPV + b, (npv[b] + (uint32_t)(t >> 1)) & 1);
       };
-      float m = -INFINITY, l = 0.0f;
+      // (rows beyond the item's have no say in when the reference moves: with m at infinity
+      // it never does for them, and what lies in them does not show in the others' rounding)
+      float m = valid ? -INFINITY : INFINITY, l = 0.0f;
       const uint32_t ob = lanes + kColO + (D == 128 ? h * 128 : 0) + sp * 64;
       for (int t = t0; t < n; t += few ? 2 : 1) {
         const int b = D == 256 ? (int)((par + t) & 1) : h;  // score buffer
@@ -822,6 +815,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         // this warp's share of the first (k = 0) or last 64 keys' probabilities is written
+        // (head_dim 256: warpgroups 2 and 3 have no share of the first, but that product adds to
+        // all columns of O and reads V rows that they zeroed: they announce k = 0 too, once
+        // they are done with both)
         auto announce = [&](int k) {
           wait_st();
           fence_before();
@@ -881,6 +877,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               tm_store16(ob + 16 * i, reinterpret_cast<const uint32_t*>(o));
             }
           }
+          if (D == 256 && sp >= 2) announce(0);
           const float neg = m == -INFINITY ? 0.0f : -m * c;
           const u64 neg2 = pack2(neg, neg), c2 = pack2(c, c);
           u64 sum[2] = {0, 0};
@@ -901,6 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           unpack2(add2(sum[0], sum[1]), s0, s1);
           l += s0 + s1;
         } else {
+          if (D == 256 && sp >= 2) announce(0);
           uint32_t z[16];
 #pragma unroll
           for (int i = 0; i < 16; i++) z[i] = 0;

@@ -57,6 +57,9 @@ int spark_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int reqs,
   if (!ctx_lens || !new_lens || !block_table || !query_start || !seq_lens || !error || !counter)
     return SPARK_ERR_INVALID_ARG;
   if (rows > 0 && (!positions || !slot_mapping)) return SPARK_ERR_INVALID_ARG;
+  // every CTA reads all lengths, while others write already
+  if (seq_lens == ctx_lens || seq_lens == new_lens || query_start == ctx_lens || query_start == new_lens)
+    return SPARK_ERR_INVALID_ARG;
   if (free_blocks ? (!free_head || !free_head_out) : (free_head || free_head_out)) return SPARK_ERR_INVALID_ARG;
   if (reqs <= 0 || rows < 0 || num_free < 0 || block_size <= 0 || table_width <= 0 || table_stride < table_width)
     return SPARK_ERR_UNSUPPORTED_SHAPE;
@@ -114,7 +117,7 @@ static int check_attn_shape(int max_tokens, int max_reqs, int nq, int nkv, int h
   if (max_tokens > (1 << 22) || max_reqs > (1 << 16) || nkv > 4096) return SPARK_ERR_TOO_LARGE;
   const paged::Layout l = paged::layout_of(max_tokens, max_reqs, nq, nkv, head_dim);
   if ((int64_t)l.max_items * nkv > (1 << 30) ||
-      (int64_t)l.max_entries * nkv * l.tile_tok * (nq / nkv) > 0xffffffffLL)
+      (int64_t)l.max_entries * nkv * l.tile_tok * (nq / nkv) > (1LL << 30))
     return SPARK_ERR_TOO_LARGE;
   return SPARK_OK;
 }

@@ -12,7 +12,7 @@ namespace spark {
 namespace paged {
 
 // error word bits (the attention kernel's wait codes 1 and 2 are in attn_paged.cuh)
-constexpr int kBadLength = 4;    // a negative length, or starts that go down
+constexpr int kBadLength = 4;    // a length out of range, or starts that go down
 constexpr int kNoPages = 8;      // the free list is shorter than the pages needed
 constexpr int kTableWidth = 16;  // a request is longer than its block table row
 constexpr int kNoRows = 32;      // more tokens than output rows
@@ -437,6 +437,9 @@ struct AttnPlanArgs {
 constexpr int kAttnPlanThreads = 1024;
 constexpr int kBins = 1024;
 constexpr int kPlanStarts = 1024, kPlanTiles = 1024;
+// longest request: key positions are 32-bit numbers, also those of the tiles and page ids
+// read ahead past its end
+constexpr int kMaxKeys = 0x7fff0000;
 
 // Tile i of the batch: everything but how it is cut.
 struct Tile {
@@ -521,14 +524,15 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
   // tiles per request
   if (prefix_kind) {
     prefix = p.prefix_len[0];
-    if (prefix < 0) {
+    if (prefix < 0 || prefix > kMaxKeys) {
       prefix = 0;
       if (tid == 0) bad_s = kBadLength;
     }
     for (int r = tid; r < R; r += kAttnPlanThreads) {
       const int n = p.seq_lens[r];
-      if (n < 0) atomicOr(&bad_s, kBadLength);
-      lens[r] = n < 0 ? 0 : n;
+      const bool ok = n >= 0 && n <= kMaxKeys;
+      if (!ok) atomicOr(&bad_s, kBadLength);
+      lens[r] = ok ? n : 0;
     }
     npre = (R + p.lay.tile_tok - 1) / p.lay.tile_tok;
     nt = npre + R;
@@ -539,9 +543,9 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
       long long n = 0, dummy = 0, tot[2];
       if (r < R) {
         const int q0 = p.query_start[r], q1 = p.query_start[r + 1], len = p.seq_lens[r];
-        const bool ok = q0 >= 0 && q1 >= q0 && q1 <= p.tokens && len >= 0;
+        const bool ok = q0 >= 0 && q1 >= q0 && q1 <= p.tokens && len >= 0 && len <= kMaxKeys;
         if (!ok) atomicOr(&bad_s, kBadLength);
-        lens[r] = len < 0 ? 0 : len;
+        lens[r] = ok ? len : 0;
         n = ok ? (q1 - q0 + p.lay.tile_tok - 1) / p.lay.tile_tok : 0;
       }
       long long a = n;
@@ -804,7 +808,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(AttnArgs p) {
   const Entry* entries = reinterpret_cast<const Entry*>(p.plan + p.lay.entries);
   const int g = p.nq / p.nkv, lane = threadIdx.x & 31;
   const int n = hdr->entries, jr = hdr->join_rows;
-  // (entries x kv heads x rows: below 2^31, since part rows x kv heads are)
+  // (entries x kv heads x rows: below 2^31, checked on the host)
   const uint32_t total = (uint32_t)n * p.nkv * jr, step = gridDim.x * (kJoinThreads / 32);
   for (uint32_t w = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5); w < total; w += step) {
     const uint32_t x = w / (uint32_t)jr, e = x / (uint32_t)p.nkv;

@@ -68,6 +68,7 @@ PLANS = [  # (cached, new, block size, spare rows)
     ([0] * 700, [(7 * i) % 31 for i in range(700)], 16, 100),
     ([i * 3 for i in range(1500)], [1] * 1500, 64, 0),
     ([0, 0], [70001, 33], 48, 7),
+    ([i % 40 for i in range(8192)], [i % 3 for i in range(8192)], 16, 5),  # the most requests: 98 KB of starts
 ]
 
 
@@ -444,6 +445,42 @@ def test_attn_prompt_reports_bad_pages_and_starts(cuda):
         assert int(plan.error) == ops.ERR_LENGTH and int(b["err"]) == 0
 
 
+@pytest.mark.parametrize("n", [-1, 0x7fff0001, 0x7fffffff])
+def test_attn_plan_lengths_out_of_range(cuda, n):
+    """A request of no valid length is left out and reported; the others are right."""
+    import torch
+    from spark_b200 import ops
+    nq, nkv, D, bs = 8, 2, 128, 16
+    b = _batch([0, 100], [30, 20], nq, nkv, D, bs, seed=7)
+    ref, mag = _attn_ref(b, nq, nkv, D, D ** -0.5)
+    b["lens"][1] = n
+    plan = ops.AttnPlan(50, 2, nq, nkv, D).update(b["start"], b["lens"])
+    out = torch.full_like(b["q"], 3.0)
+    ops.attn_prompt_out(b["q"], b["kc"], b["vc"], b["table"], plan, D ** -0.5, out, b["err"])
+    torch.cuda.synchronize()
+    assert int(plan.error) == ops.ERR_LENGTH and int(b["err"]) == 0
+    _close(out[:30], ref[:30], mag[:30])
+    assert bool((out[30:] == 3.0).all())
+    # a prefix of no valid length counts as none
+    one = _batch([40, 60], [1, 1], nq, nkv, D, bs, seed=8)
+    plan = ops.AttnPlan(2, 2, nq, nkv, D).update_prefix(one["lens"], torch.tensor([n], dtype=torch.int32, device="cuda"))
+    out = torch.full_like(one["q"], 3.0)
+    ops.attn_shared_prefix_out(one["q"], one["kc"], one["vc"], one["table"], plan, D ** -0.5, out, one["err"])
+    torch.cuda.synchronize()
+    assert int(plan.error) == ops.ERR_LENGTH and int(one["err"]) == 0
+    _close(out, *_attn_ref(one, nq, nkv, D, D ** -0.5))
+
+
+def test_paged_plan_refuses_outputs_that_are_inputs(cuda):
+    import torch
+    from spark_b200 import ops
+    from spark_b200._lib import SparkError
+    z = lambda n, t=torch.int32: torch.zeros(n, dtype=t, device="cuda")  # noqa: E731
+    ctx = z(2)
+    with pytest.raises(SparkError):  # lengths advanced in place: other blocks still read them
+        ops.paged_plan_out(ctx, z(2), z((2, 4)), 16, z(3), ctx, z(4, torch.int64), z(4, torch.int64), z(1), z(1))
+
+
 PREFIXES = [  # (prefix, own tokens of each request, nq, nkv, D, block size)
     (128, [1, 2], 8, 2, 128, 128),
     (2048, [1, 100, 7, 300, 128, 129, 1, 1], 32, 8, 128, 128),
@@ -656,6 +693,35 @@ def test_attn_prompt_pages_past_32_bit_offsets(cuda):
     assert torch.equal(kc[ids[0], :, 5], qkv[5].view(-1, D)[nq:nq + nkv])
     ref, mag = _attn_ref(b, nq, nkv, D, D ** -0.5)
     _close(out, ref, mag)
+
+
+@pytest.mark.parametrize("D,nq,nkv", [(128, 32, 8), (128, 24, 4), (256, 16, 4), (256, 24, 4)])
+def test_attn_prompt_same_bits_every_time(cuda, D, nq, nkv):
+    """Items of all kinds behind one another in a CTA (rows without tokens, whose warps skip
+    what the others wait for; references that move at every tile; parts): 200 replays, one
+    result."""
+    import torch
+    from spark_b200 import ops
+    ctx = [0, 2000, 77, 0, 5000, 31] * 12
+    new = [1, 3, 200, 130, 1, 33] * 12
+    b = _batch(ctx, new, nq, nkv, D, 16, seed=34)
+    at = torch.arange(16, device="cuda") / 4  # the reference moves inside a page and from page to page
+    b["kc"][:, :, :, 0] = (torch.rand((b["kc"].shape[0], 1, 1), device="cuda") * 60 + at).to(torch.bfloat16).expand(
+        b["kc"].shape[:3])
+    b["q"][:, :, 0] = 16
+    plan = ops.AttnPlan(b["q"].shape[0], len(ctx), nq, nkv, D).update(b["start"], b["lens"])
+    out = torch.zeros_like(b["q"])
+    ops.attn_prompt_out(b["q"], b["kc"], b["vc"], b["table"], plan, D ** -0.5, out, b["err"])
+    torch.cuda.synchronize()
+    ref, mag = _attn_ref(b, nq, nkv, D, D ** -0.5)
+    _close(out, ref, mag)
+    want = out.clone()
+    differ = torch.zeros(1, dtype=torch.int64, device="cuda")
+    for _ in range(200):
+        out.zero_()
+        ops.attn_prompt_out(b["q"], b["kc"], b["vc"], b["table"], plan, D ** -0.5, out, b["err"])
+        differ += (out.view(torch.int16) != want.view(torch.int16)).sum()
+    assert int(differ) == 0 and int(b["err"]) == 0
 
 
 def test_attn_two_calls_at_once_with_a_plan_each(cuda):
