@@ -321,11 +321,7 @@ __device__ __forceinline__ void store32(void* dst, const uint32_t* v, bool wide)
     reinterpret_cast<uint4*>(dst)[1] = make_uint4(v[4], v[5], v[6], v[7]);
   }
 }
-__device__ __forceinline__ int warp_min_i(int v) {
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) v = min(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
+__device__ __forceinline__ int warp_min_i(int v) { return __reduce_min_sync(0xffffffffu, v); }
 
 // The CTA's i-th work index (item x kv head): forward and backward through the CTAs in
 // turn, so that a CTA that got a long item of one pass gets a short one of the next.
@@ -754,6 +750,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) bar_arrive(bar(xbar));
       return wait(xbar, nx++ & 1);
     };
+    const int row_tok = r / g, head_row = r - row_tok * g;  // this thread's row: token of the half, head of the group
     for (;; qi++) {
       const int q = qi & 1;
       if (!(ok = wait(kBarQFull + q, (qi >> 1) & 1))) break;
@@ -767,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // alternating tiles: the item's tile t is in score buffer (par + t) & 1; few rows: this
       // half has the tiles of its own buffer, t0, t0 + 2 ..
       const int t0 = few ? (int)(h ^ par) : 0;
-      const int local = r / g + (D == 128 && !few ? h * p.lay.half_tok : 0);  // token of the item
+      const int local = row_tok + (D == 128 && !few ? h * p.lay.half_tok : 0);  // token of the item
       const bool valid = r < g * p.lay.half_tok && local < it.ntok && it.tok0 + local < p.tokens;
       const int2 kk = valid ? row_keys(it, lens, p.window, local) : make_int2(0, 0);
       const bool any_valid = __any_sync(0xffffffffu, valid);
@@ -932,20 +929,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (any_valid) {
-        const int head_row = r % g, tok = it.tok0 + local, head = kvh * g + head_row;
-        const float inv = 1.0f / l;
+        const int tok = it.tok0 + local, head = kvh * g + head_row;
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // (no key at all: zero)
         // (few rows: the even tiles' part, then the odd ones')
         const int64_t prow = (int64_t)(it.part + (t0 * it.ntok + local) * g + head_row) * p.nkv + kvh;
-#pragma unroll 1
+        // (loads of tensor memory in flight together, as far as the registers go: one after
+        // the other a wide window takes 4% longer, all four at head_dim 128 the rest 2%)
+#pragma unroll(D == 128 ? 2 : 4)
         for (int i = 0; i < 4; i++) {
           const int col = sp * 64 + 16 * i;
-          float o[16];
+          float o[16] = {};
           if (mine > 0) tm_load16(ob + 16 * i, o);
           if (valid && it.part < 0) {
             uint32_t v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++)  // (no key at all: zero)
-              v[j] = l != 0.0f ? pack_bf16(o[2 * j] * inv, o[2 * j + 1] * inv) : 0;
+            for (int j = 0; j < 8; j++) v[j] = pack_bf16(o[2 * j] * inv, o[2 * j + 1] * inv);
             store32(p.out + tok * p.o_tok + head * p.o_head + col, v, args.wide);
           } else if (valid && l != 0.0f) {
             float* dst = p.part_o + prow * D + col;
