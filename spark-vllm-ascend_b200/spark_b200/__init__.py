@@ -5,6 +5,8 @@ Subpackages / modules:
   ops       torch-facing operators and torch.ops.spark_b200.* registrations
   config    SparkConfig (synthetic 4B decoder by default)
   model     synthetic weights, paged KV cache and the CUDA-graph decode engine
+  prefill   batched and packed prompt prefill
+  batch     decode of several sequences in one launch per step
   plugin    vLLM general-plugin entry point (registration only)
 """
 from __future__ import annotations
