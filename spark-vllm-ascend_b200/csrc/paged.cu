@@ -57,13 +57,13 @@ int spark_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int reqs,
   if (!ctx_lens || !new_lens || !block_table || !query_start || !seq_lens || !error || !counter)
     return SPARK_ERR_INVALID_ARG;
   if (rows > 0 && (!positions || !slot_mapping)) return SPARK_ERR_INVALID_ARG;
-  // every CTA reads all lengths, while others write already
-  if (seq_lens == ctx_lens || seq_lens == new_lens || query_start == ctx_lens || query_start == new_lens)
-    return SPARK_ERR_INVALID_ARG;
   if (free_blocks ? (!free_head || !free_head_out) : (free_head || free_head_out)) return SPARK_ERR_INVALID_ARG;
   if (reqs <= 0 || rows < 0 || num_free < 0 || block_size <= 0 || table_width <= 0 || table_stride < table_width)
     return SPARK_ERR_UNSUPPORTED_SHAPE;
   if (reqs > paged::kPlanMaxReqs) return SPARK_ERR_TOO_LARGE;
+  // every CTA reads all lengths, while others write already
+  if (seq_lens == ctx_lens || seq_lens == new_lens || query_start == ctx_lens || query_start == new_lens)
+    return SPARK_ERR_INVALID_ARG;
   paged::PlanArgs p;
   memset(&p, 0, sizeof(p));
   p.ctx = ctx_lens, p.nw = new_lens, p.free_ids = free_blocks, p.free_head = free_head;

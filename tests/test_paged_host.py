@@ -31,7 +31,8 @@ def _plan(L, **k):
     (dict(ctx=None), INVALID), (dict(error=None), INVALID), (dict(counter=None), INVALID), (dict(rows=5), INVALID),
     (dict(head=None), INVALID), (dict(free=None), INVALID), (dict(head_out=None), INVALID), (dict(reqs=0), SHAPE),
     (dict(reqs=-3), SHAPE), (dict(rows=-1), SHAPE), (dict(bs=0), SHAPE), (dict(width=0), SHAPE),
-    (dict(stride=7), SHAPE), (dict(num_free=-1), SHAPE), (dict(reqs=8193), LARGE)])
+    (dict(stride=7), SHAPE), (dict(num_free=-1), SHAPE), (dict(reqs=8193), LARGE),
+    (dict(qs=OFF), INVALID), (dict(sl=OFF), INVALID)])  # (seq_lens / query_start in the place of the lengths)
 def test_paged_plan_refuses(L, bad, status):
     assert _plan(L, **bad) == status
 
@@ -52,6 +53,13 @@ def _rows(L, **k):
     (dict(qkv=OFF), ALIGN), (dict(kc=OFF), ALIGN), (dict(q=OFF), ALIGN), (dict(kg=OFF), ALIGN)])
 def test_rope_store_refuses(L, bad, status):
     assert _rows(L, **bad) == status
+
+
+def test_attn_plan_sizes_too_large_are_refused(L):
+    for fn in (L.spark_attn_plan_bytes, L.spark_attn_part_rows):
+        assert fn(1 << 16, 1 << 16, 128, 128, 128) == -1  # rows to join past 2^30
+        assert fn(1 << 16, 1 << 15, 32, 8, 128) > 0
+        assert fn((1 << 22) + 1, 1, 32, 8, 128) == -1
 
 
 def test_rope_store_of_no_rows_is_no_work(L):
