@@ -308,6 +308,8 @@ __device__ __forceinline__ void probs16(const float* s, u64 c2, u64 neg2, u64 (&
                "r"(pk[2]), "r"(pk[3]), "r"(pk[4]), "r"(pk[5]), "r"(pk[6]), "r"(pk[7]), "r"(addr)
                : "memory");
 }
+// (head_dim 256 has half the exponentials to the same products and takes none: wide window 62.5
+// -> 61 us; head_dim 128 with 0 / 1 / 2 / 3 of 8 pairs: 8 packed prompts 167 / 165.6 / 165.4 / 167.5 us)
 constexpr int kPolyPairs = 2;
 
 // 32 bytes (wide) or two times 16 to global memory
@@ -882,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int q = 0; q < NQ; q++) {
             if (q > 0) load(q);
             const uint32_t pb = sb + 64 * q + 32 * sp;
-            if (edge) {
+            if (D == 256 || edge) {
               probs16<0>(s, c2, neg2, sum, pb);
               probs16<0>(s + 16, c2, neg2, sum, pb + 8);
             } else {
