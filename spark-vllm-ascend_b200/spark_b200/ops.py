@@ -302,13 +302,14 @@ ERR_PAGE, ERR_POSITION, ERR_SLOT = 64, 128, 256
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _launch(dev: int, name: str, *args) -> None:
     """Launch on device ``dev`` (the tensors' own), on its current stream.  Pointers are
     passed as integers and the checks below build no message before one fails: these
     calls are made per layer and step, where host time counts."""
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         call(name, *args, _raw_stream(dev))
         return
     with torch.cuda.device(dev):
@@ -325,6 +326,14 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int) -> None:
         return
     _cuda(t, name, dtype)
     raise ValueError(f"{name} must be on cuda:{dev}, got {t.device}")
+
+
+def _need_all(dev: int, dtype: torch.dtype, tensors, names) -> None:
+    """``_need`` of several tensors (in one loop: 0.1 us a tensor instead of 0.2)."""
+    for t in tensors:
+        if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+            for u, name in zip(tensors, names):
+                _need(u, name, dtype, dev)
 
 
 def _home(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
@@ -355,14 +364,9 @@ def paged_plan_out(ctx_lens, new_lens, block_table, block_size, query_start, seq
     i32 = torch.int32
     dev = _home(ctx_lens, "ctx_lens", i32)
     R, rows = ctx_lens.numel(), positions.numel()
-    _need(ctx_lens, "ctx_lens", i32, dev)
-    _need(new_lens, "new_lens", i32, dev)
-    _need(query_start, "query_start", i32, dev)
-    _need(seq_lens, "seq_lens", i32, dev)
-    _need(counter, "counter", i32, dev)
-    _need(error, "error", i32, dev)
-    _need(positions, "positions", torch.int64, dev)
-    _need(slot_mapping, "slot_mapping", torch.int64, dev)
+    _need_all(dev, i32, (ctx_lens, new_lens, query_start, seq_lens, counter, error),
+              ("ctx_lens", "new_lens", "query_start", "seq_lens", "counter", "error"))
+    _need_all(dev, torch.int64, (positions, slot_mapping), ("positions", "slot_mapping"))
     if R < 1 or new_lens.numel() != R or seq_lens.numel() != R or query_start.numel() != R + 1:
         raise ValueError("ctx_lens, new_lens and seq_lens hold one entry per request, query_start one more")
     if slot_mapping.numel() != rows:
@@ -374,9 +378,7 @@ def paged_plan_out(ctx_lens, new_lens, block_table, block_size, query_start, seq
         raise ValueError("give free_blocks and free_head together (and free_head_out only with them)")
     if free_blocks is not None:
         free_head_out = free_head if free_head_out is None else free_head_out
-        _need(free_blocks, "free_blocks", i32, dev)
-        _need(free_head, "free_head", i32, dev)
-        _need(free_head_out, "free_head_out", i32, dev)
+        _need_all(dev, i32, (free_blocks, free_head, free_head_out), ("free_blocks", "free_head", "free_head_out"))
         if free_head.numel() != 1 or free_head_out.numel() != 1:
             raise ValueError("free_head must hold one int32")
     width = block_table.shape[1]
@@ -399,12 +401,8 @@ def qk_norm_rope_store_rows(qkv, nq, nkv, head_dim, q_gamma, k_gamma, eps, cos_s
     if qkv.dim() != 2 or (qkv.stride(1) != 1 and qkv.shape[1] != 1) or qkv.shape[1] < (nq + 2 * nkv) * head_dim:
         raise ValueError(f"qkv must be [rows, >= {(nq + 2 * nkv) * head_dim}] with dense rows, got {tuple(qkv.shape)}")
     rows = qkv.shape[0]
-    _need(cos_sin, "cos_sin", BF16, dev)
-    _need(k_cache, "k_cache", BF16, dev)
-    _need(v_cache, "v_cache", BF16, dev)
-    _need(q_out, "q_out", BF16, dev)
-    _need(positions, "positions", torch.int64, dev)
-    _need(slot_mapping, "slot_mapping", torch.int64, dev)
+    _need_all(dev, BF16, (cos_sin, k_cache, v_cache, q_out), ("cos_sin", "k_cache", "v_cache", "q_out"))
+    _need_all(dev, torch.int64, (positions, slot_mapping), ("positions", "slot_mapping"))
     _need(error, "error", torch.int32, dev)
     if positions.numel() < rows or slot_mapping.numel() < rows:
         raise ValueError("positions and slot_mapping must hold one entry per row")
@@ -413,8 +411,7 @@ def qk_norm_rope_store_rows(qkv, nq, nkv, head_dim, q_gamma, k_gamma, eps, cos_s
     if (q_gamma is None) != (k_gamma is None):
         raise ValueError("give q_gamma and k_gamma together")
     if q_gamma is not None:
-        _need(q_gamma, "q_gamma", BF16, dev)
-        _need(k_gamma, "k_gamma", BF16, dev)
+        _need_all(dev, BF16, (q_gamma, k_gamma), ("q_gamma", "k_gamma"))
         if q_gamma.numel() != head_dim or k_gamma.numel() != head_dim:
             raise ValueError("q_gamma and k_gamma must hold head_dim values")
     if cos_sin.dim() != 2:
@@ -509,8 +506,7 @@ def _attn_paged(kind, q, k_cache, v_cache, block_table, plan, scale, out, error,
     tokens = q.shape[0]
     if out.shape[0] < tokens or tokens > plan.max_tokens:
         raise ValueError(f"{tokens} tokens: out has {out.shape[0]} rows, the plan room for {plan.max_tokens}")
-    _need(k_cache, "k_cache", BF16, dev)
-    _need(v_cache, "v_cache", BF16, dev)
+    _need_all(dev, BF16, (k_cache, v_cache), ("k_cache", "v_cache"))
     ks = k_cache.shape
     if len(ks) != 4 or v_cache.shape != ks or ks[1] != nkv or ks[3] != D:
         raise ValueError(f"caches must be [blocks, {nkv}, block_size, {D}]")
