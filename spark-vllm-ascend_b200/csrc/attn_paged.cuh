@@ -23,7 +23,7 @@
 //                   piece and 64 columns into the ring, 128-byte swizzle;
 //   warp 17         owns the tensor memory; one lane issues all MMAs and commits;
 //   warp 18         the next item's description and Q, as soon as the last score product has
-//                   read the buffer (warp 19 only completes the register split).
+//                   read the buffer (warp 19 is idle).
 // Shared memory: Q 64 KB, a ring of five 32-KB chunks (128 keys x 128 columns of K or V).
 // Tensor memory: scores S0 S1 (128 columns each; the p of 32 keys are written over the first
 // half of their scores' columns, which no other warp reads), sums O0 O1.
@@ -65,11 +65,6 @@ namespace paged {
 namespace tc {
 
 constexpr int kThreads = 640;
-// registers: 96 a thread at launch; for head_dim 128 warps 16-19 give up 32 each and the
-// softmax warps take 8 (4 x 104 + 64 = 5 x 96): a spill in the softmax loop costs the shared
-// memory bandwidth that the MMAs live on (150 bytes: a third more time).  For head_dim 256 a
-// softmax thread has half as many scores and 96 do.
-constexpr int kRegsLaunch = 96, kRegsSoftmax = 104, kRegsRest = 64;
 constexpr int kSoftmaxWarps = 16;
 constexpr int kProducerWarp = 16, kMmaWarp = 17, kQWarp = 18;
 constexpr int kStages = 5;
@@ -409,10 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t nwork = (uint32_t)hdr->items * (uint32_t)p.nkv, room = (uint32_t)p.lay.max_items * (uint32_t)p.nkv;
   const int g = p.nq / p.nkv;
 
-  // (each warpgroup changes its share inside its own branch, where the register allocator
-  // can tell which share holds)
   if (warp >= kSoftmaxWarps) {
-    if (D == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
     if (warp == kProducerWarp) {
       // ---------------------------------------------------------------- K / V producer
       uint32_t ring = 0;
@@ -550,47 +542,101 @@ __global__ void __launch_bounds__(kThreads, 1)
       // values in uniform registers; one lane, always the same, issues.  Issued from a
       // one-lane branch instead, an MMA took about 80 cycles to hand over.)
       {
-        uint32_t ring = 0, qi = 0, np[2] = {0, 0};  // ring: first chunk of the item
+        uint32_t qi = 0, np[2] = {0, 0};
         bool ok = true;
-        auto wait = [&](int i, uint32_t parity) -> bool {
-          return __all_sync(0xffffffffu, bar_wait(bar(i), parity, limit_ns, abort_flag));
-        };
+        // head_dim 256: mostly what is waited for is done, and one look at all of it together costs
+        // 200 cycles in which the tensor pipe runs dry, a look at each as much again (one unit
+        // 1.87 -> 1.68 us).  At head_dim 128 probabilities are mostly waited for: looks in front of
+        // the wait cost 2%.
         auto ready = [&](int i, uint32_t parity) -> bool { return __all_sync(0xffffffffu, bar_test(bar(i), parity)); };
-        auto full = [&](uint32_t r) -> bool {
-          return wait(kBarFull + r % kStages, (r / kStages) & 1);
+        auto wait = [&](int i, uint32_t parity) -> bool {
+          return (D == 256 && ready(i, parity)) || __all_sync(0xffffffffu, bar_wait(bar(i), parity, limit_ns, abort_flag));
         };
-        auto stage = [&](uint32_t r) { return base + kOffRing + (r % kStages) * kChunk; };
-        // S_h = Q_q K^T of the tile whose first chunk is r
-        auto scores = [&](int h, int q, uint32_t r) {
+        // A place in the ring; chunks are used in ring order, but for the scores of a next item
+        // that are issued early
+        struct Pos {
+          uint32_t s, ph;
+        };
+        Pos cur{0, 0};
+        auto step = [](Pos r, int k) -> Pos {  // (k < kStages)
+          r.s += (uint32_t)k;
+          if (r.s >= (uint32_t)kStages) {
+            r.s -= kStages;
+            r.ph ^= 1;
+          }
+          return r;
+        };
+        // the tile at r is in shared memory and phase `parity` of barrier i (-1: none) is over
+        auto ready_tile = [&](Pos r, int i, uint32_t parity) -> bool {
+          const Pos x = step(r, NC - 1);
+          const bool a = bar_test(bar(kBarFull + r.s), r.ph), b = NC == 1 || bar_test(bar(kBarFull + x.s), x.ph);
+          return __all_sync(0xffffffffu, a && b && (i < 0 || bar_test(bar(i), parity)));
+        };
+        auto full_tile = [&](Pos r) -> bool {
+          if (ready_tile(r, -1, 0)) return true;
+          bool f = wait(kBarFull + r.s, r.ph);
+          if (NC == 2) f = f && wait(kBarFull + step(r, 1).s, step(r, 1).ph);
+          return f;
+        };
+        auto stage = [&](Pos r) { return base + kOffRing + r.s * kChunk; };
+        // S_h = Q_q K^T of the tile at r; then, all announced from the same lane's turn, the
+        // scores, the tile's place (`done`) and a barrier of the caller's (or -1)
+        auto scores = [&](int h, int q, Pos r, bool done, int also) {
 #pragma unroll
           for (int c = 0; c < NC; c++) {
-            const uint64_t kd = desc_k(stage(r + c)), qd = desc_k(base + (uint32_t)(q * kChunk + c * kChunk));
+            const uint64_t kd = desc_k(stage(step(r, c))), qd = desc_k(base + (uint32_t)(q * kChunk + c * kChunk));
             if (elect_one()) {
 #pragma unroll
               for (int j = 0; j < 8; j++) {
                 const uint32_t off = (uint32_t)((j >> 2) * (kSub >> 4) + 2 * (j & 3));
                 mma_ss(tmem + kColS + h * 128, qd + off, kd + off, kIdescS, (c | j) != 0);
               }
-              if (c == NC - 1) commit(bar(kBarS + h));
+              if (c == NC - 1) {
+                commit(bar(kBarS + h));
+                if (done) {
+                  commit(bar(kBarEmpty + r.s));
+                  if (NC == 2) commit(bar(kBarEmpty + step(r, 1).s));
+                }
+                if (also >= 0) commit(bar(also));
+              }
             }
             __syncwarp();
           }
         };
-        // O += P_h V of the tile whose first chunk is r, in two steps: the first 64 keys'
-        // probabilities are multiplied while the others are still computed
-        auto sums = [&](int h, int o, uint32_t r, uint32_t accum) -> bool {
+        // O += P_h V of the tile at r (`fresh`: V has not been waited for), in two steps: the
+        // first 64 keys' probabilities are multiplied while the others are still computed.
+        // `seen`: in, whether to look for the tile at `next` on the way; out, whether it is there.
+        auto sums = [&](int h, int o, Pos r, uint32_t accum, bool fresh, bool done, int also, bool& seen,
+                        Pos next) -> bool {
 #pragma unroll
           for (int k = 0; k < 2; k++) {
-            if (!wait((k ? kBarP2 : kBarP) + h, np[h] & 1)) return false;
+            const int pb = (k ? kBarP2 : kBarP) + h;
+            const uint32_t pp = np[h] & 1;
+            if (k == 0 && fresh) {
+              if (!ready_tile(r, pb, pp) && !(full_tile(r) && wait(pb, pp))) return false;
+            } else if (k == 1 && seen) {
+              seen = ready_tile(next, pb, pp);
+              if (!seen && !wait(pb, pp)) return false;
+            } else if (!wait(pb, pp)) {
+              return false;
+            }
             fence_after();
 #pragma unroll
             for (int c = 0; c < NC; c++) {
-              const uint64_t vd = desc_v(stage(r + c));
+              const uint64_t vd = desc_v(stage(step(r, c)));
               if (elect_one()) {
 #pragma unroll
                 for (int j = 4 * k; j < 4 * k + 4; j++)
                   mma_ts(tmem + kColO + (o + c) * 128, tmem + kColS + h * 128 + 32 * (j >> 1) + 8 * (j & 1),
                          vd + j * (2048 >> 4), kIdescO, accum | (j != 0));
+                if (k == 1 && c == NC - 1) {
+                  if (D == 256) commit(bar(kBarPV + h));
+                  if (done) {
+                    commit(bar(kBarEmpty + r.s));
+                    if (NC == 2) commit(bar(kBarEmpty + step(r, 1).s));
+                  }
+                  if (also >= 0) commit(bar(also));
+                }
               }
               __syncwarp();
             }
@@ -602,28 +648,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (elect_one()) commit(bar(i));
           __syncwarp();
         };
-        auto release = [&](uint32_t r) {
-#pragma unroll
-          for (int c = 0; c < NC; c++) announce(kBarEmpty + (r + c) % kStages);
-        };
-        auto full_tile = [&](uint32_t r) {
-          bool f = full(r);
-          if (NC == 2) f = f && full(r + 1);
-          return f;
-        };
         // tiles and mode of the item in slot i & 1
         auto describe = [&](uint32_t i, int& tiles, bool& alternate) {
           const Item* slot = reinterpret_cast<const Item*>(gbase + kOffItem + 64 * (i & 1));
           tiles = __shfl_sync(0xffffffffu, slot->nkt, 0);
           alternate = D == 256 || (__shfl_sync(0xffffffffu, slot->flags, 0) & kFlagFew);
         };
-        // Alternating tiles: the scores of tile t of item i (first chunk r), into buffer b
-        auto alt_scores = [&](uint32_t i, int t, int n, int b, uint32_t r) {
-          const uint32_t rk = r + (uint32_t)(NC * k_index(t, 2));
+        // Alternating tiles: the scores of tile t of item i (its K at r), into buffer b
+        auto alt_scores = [&](uint32_t i, int t, int n, int b, Pos r) {
           fence_after();
-          scores(b, D == 256 ? 0 : (int)(i & 1), rk);
-          release(rk);
-          if (t + 1 == n) announce(kBarQEmpty + (i & 1));
+          scores(b, D == 256 ? 0 : (int)(i & 1), r, true, t + 1 == n ? kBarQEmpty + (int)(i & 1) : -1);
         };
         int early = 0;      // score tiles of this item that were issued behind the last one's
         uint32_t par = 0;   // score buffer of the item's first alternating tile
@@ -645,51 +679,48 @@ __global__ void __launch_bounds__(kThreads, 1)
             continue;
           }
           if (!alternate) {
-            if (!(ok = full(ring))) break;
+            if (!(ok = full_tile(cur))) break;
             fence_after();
-            scores(0, 0, ring);
-            scores(1, 1, ring);
-            release(ring);
-            if (n == 1) announce(kBarQEmpty + (qi & 1));
-            ring++;
+            scores(0, 0, cur, false, -1);
+            scores(1, 1, cur, true, n == 1 ? kBarQEmpty + (int)(qi & 1) : -1);
+            cur = step(cur, 1);
             for (int t = 0; t < n && ok; t++) {
-              const uint32_t rv = ring, rk = ring + 1;
               const bool more = t + 1 < n;
-              if (!(ok = full(rv))) break;
+              const Pos rv = cur, rk = step(cur, 1);
               for (int h = 0; h < 2; h++) {
-                if (!(ok = sums(h, h, rv, t > 0))) break;
-                if (h == 0 && more) {
-                  if (!(ok = full(rk))) break;
+                bool seen = false;
+                if (!(ok = sums(h, h, rv, t > 0, h == 0, h == 1, more ? -1 : kBarO + h, seen, rk))) break;
+                if (!more) continue;
+                if (h == 0) {
+                  if (!(ok = seen || full_tile(rk))) break;
                   fence_after();
                 }
-                if (more) scores(h, h, rk);
-                else announce(kBarO + h);
+                scores(h, h, rk, h == 1, h == 1 && t + 2 == n ? kBarQEmpty + (int)(qi & 1) : -1);
               }
-              if (!ok) break;
-              release(rv);
-              if (more) release(rk);
-              if (t + 2 == n) announce(kBarQEmpty + (qi & 1));
-              ring += more ? 2 : 1;
+              cur = step(cur, more ? 2 : 1);
             }
             if (!ok) break;
           } else {
             for (int t = early; t < 2 && t < n && ok; t++) {
-              if (!(ok = full_tile(ring + NC * k_index(t, 2)))) break;
-              alt_scores(qi, t, n, (par + t) & 1, ring);
+              const Pos rk = step(cur, NC * t);
+              if (!(ok = full_tile(rk))) break;
+              alt_scores(qi, t, n, (par + t) & 1, rk);
             }
             if (!ok) break;
             early = 0;
-            const uint32_t next_ring = ring + (uint32_t)(2 * NC * n);
+            cur = step(cur, NC * (n < 2 ? n : 2));
             for (int t = 0; t < n; t++) {
               const int b = (par + t) & 1;
-              const uint32_t rv = ring + (uint32_t)(NC * v_index(t, n, 2));
-              if (!(ok = full_tile(rv) && sums(b, D == 128 ? b : 0, rv, D == 128 ? t > 1 : t > 0))) break;
-              if (D == 256) announce(kBarPV + b);
-              if (D == 256 ? t + 1 == n : t + 2 >= n) announce(kBarO + (D == 128 ? b : 0));
-              release(rv);
+              const bool end = D == 256 ? t + 1 == n : t + 2 >= n;  // of this buffer's sums
+              bool seen = t + 2 < n;
+              if (!(ok = sums(b, D == 128 ? b : 0, cur, D == 128 ? t > 1 : t > 0, true, true,
+                              end ? kBarO + (D == 128 ? b : 0) : -1, seen, step(cur, NC))))
+                break;
+              cur = step(cur, NC);
               if (t + 2 < n) {
-                if (!(ok = full_tile(ring + NC * k_index(t + 2, 2)))) break;
-                alt_scores(qi, t + 2, n, b, ring);
+                if (!(ok = seen || full_tile(cur))) break;
+                alt_scores(qi, t + 2, n, b, cur);
+                cur = step(cur, NC);
                 continue;
               }
               // The next item's first scores fill the gap while this one's last softmax
@@ -699,16 +730,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 known = true;
               }
               for (; known && next_alt && early < t + 3 - n && early < next_n; early++) {
-                const uint32_t rk = next_ring + (uint32_t)(NC * k_index(early, 2));
-                if (!ready(kBarFull + rk % kStages, (rk / kStages) & 1) ||
-                    (NC == 2 && !ready(kBarFull + (rk + 1) % kStages, ((rk + 1) / kStages) & 1)))
-                  break;
-                alt_scores(qi + 1, early, next_n, (par + n + early) & 1, next_ring);
+                const Pos rk = step(step(cur, NC * (n - 1 - t)), NC * early);  // behind this item's last V
+                if (!ready_tile(rk, -1, 0)) break;
+                alt_scores(qi + 1, early, next_n, (par + n + early) & 1, rk);
               }
             }
             if (!ok) break;
             par = (par + n) & 1;
-            ring = next_ring;
           }
         }
         if (!ok && lane == 0) fail();
@@ -721,7 +749,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
     }
   } else {
-    if (D == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ---------------------------------------------------------------- softmax and epilogue
     // SP warpgroups share the rows of a half (a thread of each owns the same row), 128 / SP
     // score columns and 64 sum columns each

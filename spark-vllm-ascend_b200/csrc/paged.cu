@@ -28,14 +28,6 @@ static int attn_launch(const paged::AttnArgs& p, int64_t wait_ns, cudaStream_t s
       !encode_map(&mk, bf, p.k_cache, D, rows, D * 2, 64, (uint32_t)t.piece, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !encode_map(&mv, bf, p.v_cache, D, rows, D * 2, 64, (uint32_t)t.piece, CU_TENSOR_MAP_SWIZZLE_128B))
     return SPARK_ERR_LAUNCH;
-  // the register split inside the kernel draws on what it was launched with: a build that
-  // uses fewer registers a thread would wait for ever, so it is refused here
-  static const bool split_ok = [] {
-    cudaFuncAttributes fa;
-    return cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(&paged::tc::attn_kernel<D>)) == cudaSuccess &&
-           (D != 128 || fa.numRegs >= paged::tc::kRegsLaunch);
-  }();
-  if (!split_ok) return SPARK_ERR_LAUNCH;
   const int grid = (int)std::min<int64_t>((int64_t)p.lay.max_items * p.nkv, num_sms());
   const int st = launch(paged::tc::attn_kernel<D>, dim3(grid), dim3(paged::tc::kThreads), paged::tc::kSmemBytes,
                         stream, mq, mk, mv, t);
