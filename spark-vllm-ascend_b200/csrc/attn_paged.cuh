@@ -44,6 +44,13 @@
 // when every warp of the half has rescaled its columns of it, or read them out for the last
 // item.
 //
+// Measured (32 query and 8 kv heads of 128): a causal prompt of 16384 1.97 ms = 1118 TFLOP/s (1044 when
+// repeated until the power cap takes the clock to 1.63 GHz), of 2048 47 us; 8 tokens behind 32768
+// keys each 136 us = 6.1 TB/s.  A unit of 256 rows x 128 keys takes 1.93 us (head_dim 256, 128 rows:
+// 1.68 us) where its products alone take 1.15: a half's scores, maximum, probabilities and sums
+// follow one another, two halves fill each other's gaps, and a third set of scores has no room in
+// tensor memory.  Around an item 3-4 us, around a call (with the join) 9-10 us.
+//
 // Stale memory: a K / V row at or past the request's length (or before the window) may hold
 // anything.  Scores are masked by selection, and V rows outside [klo, len) are zeroed in
 // shared memory before their product, since 0 * NaN is NaN.
