@@ -666,6 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_after();
           scores(b, D == 256 ? 0 : (int)(i & 1), r, true, t + 1 == n ? kBarQEmpty + (int)(i & 1) : -1);
         };
+        bool first0 = false;  // half 0's first scores of this item were issued behind the last one's
         int early = 0;      // score tiles of this item that were issued behind the last one's
         uint32_t par = 0;   // score buffer of the item's first alternating tile
         // What was read of the next item ahead of its turn is kept: once its scores are issued
@@ -688,25 +689,40 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!alternate) {
             if (!(ok = full_tile(cur))) break;
             fence_after();
-            scores(0, 0, cur, false, -1);
+            if (!first0) scores(0, 0, cur, false, -1);
+            first0 = false;
             scores(1, 1, cur, true, n == 1 ? kBarQEmpty + (int)(qi & 1) : -1);
             cur = step(cur, 1);
-            for (int t = 0; t < n && ok; t++) {
-              const bool more = t + 1 < n;
+            bool unseen = false;  // (no look for the next K on the way: see wait)
+            for (int t = 0; t + 1 < n && ok; t++) {
               const Pos rv = cur, rk = step(cur, 1);
               for (int h = 0; h < 2; h++) {
-                bool seen = false;
-                if (!(ok = sums(h, h, rv, t > 0, h == 0, h == 1, more ? -1 : kBarO + h, seen, rk))) break;
-                if (!more) continue;
+                if (!(ok = sums(h, h, rv, t > 0, h == 0, h == 1, -1, unseen, rk))) break;
                 if (h == 0) {
-                  if (!(ok = seen || full_tile(rk))) break;
+                  if (!(ok = full_tile(rk))) break;
                   fence_after();
                 }
                 scores(h, h, rk, h == 1, h == 1 && t + 2 == n ? kBarQEmpty + (int)(qi & 1) : -1);
               }
-              cur = step(cur, more ? 2 : 1);
+              cur = step(cur, 2);
             }
             if (!ok) break;
+            const Pos rv = cur;
+            cur = step(cur, 1);
+            if (!(ok = sums(0, 0, rv, n > 1, true, false, kBarO, unseen, cur))) break;
+            // half 0's first scores of the next item, if its Q and K are there already, so that
+            // they are done when the half's warps have written this one's rows (1% of a prompt
+            // of 2048; inside the loop above the same look cost the other tiles 2%)
+            if (ready(kBarQFull + ((qi + 1) & 1), ((qi + 1) >> 1) & 1)) {
+              describe(qi + 1, next_n, next_alt);
+              known = true;
+              if (!next_alt && next_n > 0 && ready_tile(cur, -1, 0)) {
+                fence_after();
+                scores(0, 0, cur, false, -1);
+                first0 = true;
+              }
+            }
+            if (!(ok = sums(1, 1, rv, n > 1, false, true, kBarO + 1, unseen, cur))) break;
           } else {
             for (int t = early; t < 2 && t < n && ok; t++) {
               const Pos rk = step(cur, NC * t);
