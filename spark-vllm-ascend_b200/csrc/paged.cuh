@@ -456,8 +456,8 @@ __device__ __forceinline__ Tile prompt_tile(const AttnPlanArgs& p, int q0, int n
   t.len = len;
   const int last = t.pos0 + t.ntok;  // exclusive causal limit of the last row
   t.khi = last < 0 ? 0 : last;
-  const int lo = p.window > 0 ? t.pos0 + 1 - p.window : 0;
-  t.klo = lo < 0 ? 0 : lo;
+  // (compared first: with a window near 2^31 the difference of a negative position wraps)
+  t.klo = p.window > 0 && t.pos0 >= p.window ? t.pos0 + 1 - p.window : 0;
   t.key0 = t.klo / kKeyTile * kKeyTile;
   t.nkt = t.khi > t.klo ? (t.khi - t.key0 + kKeyTile - 1) / kKeyTile : 0;
   t.flags = p.D == 128 && t.ntok <= p.lay.half_tok && t.nkt > 1 ? kFlagFew : 0;
@@ -788,7 +788,7 @@ __device__ __forceinline__ int2 row_keys(const Item& it, const int* lens, int wi
   } else {
     const int pos = it.pos0 + i;
     hi = pos + 1 < hi ? pos + 1 : hi;
-    if (window > 0 && pos + 1 - window > lo) lo = pos + 1 - window;
+    if (window > 0 && pos >= window && pos + 1 - window > lo) lo = pos + 1 - window;  // (see prompt_tile)
   }
   return make_int2(lo, hi);
 }

@@ -66,3 +66,24 @@ def test_attn_prompt_infinite_scores(cuda, D, nq, nkv, new):
                 assert bool(out[first:end].isnan().all()), i
             else:
                 _close(out[first:end], ref[first:end], mag[first:end])
+
+
+@pytest.mark.parametrize("D,nq,nkv", [(128, 8, 2), (256, 8, 2)])
+@pytest.mark.parametrize("window", [0x7fffffff, 0x7fff0000, 1 << 30, 0])
+def test_attn_prompt_window_larger_than_any_request(cuda, D, nq, nkv, window):
+    """A window past every length is no window, also for rows in front of the first key (more
+    queries than keys)."""
+    import torch
+    from spark_b200 import ops
+    b = _batch([0, 0], [140, 20], nq, nkv, D, 16, seed=62)
+    lens = [100, 20]
+    b["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+    b["len"] = lens
+    plan = ops.AttnPlan(160, 2, nq, nkv, D, window=window).update(b["start"], b["lens"])
+    out = torch.full_like(b["q"], float("nan"))
+    ops.attn_prompt_out(b["q"], b["kc"], b["vc"], b["table"], plan, D ** -0.5, out, b["err"])
+    torch.cuda.synchronize()
+    assert int(b["err"]) == 0 and int(plan.error) == 0
+    ref, mag = _attn_ref(b, nq, nkv, D, D ** -0.5)
+    assert bool((out[:40] == 0).all()) and bool((out[40:140] != 0).any())
+    _close(out, ref, mag)
