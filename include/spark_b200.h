@@ -278,7 +278,8 @@ int spark_qk_norm_rope_store_rows(const uint16_t* qkv, int64_t row_stride, int r
  * its seq_lens[r] keys; `window` > 0: each token attends to its last `window` positions,
  * itself included.  prefix_len given (device int32, and query_start NULL): one query token
  * per request, request r attends to all its seq_lens[r] keys, the first *prefix_len of
- * which are the same for all and are read through the first request's table, once.
+ * which are the same for all and are read through the first request's table, once (a
+ * shorter request sees its own seq_lens[r] of them; what lies behind the longest one is not read).
  * plan: spark_attn_plan_bytes bytes for the same maxima, 16-byte aligned;
  * reqs <= max_reqs.  Starts outside [0, max_tokens] or descending drop the request. */
 int64_t spark_attn_plan_bytes(int max_tokens, int max_reqs, int nq, int nkv, int head_dim);

@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
   // of small batches: first tile per request, and (key tiles, flags | rows << 8) per tile
   __shared__ int starts_s[kPlanStarts + 1];
   __shared__ int2 brief_s[kPlanTiles];
-  __shared__ int entries_s, rows_s, bad_s, join_s;
+  __shared__ int entries_s, rows_s, bad_s, join_s, keys_s;
   const int tid = threadIdx.x, R = p.reqs;
   Header* hdr = reinterpret_cast<Header*>(p.plan);
   Item* items = reinterpret_cast<Item*>(p.plan + p.lay.items);
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
   int2* bases = reinterpret_cast<int2*>(p.plan + p.lay.bases);  // (first partial row, parts)
   int* lens = reinterpret_cast<int*>(p.plan + p.lay.lens);
   pdl_wait();
-  if (tid == 0) entries_s = rows_s = bad_s = join_s = 0;
+  if (tid == 0) entries_s = rows_s = bad_s = join_s = keys_s = 0;
   __syncthreads();
   const bool prefix_kind = p.prefix_len != nullptr;
   int prefix = 0, npre = 0, nt = 0;
@@ -528,12 +528,16 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
       prefix = 0;
       if (tid == 0) bad_s = kBadLength;
     }
+    int most = 0;
     for (int r = tid; r < R; r += kAttnPlanThreads) {
       const int n = p.seq_lens[r];
       const bool ok = n >= 0 && n <= kMaxKeys;
       if (!ok) atomicOr(&bad_s, kBadLength);
       lens[r] = ok ? n : 0;
+      if (ok && n > most) most = n;
     }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((tid & 31) == 0 && most) atomicMax(&keys_s, most);
     npre = (R + p.lay.tile_tok - 1) / p.lay.tile_tok;
     nt = npre + R;
   } else {
@@ -564,6 +568,8 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
     nt = (int)sum;
   }
   __syncthreads();
+  // (no request holds what lies behind the longest one: neither a page id nor finite values)
+  if (prefix > keys_s) prefix = keys_s;
   bool allow_few = true;
   auto tile_at = [&](int i) {
     if (prefix_kind) return prefix_tile(p, lens, prefix, npre, i);

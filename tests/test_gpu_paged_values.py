@@ -87,3 +87,25 @@ def test_attn_prompt_window_larger_than_any_request(cuda, D, nq, nkv, window):
     ref, mag = _attn_ref(b, nq, nkv, D, D ** -0.5)
     assert bool((out[:40] == 0).all()) and bool((out[40:140] != 0).any())
     _close(out, ref, mag)
+
+
+@pytest.mark.parametrize("D,nq,nkv", [(128, 8, 2), (256, 8, 2)])
+def test_attn_shared_prefix_longer_than_every_request(cuda, D, nq, nkv):
+    """A prefix length past all requests (a batch of padded slots in the extreme) reads no
+    position that none of them holds: no page id behind their ends is looked at, and what the last
+    page carries there does not matter."""
+    import torch
+    from spark_b200 import ops
+    b = _batch([89, 69, 0], [1, 1, 1], nq, nkv, D, 16, seed=63, shared=64)
+    prefix = torch.tensor([400], dtype=torch.int32, device="cuda")
+    b["table"][1:, :6] = b["table"][0, :6]  # (the longest request holds what all share)
+    for lens in ([90, 70, 0], [0, 0, 0]):
+        b["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        b["len"] = lens
+        plan = ops.AttnPlan(3, 3, nq, nkv, D).update_prefix(b["lens"], prefix)
+        out = torch.full_like(b["q"], float("nan"))
+        ops.attn_shared_prefix_out(b["q"], b["kc"], b["vc"], b["table"], plan, D ** -0.5, out, b["err"])
+        torch.cuda.synchronize()
+        assert int(b["err"]) == 0 and int(plan.error) == 0, lens
+        ref, mag = _attn_ref(b, nq, nkv, D, D ** -0.5)
+        _close(out, ref, mag)
