@@ -142,18 +142,19 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs p) {
   if (bad && blockIdx.x == 0 && tid == 0) atomicOr(p.error, bad);
   const int tokens = bad ? 0 : (int)t_sum, pages = bad ? 0 : (int)p_sum;
   const int gtid = blockIdx.x * kPlanThreads + tid, gthreads = gridDim.x * kPlanThreads;
-  for (int r = gtid; r <= R; r += gthreads) {
+  for (int r = gtid; r <= R; r += gthreads) {  // (R <= kPlanMaxReqs)
     p.query_start[r] = bad ? 0 : start[r];
     if (r < R) p.seq_lens[r] = bad ? 0 : ctx_s[r] + (start[r + 1] - start[r]);
   }
-  for (int i = gtid; i < pages; i += gthreads) {
+  // (unsigned: the step past 2^31 - 1 rows or pages is not one below zero)
+  for (uint32_t i = gtid; i < (uint32_t)pages; i += gthreads) {
     const int r = find_request(page0, R, i);
     const int first = (int)(((long long)ctx_s[r] + bs - 1) / bs);
     p.table[r * p.table_stride + first + (i - page0[r])] = p.free_ids[head + i];
   }
-  for (int i = gtid; i < p.rows; i += gthreads) {
+  for (uint32_t i = gtid; i < (uint32_t)p.rows; i += gthreads) {
     long long pos = 0, slot = -1;
-    if (i < tokens) {
+    if (i < (uint32_t)tokens) {
       const int r = find_request(start, R, i);
       const int c = ctx_s[r], at = c + (i - start[r]);  // (below seq_lens[r]: fits)
       const int pg = at / bs, first = (int)(((long long)c + bs - 1) / bs);
