@@ -301,6 +301,9 @@ ERR_WAIT, ERR_LENGTH, ERR_NO_PAGES, ERR_TABLE_WIDTH, ERR_NO_ROWS = 1, 4, 8, 16, 
 ERR_PAGE, ERR_POSITION, ERR_SLOT = 64, 128, 256
 
 
+# the C interface's sizes are 32-bit; ctypes drops what is above them without a word
+_INT_MAX = (1 << 31) - 1
+
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
@@ -373,6 +376,8 @@ def paged_plan_out(ctx_lens, new_lens, block_table, block_size, query_start, seq
         raise ValueError("positions and slot_mapping must have the same length")
     if counter.numel() < 1 or error.numel() < 1:
         raise ValueError("counter and error must hold one int32")
+    if rows > _INT_MAX or block_size > _INT_MAX or (free_blocks is not None and free_blocks.numel() > _INT_MAX):
+        raise ValueError("rows, block_size and free_blocks must be below 2^31")
     _block_table(block_table, R, dev)
     if (free_blocks is None) != (free_head is None) or (free_head_out is not None and free_head is None):
         raise ValueError("give free_blocks and free_head together (and free_head_out only with them)")
@@ -445,7 +450,8 @@ class AttnPlan:
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         _check(device.type == "cuda", "the plan lives on a CUDA device")
-        _check(window >= 0, "window must be positive, or 0 for none")
+        _check(0 <= window <= _INT_MAX, "window must be positive and below 2^31, or 0 for none")
+        _check(max(max_tokens, max_reqs, nq, nkv, head_dim) <= _INT_MAX, "sizes must be below 2^31")
         nbytes = lib().spark_attn_plan_bytes(max_tokens, max_reqs, nq, nkv, head_dim)
         _check(nbytes > 0, f"unsupported attention shape: {max_tokens} tokens, {max_reqs} requests, {nq} query / "
                            f"{nkv} kv heads of {head_dim}")
