@@ -232,8 +232,9 @@ int spark_slot_mapping(int64_t num_tokens, int64_t max_tokens, const int32_t* qu
  * `error` (int32 on the device, required) collects bits: 4 a length out of range or
  * descending starts, 8 the free list ran out, 16 a request longer than its block table
  * row, 32 more tokens than output rows, 64 a block table entry outside the cache, 128 a
- * position outside the rotation table, 256 a slot outside the cache; 1 and 2 as in
- * spark_q4_gemm_tc.  What does not fit is skipped, never dereferenced.
+ * position outside the rotation table, 256 a slot outside the cache, 512 a plan made for
+ * another shape or window (or not made at all: zeros); 1 and 2 as in spark_q4_gemm_tc.
+ * What does not fit is skipped, never dereferenced.
  * ====================================================================== */
 
 /* Block tables, token positions and slot maps from request lengths, in one launch.
@@ -294,8 +295,9 @@ int spark_attn_plan(const int32_t* query_start, const int32_t* seq_lens, const i
  * the keys its plan gives it, fp32 statistics; a token without keys is zero.  Rows of out
  * behind the last planned token are left alone.  K and V of positions at or past a
  * request's length may hold anything (NaN included).  head_dim 128 or 256, nq / nkv any
- * integer up to 128, scale > 0; strides in elements, multiples of 8; the maxima and window
- * are the plan's.  part_o fp32 [spark_attn_part_rows][nkv][head_dim] and part_ml fp32
+ * integer up to 128, scale > 0; strides in elements, multiples of 8.  The maxima, head
+ * layout and window must be the plan's (else bit 512 and nothing is written), and block_table
+ * has a row for each of its requests.  part_o fp32 [spark_attn_part_rows][nkv][head_dim] and part_ml fp32
  * [spark_attn_part_rows][nkv][2] are workspace: calls that may overlap need a plan and
  * workspace each.  wait_ns bounds each wait inside the kernel as in spark_q4_gemm_tc; bit
  * 1 of *error: a wait ran out and out is not valid.  Replaces vLLM's torch attention of

@@ -378,7 +378,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   const Header* hdr = reinterpret_cast<const Header*>(p.plan);
   const Item* items = reinterpret_cast<const Item*>(p.plan + p.lay.items);
-  const uint32_t nwork = (uint32_t)hdr->items * (uint32_t)p.nkv, room = (uint32_t)p.lay.max_items * (uint32_t)p.nkv;
+  const bool fits = plan_fits<D>(p, hdr);
+  if (!fits && blockIdx.x == 0 && tid == 0) atomicOr(p.error, kBadPlan);
+  const uint32_t nwork = fits ? (uint32_t)hdr->items * (uint32_t)p.nkv : 0;
   const int g = p.nq / p.nkv;
 
   if (warp >= kSoftmaxWarps) {
@@ -390,8 +392,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t rows_total = p.num_blocks * p.nkv * p.bs;
       for (uint32_t pass = 0; ok; pass++) {
         const uint32_t w = work_index(pass);
-        if (w >= room) break;
-        const Item it = items[w / p.nkv];  // (its load does not wait for the number of items)
+        if (pass && w >= nwork) break;
+        const Item it = items[w / p.nkv];  // (the first one's load does not wait for the header)
         if (w >= nwork) break;
         const int kvh = (int)(w % p.nkv);
         const int n = it.nkt;
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t w = work_index(pass);
           Item it;
           int kvh = 0;
-          if (w < room) {
+          if (!pass || w < nwork) {
             it = items[w / p.nkv];
             kvh = (int)(w % p.nkv);
           }

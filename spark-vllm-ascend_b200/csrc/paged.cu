@@ -28,7 +28,7 @@ static int attn_launch(const paged::AttnArgs& p, int64_t wait_ns, cudaStream_t s
       !encode_map(&mk, bf, p.k_cache, D, rows, D * 2, 64, (uint32_t)t.piece, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !encode_map(&mv, bf, p.v_cache, D, rows, D * 2, 64, (uint32_t)t.piece, CU_TENSOR_MAP_SWIZZLE_128B))
     return SPARK_ERR_LAUNCH;
-  const int grid = (int)std::min<int64_t>((int64_t)p.lay.max_items * p.nkv, num_sms());
+  const int grid = (int)std::min<int64_t>((int64_t)p.lay.max_items * p.nkv, std::min(num_sms(), kNumSMs));
   const int st = launch(paged::tc::attn_kernel<D>, dim3(grid), dim3(paged::tc::kThreads), paged::tc::kSmemBytes,
                         stream, mq, mk, mv, t);
   if (st) return st;
@@ -137,7 +137,7 @@ int spark_attn_plan(const int32_t* query_start, const int32_t* seq_lens, const i
   paged::AttnPlanArgs p;
   memset(&p, 0, sizeof(p));
   p.query_start = query_start, p.seq_lens = seq_lens, p.prefix_len = prefix_len;
-  p.reqs = reqs, p.tokens = max_tokens, p.nq = nq, p.nkv = nkv, p.D = head_dim, p.window = window;
+  p.reqs = reqs, p.tokens = max_tokens, p.max_reqs = max_reqs, p.nq = nq, p.nkv = nkv, p.D = head_dim, p.window = window;
   p.lay = paged::layout_of(max_tokens, max_reqs, nq, nkv, head_dim);
   p.plan = static_cast<unsigned char*>(plan), p.error = error;
   return launch(paged::attn_plan_kernel, dim3(1), dim3(paged::kAttnPlanThreads), 0, as_stream(stream), p);
@@ -173,6 +173,7 @@ int spark_attn_paged(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_str
   p.q = q, p.k_cache = k_cache, p.v_cache = v_cache, p.table = block_table, p.table_stride = table_stride;
   p.q_tok = q_tok_stride, p.q_head = q_head_stride, p.o_tok = out_tok_stride, p.o_head = out_head_stride;
   p.num_blocks = num_blocks, p.table_width = table_width, p.bs = block_size, p.tokens = tokens;
+  p.max_tokens = max_tokens, p.max_reqs = max_reqs;
   p.nq = nq, p.nkv = nkv, p.window = window, p.scale = scale;
   p.plan = static_cast<const unsigned char*>(plan);
   p.lay = paged::layout_of(max_tokens, max_reqs, nq, nkv, head_dim);

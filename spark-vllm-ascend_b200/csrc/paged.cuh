@@ -19,6 +19,7 @@ constexpr int kNoRows = 32;      // more tokens than output rows
 constexpr int kBadPage = 64;     // a block table entry outside the cache
 constexpr int kBadPosition = 128;  // a position outside the rotation table
 constexpr int kBadSlot = 256;    // a slot outside the cache
+constexpr int kBadPlan = 512;    // a plan made for another shape or window, or none
 
 // ------------------------------------------------------------------ block tables and slot maps
 // Requests r = 0 .. R-1 with ctx[r] cached and nw[r] new tokens:
@@ -364,7 +365,6 @@ __global__ void __launch_bounds__(kRopeMaxThreads, 10) rope_store_kernel(RopeArg
 // long against the even share of all work is cut into parts, whose unnormalised sums go to
 // the partial buffers and are joined by combine_kernel.
 constexpr int kKeyTile = 128;
-constexpr int kPromptPlan = 1, kPrefixPlan = 2;
 
 struct alignas(16) Item {
   int tok0, ntok;   // query tokens
@@ -385,11 +385,19 @@ struct alignas(16) Entry {  // rows to join: tokens tok0 .. tok0 + ntok - 1, par
   int tok0, ntok, base_a, n_a, stride_a, base_b, n_b, stride_b;
 };
 
-struct Header {
-  int items, entries, kind, part_rows, reqs, tokens, window;
-  int join_rows;  // rows of the largest entry
-  int pad[8];
+// What the plan was made for stands in its header: the attention compares it with its own
+// arguments, since every offset and partial row below follows from them.
+struct Shape {
+  int max_tokens, max_reqs, nq, nkv, head_dim, window;
 };
+struct alignas(16) Header {
+  int items, entries;
+  int join_rows;  // rows of the largest entry
+  int pad0;
+  Shape shape;
+  int pad1[6];
+};
+static_assert(sizeof(Header) == 64, "items start at a multiple of 16 bytes");
 
 struct Layout {
   int tile_tok, half_tok, max_tiles, max_items, max_entries, budget, part_rows;
@@ -423,13 +431,15 @@ __host__ __device__ inline Layout layout_of(int T, int R, int nq, int nkv, int D
   l.tiles = take((int64_t)l.max_tiles * sizeof(int2));
   l.bases = take((int64_t)l.max_tiles * sizeof(int2));
   l.lens = take(((int64_t)R + 1) * sizeof(int));
-  l.bytes = at;
+  // (one item per CTA is read before the header is known to match: any plan has room for them)
+  const int64_t least = sizeof(Header) + (int64_t)kNumSMs * sizeof(Item);
+  l.bytes = at > least ? at : least;
   return l;
 }
 
 struct AttnPlanArgs {
   const int32_t *query_start, *seq_lens, *prefix_len;  // prefix_len: the shared-prefix plan
-  int reqs, tokens, nq, nkv, D, window;
+  int reqs, tokens, max_reqs, nq, nkv, D, window;
   Layout lay;
   unsigned char* plan;
   int* error;
@@ -760,12 +770,8 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(AttnPlanArg
   }
   if (tid == 0) {
     hdr->entries = prefix_kind ? R : entries_s;
-    hdr->kind = prefix_kind ? kPrefixPlan : kPromptPlan;
-    hdr->part_rows = rows_s;
     hdr->join_rows = prefix_kind ? p.nq / p.nkv : join_s;
-    hdr->reqs = R;
-    hdr->tokens = p.tokens;
-    hdr->window = p.window;
+    hdr->shape = {p.tokens, p.max_reqs, p.nq, p.nkv, p.D, p.window};
     if (bad_s) atomicOr(p.error, bad_s);
   }
 }
@@ -776,7 +782,7 @@ struct AttnArgs {
   int64_t q_tok, q_head, o_tok, o_head;  // strides in elements
   const int32_t* table;
   int64_t table_stride, num_blocks;
-  int table_width, bs, tokens, nq, nkv, window;
+  int table_width, bs, tokens, max_tokens, max_reqs, nq, nkv, window;
   float scale;
   const unsigned char* plan;
   Layout lay;
@@ -785,6 +791,14 @@ struct AttnArgs {
   uint16_t* out;
   int* error;
 };
+
+// the plan is one of this call's shape and window
+template <int D>
+__device__ __forceinline__ bool plan_fits(const AttnArgs& p, const Header* hdr) {
+  const Shape s = hdr->shape;
+  return s.max_tokens == p.max_tokens && s.max_reqs == p.max_reqs && s.nq == p.nq && s.nkv == p.nkv &&
+         s.head_dim == D && s.window == p.window;
+}
 
 // keys row (token i of the item) may see, within the item's part
 __device__ __forceinline__ int2 row_keys(const Item& it, const int* lens, int window, int i) {
@@ -814,7 +828,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(AttnArgs p) {
   const Header* hdr = reinterpret_cast<const Header*>(p.plan);
   const Entry* entries = reinterpret_cast<const Entry*>(p.plan + p.lay.entries);
   const int g = p.nq / p.nkv, lane = threadIdx.x & 31;
-  const int n = hdr->entries, jr = hdr->join_rows;
+  const int n = plan_fits<D>(p, hdr) ? hdr->entries : 0, jr = hdr->join_rows;
   // (entries x kv heads x rows: below 2^31, checked on the host)
   const uint32_t total = (uint32_t)n * p.nkv * jr, step = gridDim.x * (kJoinThreads / 32);
   for (uint32_t w = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5); w < total; w += step) {

@@ -298,7 +298,7 @@ def kv_store_(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
 # ---------------------------------------------------------------- batches over the paged cache
 # error-word bits of these operators (include/spark_b200.h)
 ERR_WAIT, ERR_LENGTH, ERR_NO_PAGES, ERR_TABLE_WIDTH, ERR_NO_ROWS = 1, 4, 8, 16, 32
-ERR_PAGE, ERR_POSITION, ERR_SLOT = 64, 128, 256
+ERR_PAGE, ERR_POSITION, ERR_SLOT, ERR_PLAN = 64, 128, 256, 512
 
 
 # the C interface's sizes are 32-bit; ctypes drops what is above them without a word

@@ -4,6 +4,8 @@ from __future__ import annotations
 
 import pytest
 
+from test_gpu_paged import _attn_ref, _batch, _close
+
 pytestmark = pytest.mark.gpu
 
 
@@ -29,3 +31,41 @@ def test_paged_plan_of_the_most_rows(cuda):
             assert bool((part == want).all())
     del both, pos, slots
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("D,nq,nkv", [(128, 8, 2), (256, 8, 2)])
+def test_attn_refuses_a_plan_of_another_shape(cuda, D, nq, nkv):
+    """The C entry point given a plan made for other maxima, another head layout or window, or
+    none: reported, nothing written; with the plan's own it is right."""
+    import torch
+    from spark_b200 import ops
+    from spark_b200._lib import call
+    b = _batch([100, 0], [20, 30], nq, nkv, D, 16, seed=70)
+    plan = ops.AttnPlan(64, 4, nq, nkv, D, window=40).update(b["start"], b["lens"])
+    out = torch.full_like(b["q"], 3.0)
+
+    def run(buf, **change):
+        a = {**dict(tokens=64, reqs=4, nq=nq, nkv=nkv, window=40), **change}
+        b["err"].zero_()
+        call("spark_attn_paged", b["q"].data_ptr(), nq * D, D, 50, b["kc"].data_ptr(), b["vc"].data_ptr(),
+             b["kc"].shape[0], 16, b["table"].data_ptr(), b["table"].stride(0), b["table"].shape[1], a["tokens"],
+             a["reqs"], a["nq"], a["nkv"], D, a["window"], D ** -0.5, buf.data_ptr(), plan.part_o.data_ptr(),
+             plan.part_ml.data_ptr(), out.data_ptr(), nq * D, D, b["err"].data_ptr(), -1,
+             torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        return int(b["err"])
+
+    for change in (dict(tokens=63), dict(reqs=3), dict(nq=4), dict(nkv=1), dict(window=0), dict(window=41)):
+        assert run(plan.buf, **change) == ops.ERR_PLAN, change
+        assert bool((out == 3.0).all())
+    assert run(torch.zeros_like(plan.buf)) == ops.ERR_PLAN and bool((out == 3.0).all())
+    assert run(plan.buf) == 0
+    ref, mag = _attn_ref(b, nq, nkv, D, D ** -0.5, 40)
+    _close(out, ref, mag)
+
+
+def test_attn_plans_have_room_for_an_item_per_block():
+    """(each block reads its first item before it knows that the plan is one of its shape)"""
+    from spark_b200._lib import lib
+    for shape in ((1, 1, 4096, 4096, 128), (1, 1, 8, 1, 128), (1, 1, 592, 592, 256)):
+        assert lib().spark_attn_plan_bytes(*shape) >= 64 + 148 * 48
