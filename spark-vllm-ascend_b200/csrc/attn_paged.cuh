@@ -265,9 +265,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // p = 2^(s c + neg) of 16 scores: sums in fp32, the bf16 pairs to tensor memory.  Every
 // exponential is the special-function unit's (a relative error of 2^-22, a NaN stays one, an
-// infinite difference is 0 or infinite).  A quarter of them by a clamped cubic instead took 1.5%
-// off packed prompts and 3% off a long shared prefix (184 -> 181.5, 91.3 -> 88.3 us), but the row
-// sums then had its 7.5e-5 and a NaN score became a small weight.
+// infinite difference is 0 or infinite).
 __device__ __forceinline__ void probs16(const float* s, u64 c2, u64 neg2, u64 (&sum)[2], uint32_t addr) {
   uint32_t pk[8];
 #pragma unroll
@@ -902,7 +900,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float neg = m == -INFINITY ? 0.0f : -m * c;
           const u64 neg2 = pack2(neg, neg), c2 = pack2(c, c);
           u64 sum[2] = {0, 0};
-#pragma unroll
+          // (not unrolled: both halves' probabilities side by side spill 28 bytes; packed prompts 184.6
+          // -> 182.6, long shared prefix 90.4 -> 88.2, 8 x 2048 prefix 15.3 -> 14.9 us)
+#pragma unroll 1
           for (int q = 0; q < NQ; q++) {
             if (q > 0) load(q);
             const uint32_t pb = sb + 64 * q + 32 * sp;
