@@ -297,7 +297,7 @@ int spark_attn_plan(const int32_t* query_start, const int32_t* seq_lens, const i
  * request's length may hold anything (NaN included).  head_dim 128 or 256, nq / nkv any
  * integer up to 128, scale > 0; strides in elements, multiples of 8.  The maxima, head
  * layout and window must be the plan's (else bit 512 and nothing is written), and block_table
- * has a row for each of its requests.  part_o fp32 [spark_attn_part_rows][nkv][head_dim] and part_ml fp32
+ * has a row for each of its requests (spark_attn_paged_bounded checks that on the device).  part_o fp32 [spark_attn_part_rows][nkv][head_dim] and part_ml fp32
  * [spark_attn_part_rows][nkv][2] are workspace: calls that may overlap need a plan and
  * workspace each.  wait_ns bounds each wait inside the kernel as in spark_q4_gemm_tc; bit
  * 1 of *error: a wait ran out and out is not valid.  Replaces vLLM's torch attention of
@@ -308,6 +308,16 @@ int spark_attn_paged(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_str
                      int nq, int nkv, int head_dim, int window, float scale, const void* plan, float* part_o,
                      float* part_ml, uint16_t* out, int64_t out_tok_stride, int64_t out_head_stride, int* error,
                      int64_t wait_ns, void* stream);
+
+/* As spark_attn_paged, for a block table of table_rows rows: a request of the plan past them is
+ * reported (bit 64) and its keys count as zeros.  For calls whose plan is made elsewhere, such as
+ * a captured call whose work list is updated between replays. */
+int spark_attn_paged_bounded(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int tokens,
+                             const uint16_t* k_cache, const uint16_t* v_cache, int64_t num_blocks, int block_size,
+                             const int32_t* block_table, int64_t table_stride, int table_width, int table_rows,
+                             int max_tokens, int max_reqs, int nq, int nkv, int head_dim, int window, float scale,
+                             const void* plan, float* part_o, float* part_ml, uint16_t* out, int64_t out_tok_stride,
+                             int64_t out_head_stride, int* error, int64_t wait_ns, void* stream);
 
 /* Enable / disable programmatic dependent launch on the kernels above (default on). */
 int spark_set_pdl(int enabled);

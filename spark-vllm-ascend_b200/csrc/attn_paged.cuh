@@ -403,7 +403,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int key = it.key0 + x * pr;
           if (x >= n * pp || key >= it.len || key + pr <= it.klo) return -1;
           const int pg = key / p.bs;
-          const int id = pg < p.table_width ? __ldg(p.table + it.req * p.table_stride + pg) : -1;
+          const int id =
+              pg < p.table_width && it.req < p.table_rows ? __ldg(p.table + it.req * p.table_stride + pg) : -1;
           if (id < 0 || id >= p.num_blocks) {
             atomicOr(p.error, kBadPage);
             return (int)rows_total;  // outside the map: zeros

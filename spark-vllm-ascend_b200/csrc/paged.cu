@@ -143,17 +143,17 @@ int spark_attn_plan(const int32_t* query_start, const int32_t* seq_lens, const i
   return launch(paged::attn_plan_kernel, dim3(1), dim3(paged::kAttnPlanThreads), 0, as_stream(stream), p);
 }
 
-int spark_attn_paged(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int tokens,
-                     const uint16_t* k_cache, const uint16_t* v_cache, int64_t num_blocks, int block_size,
-                     const int32_t* block_table, int64_t table_stride, int table_width, int max_tokens, int max_reqs,
-                     int nq, int nkv, int head_dim, int window, float scale, const void* plan, float* part_o,
-                     float* part_ml, uint16_t* out, int64_t out_tok_stride, int64_t out_head_stride, int* error,
-                     int64_t wait_ns, void* stream) {
+int spark_attn_paged_bounded(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int tokens,
+                             const uint16_t* k_cache, const uint16_t* v_cache, int64_t num_blocks, int block_size,
+                             const int32_t* block_table, int64_t table_stride, int table_width, int table_rows,
+                             int max_tokens, int max_reqs, int nq, int nkv, int head_dim, int window, float scale,
+                             const void* plan, float* part_o, float* part_ml, uint16_t* out, int64_t out_tok_stride,
+                             int64_t out_head_stride, int* error, int64_t wait_ns, void* stream) {
   if (!k_cache || !v_cache || !block_table || !plan || !part_o || !part_ml || !error) return SPARK_ERR_INVALID_ARG;
   int st = check_attn_shape(max_tokens, max_reqs, nq, nkv, head_dim);
   if (st) return st;
   if (tokens < 0 || tokens > max_tokens || num_blocks <= 0 || block_size < 16 || block_size % 16 ||
-      table_width <= 0 || table_stride < 0 || window < 0 || !(scale > 0.0f) || scale > 1e30f)
+      table_width <= 0 || table_rows <= 0 || table_stride < 0 || window < 0 || !(scale > 0.0f) || scale > 1e30f)
     return SPARK_ERR_UNSUPPORTED_SHAPE;
   if (tokens == 0) return SPARK_OK;
   if (!q || !out) return SPARK_ERR_INVALID_ARG;
@@ -172,7 +172,7 @@ int spark_attn_paged(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_str
   memset(&p, 0, sizeof(p));
   p.q = q, p.k_cache = k_cache, p.v_cache = v_cache, p.table = block_table, p.table_stride = table_stride;
   p.q_tok = q_tok_stride, p.q_head = q_head_stride, p.o_tok = out_tok_stride, p.o_head = out_head_stride;
-  p.num_blocks = num_blocks, p.table_width = table_width, p.bs = block_size, p.tokens = tokens;
+  p.num_blocks = num_blocks, p.table_width = table_width, p.table_rows = table_rows, p.bs = block_size, p.tokens = tokens;
   p.max_tokens = max_tokens, p.max_reqs = max_reqs;
   p.nq = nq, p.nkv = nkv, p.window = window, p.scale = scale;
   p.plan = static_cast<const unsigned char*>(plan);
@@ -180,6 +180,18 @@ int spark_attn_paged(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_str
   p.part_o = part_o, p.part_ml = reinterpret_cast<float2*>(part_ml), p.out = out, p.error = error;
   if (head_dim == 128) return attn_launch<128>(p, wait_ns, as_stream(stream));
   return attn_launch<256>(p, wait_ns, as_stream(stream));
+}
+
+int spark_attn_paged(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, int tokens,
+                     const uint16_t* k_cache, const uint16_t* v_cache, int64_t num_blocks, int block_size,
+                     const int32_t* block_table, int64_t table_stride, int table_width, int max_tokens, int max_reqs,
+                     int nq, int nkv, int head_dim, int window, float scale, const void* plan, float* part_o,
+                     float* part_ml, uint16_t* out, int64_t out_tok_stride, int64_t out_head_stride, int* error,
+                     int64_t wait_ns, void* stream) {
+  return spark_attn_paged_bounded(q, q_tok_stride, q_head_stride, tokens, k_cache, v_cache, num_blocks, block_size,
+                                  block_table, table_stride, table_width, max_reqs, max_tokens, max_reqs, nq, nkv,
+                                  head_dim, window, scale, plan, part_o, part_ml, out, out_tok_stride,
+                                  out_head_stride, error, wait_ns, stream);
 }
 
 }  // extern "C"

@@ -782,7 +782,7 @@ struct AttnArgs {
   int64_t q_tok, q_head, o_tok, o_head;  // strides in elements
   const int32_t* table;
   int64_t table_stride, num_blocks;
-  int table_width, bs, tokens, max_tokens, max_reqs, nq, nkv, window;
+  int table_width, table_rows, bs, tokens, max_tokens, max_reqs, nq, nkv, window;
   float scale;
   const unsigned char* plan;
   Layout lay;

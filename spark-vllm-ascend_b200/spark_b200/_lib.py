@@ -53,6 +53,8 @@ SIGNATURES: dict[str, list] = {
     "spark_attn_plan": [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P],
     "spark_attn_paged": [_P, _I64, _I64, _I, _P, _P, _I64, _I, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P,
                          _P, _I64, _I64, _P, _I64, _P],
+    "spark_attn_paged_bounded": [_P, _I64, _I64, _I, _P, _P, _I64, _I, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _I, _F,
+                                 _P, _P, _P, _P, _I64, _I64, _P, _I64, _P],
     "spark_t16_bytes": [_I, _I, _I],
     "spark_q4_pack_t16": [_P, _P, _I, _I, _I, _I, _I, _P, _P],
     "spark_step_ring_bytes": [],

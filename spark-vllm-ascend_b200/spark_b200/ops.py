@@ -522,9 +522,9 @@ def _attn_paged(kind, q, k_cache, v_cache, block_table, plan, scale, out, error,
         raise ValueError("error must hold one int32")
     qt, qh, _ = q.stride()
     ot, oh, _ = out.stride()
-    _launch(dev, "spark_attn_paged", q.data_ptr(), qt, qh, tokens, k_cache.data_ptr(), v_cache.data_ptr(), ks[0],
-            ks[2], block_table.data_ptr(), block_table.stride(0), block_table.shape[1], plan.max_tokens,
-            plan.max_reqs, nq, nkv, D, plan.window, scale, plan.buf.data_ptr(), plan.part_o.data_ptr(),
+    _launch(dev, "spark_attn_paged_bounded", q.data_ptr(), qt, qh, tokens, k_cache.data_ptr(), v_cache.data_ptr(),
+            ks[0], ks[2], block_table.data_ptr(), block_table.stride(0), block_table.shape[1], block_table.shape[0],
+            plan.max_tokens, plan.max_reqs, nq, nkv, D, plan.window, scale, plan.buf.data_ptr(), plan.part_o.data_ptr(),
             plan.part_ml.data_ptr(), out.data_ptr(), ot, oh, error.data_ptr(), wait_ns)
     return out
 

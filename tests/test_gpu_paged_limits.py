@@ -69,3 +69,34 @@ def test_attn_plans_have_room_for_an_item_per_block():
     from spark_b200._lib import lib
     for shape in ((1, 1, 4096, 4096, 128), (1, 1, 8, 1, 128), (1, 1, 592, 592, 256)):
         assert lib().spark_attn_plan_bytes(*shape) >= 64 + 148 * 48
+
+
+@pytest.mark.parametrize("D,nq,nkv", [(128, 8, 2), (256, 8, 2)])
+def test_attn_captured_with_fewer_table_rows_than_a_later_plan(cuda, D, nq, nkv):
+    """Only the attention is captured, with a table of two rows; the plan is then made for four
+    requests.  What lies behind the table is not read (here: the ids of other pages), the
+    requests that it holds are right, the rest is reported."""
+    import torch
+    from spark_b200 import ops
+    b = _batch([100, 0, 40, 300], [20, 30, 1, 1], nq, nkv, D, 16, seed=71)
+    plan = ops.AttnPlan(52, 4, nq, nkv, D).update(b["start"][:3], b["lens"][:2])
+    out = torch.zeros_like(b["q"])
+    run = lambda table: ops.attn_prompt_out(b["q"], b["kc"], b["vc"], table, plan, D ** -0.5, out, b["err"])  # noqa: E731
+    run(b["table"][:2])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(b["table"][:2])
+    plan.update(b["start"], b["lens"])
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert int(b["err"]) == ops.ERR_PAGE
+    ref, mag = _attn_ref(b, nq, nkv, D, D ** -0.5)
+    _close(out[:50], ref[:50], mag[:50])
+    assert bool((out[50:] == 0).all())  # (V of a page that is not there: zeros)
+    b["err"].zero_()
+    run(b["table"])  # the whole table: all right
+    torch.cuda.synchronize()
+    assert int(b["err"]) == 0
+    _close(out, ref, mag)

@@ -33,3 +33,14 @@ def test_paged_plan_refuses_sizes_past_32_bits(monkeypatch, what):
     with pytest.raises(ValueError, match="below 2\\^31"):
         ops.paged_plan_out(z(2), z(2), z((2, 4)), (1 << 32) + 16 if what == "block_size" else 16, z(3), z(2),
                            z(rows, torch.int64), z(rows, torch.int64), z(1), z(1), free_blocks=free, free_head=z(1))
+
+
+def test_attn_paged_bounded_refuses_a_table_without_rows():
+    import ctypes
+    import spark_b200
+    from spark_b200 import _lib
+    spark_b200.ensure_built()
+    at, scale = ctypes.c_void_p(0x1000), ctypes.c_float(0.1)  # (never dereferenced)
+    for rows in (0, -1):
+        assert _lib.lib().spark_attn_paged_bounded(at, 1024, 128, 10, at, at, 4, 16, at, 8, 8, rows, 64, 4, 8, 2, 128, 0,
+                                                   scale, at, at, at, at, 1024, 128, at, -1, None) == 2
