@@ -249,7 +249,8 @@ int spark_slot_mapping(int64_t num_tokens, int64_t max_tokens, const int32_t* qu
  * already, nothing is taken.  A batch that does not fit (bits 4, 8, 16, 32) comes out
  * empty -- all starts and lengths 0, all slots -1 -- and takes no page.  counter: int32,
  * zero before the first call, left zero; calls that may overlap need one each.
- * reqs <= 8192.  query_start and seq_lens must not be the inputs. */
+ * reqs <= 8192.  No output may overlap an input or another output (SPARK_ERR_INVALID_ARG),
+ * but for the head. */
 int spark_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int reqs, const int32_t* free_blocks,
                      int num_free, const int32_t* free_head, int32_t* free_head_out, int32_t* block_table,
                      int64_t table_stride, int table_width, int block_size, int rows, int32_t* query_start,
@@ -265,7 +266,8 @@ int spark_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int reqs,
  * in fp32 with one rounding to bf16 at the end.  q -> q_out bf16 [rows][nq][head_dim]; k
  * and v -> the caches at slot_mapping[r] (negative: padding, not stored).  A row whose
  * position is outside the table writes no q and no k (bit 128).  head_dim 128 or 256,
- * rotary_dim % 16 == 0; row_stride % 8 == 0, 16-byte aligned tensors.  Replaces the
+ * rotary_dim % 16 == 0; row_stride % 8 == 0, 16-byte aligned tensors that do not overlap
+ * (one row alone may have q_out == qkv).  Replaces the
  * rotation and store of FusedQkvStage (kernels/qkv.py:179-198) for many rows. */
 int spark_qk_norm_rope_store_rows(const uint16_t* qkv, int64_t row_stride, int rows, int nq, int nkv, int head_dim,
                                   const uint16_t* q_gamma, const uint16_t* k_gamma, float eps,

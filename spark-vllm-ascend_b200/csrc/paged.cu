@@ -11,6 +11,22 @@
 
 using namespace spark;
 
+// bytes [at, at + n) of a tensor; an absent one overlaps nothing
+struct Span {
+  const void* at;
+  int64_t n;
+};
+static bool overlap(const Span& a, const Span& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.at && b.at && a.n > 0 && b.n > 0 && x < y + (uintptr_t)b.n && y < x + (uintptr_t)a.n;
+}
+// a span and `rows` rows of `width` bytes, `pitch` apart: what lies between the rows is free
+static bool overlap(const Span& a, const void* base, int64_t rows, int64_t pitch, int64_t width) {
+  if (!overlap(a, Span{base, (rows - 1) * pitch + width})) return false;
+  const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(a.at) - reinterpret_cast<uintptr_t>(base));
+  return d < 0 || d % pitch < width || d % pitch + a.n > pitch;
+}
+
 template <int D>
 static int attn_launch(const paged::AttnArgs& p, int64_t wait_ns, cudaStream_t stream) {
   const int g = p.nq / p.nkv;
@@ -53,9 +69,23 @@ int spark_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int reqs,
   if (reqs <= 0 || rows < 0 || num_free < 0 || block_size <= 0 || table_width <= 0 || table_stride < table_width)
     return SPARK_ERR_UNSUPPORTED_SHAPE;
   if (reqs > paged::kPlanMaxReqs) return SPARK_ERR_TOO_LARGE;
-  // every CTA reads all lengths, while others write already
-  if (seq_lens == ctx_lens || seq_lens == new_lens || query_start == ctx_lens || query_start == new_lens)
-    return SPARK_ERR_INVALID_ARG;
+  // every CTA reads all lengths and the free list, while others write already (the head may be
+  // advanced in place: it is written when all have read it)
+  const int64_t tokens = 8 * (int64_t)rows;
+  const Span in[] = {{ctx_lens, 4 * (int64_t)reqs}, {new_lens, 4 * (int64_t)reqs}, {free_blocks, 4 * (int64_t)num_free},
+                     {free_head == free_head_out ? nullptr : free_head, 4}};
+  const Span out[] = {{query_start, 4 * ((int64_t)reqs + 1)}, {seq_lens, 4 * (int64_t)reqs}, {positions, tokens},
+                      {slot_mapping, tokens}, {free_head_out, 4}, {counter, 4}, {error, 4}};
+  auto on_table = [&](const Span& t) { return overlap(t, block_table, reqs, 4 * table_stride, 4 * table_width); };
+  for (const Span& i : in)
+    if (on_table(i)) return SPARK_ERR_INVALID_ARG;
+  for (const Span& o : out) {
+    if (on_table(o)) return SPARK_ERR_INVALID_ARG;
+    for (const Span& i : in)
+      if (overlap(o, i)) return SPARK_ERR_INVALID_ARG;
+    for (const Span& other : out)
+      if (&other != &o && overlap(o, other)) return SPARK_ERR_INVALID_ARG;
+  }
   paged::PlanArgs p;
   memset(&p, 0, sizeof(p));
   p.ctx = ctx_lens, p.nw = new_lens, p.free_ids = free_blocks, p.free_head = free_head;
@@ -85,6 +115,13 @@ int spark_qk_norm_rope_store_rows(const uint16_t* qkv, int64_t row_stride, int r
   if (row_stride % 8 || !aligned(qkv, 16) || !aligned(cos_sin, 16) || !aligned(k_cache, 16) ||
       !aligned(v_cache, 16) || !aligned(q_out, 16) || (q_gamma && (!aligned(q_gamma, 16) || !aligned(k_gamma, 16))))
     return SPARK_ERR_ALIGNMENT;
+  // rows are read and written in any order (a single one may be rotated in place)
+  const int64_t cache = num_blocks * nkv * block_size * (int64_t)head_dim * 2;
+  const Span x{qkv, ((rows - 1) * row_stride + (int64_t)(nq + 2 * nkv) * head_dim) * 2},
+      y{q_out, (int64_t)rows * nq * head_dim * 2}, k{k_cache, cache}, v{v_cache, cache};
+  if ((overlap(x, y) && !(rows == 1 && q_out == qkv)) || overlap(x, k) || overlap(x, v) || overlap(y, k) ||
+      overlap(y, v) || overlap(k, v))
+    return SPARK_ERR_INVALID_ARG;
   paged::RopeArgs p;
   memset(&p, 0, sizeof(p));
   p.qkv = qkv, p.qg = q_gamma, p.kg = k_gamma, p.cos_sin = cos_sin, p.positions = positions, p.slots = slot_mapping;

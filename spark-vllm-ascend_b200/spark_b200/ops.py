@@ -376,7 +376,8 @@ def paged_plan_out(ctx_lens, new_lens, block_table, block_size, query_start, seq
         raise ValueError("positions and slot_mapping must have the same length")
     if counter.numel() < 1 or error.numel() < 1:
         raise ValueError("counter and error must hold one int32")
-    if rows > _INT_MAX or block_size > _INT_MAX or (free_blocks is not None and free_blocks.numel() > _INT_MAX):
+    num_free = 0 if free_blocks is None else free_blocks.numel()
+    if rows > _INT_MAX or block_size > _INT_MAX or num_free > _INT_MAX:
         raise ValueError("rows, block_size and free_blocks must be below 2^31")
     _block_table(block_table, R, dev)
     if (free_blocks is None) != (free_head is None) or (free_head_out is not None and free_head is None):
@@ -388,7 +389,7 @@ def paged_plan_out(ctx_lens, new_lens, block_table, block_size, query_start, seq
             raise ValueError("free_head must hold one int32")
     width = block_table.shape[1]
     _launch(dev, "spark_paged_plan", ctx_lens.data_ptr(), new_lens.data_ptr(), R, _ptr(free_blocks),
-            0 if free_blocks is None else free_blocks.numel(), _ptr(free_head), _ptr(free_head_out),
+            num_free, _ptr(free_head), _ptr(free_head_out),
             block_table.data_ptr(), block_table.stride(0) if R > 1 else width, width, int(block_size), rows,
             query_start.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(),
             counter.data_ptr(), error.data_ptr())

@@ -100,3 +100,24 @@ def test_attn_captured_with_fewer_table_rows_than_a_later_plan(cuda, D, nq, nkv)
     torch.cuda.synchronize()
     assert int(b["err"]) == 0
     _close(out, ref, mag)
+
+
+def test_paged_plan_outputs_between_the_table_rows(cuda):
+    """What does not overlap is taken: one int32 buffer holds the table's rows and, between them,
+    the counter and the status word; the head next to the lengths."""
+    import torch
+    from spark_b200 import ops
+    i32 = {"dtype": torch.int32, "device": "cuda"}
+    buf = torch.zeros((3, 8), **i32)
+    buf[:, :6] = -1
+    ints = torch.zeros(16, **i32)
+    ctx, new, head, start, lens = ints[0:3], ints[3:6], ints[6:7], ints[7:11], ints[11:14]
+    new.copy_(torch.tensor([20, 1, 3]))
+    both = torch.zeros(2 * 26, dtype=torch.int64, device="cuda")
+    pos, slots = both[:26], both[26:]
+    ops.paged_plan_out(ctx, new, buf[:, :6], 16, start, lens, pos, slots, buf[0, 6:7], buf[1, 7:8],
+                       free_blocks=torch.arange(5, 15, **i32), free_head=head)
+    torch.cuda.synchronize()
+    assert buf.tolist() == [[5, 6, -1, -1, -1, -1, 0, 0], [7, -1, -1, -1, -1, -1, 0, 0], [8, -1, -1, -1, -1, -1, 0, 0]]
+    assert int(head) == 4 and start.tolist() == [0, 20, 21, 24] and lens.tolist() == [20, 1, 3]
+    assert slots.tolist() == [*range(80, 100), 112, 128, 129, 130, -1, -1]
