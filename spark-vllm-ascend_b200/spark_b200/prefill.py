@@ -117,6 +117,13 @@ def _head_logits(eng, x: torch.Tensor) -> torch.Tensor:
     return logits
 
 
+def _check_ids(ids: torch.Tensor, cfg) -> None:
+    """Refuse token ids (on the host) that are no row of the embedding: looked up on the device,
+    one would end the process's CUDA context."""
+    if ids.numel() and not (0 <= int(ids.min()) and int(ids.max()) < cfg.vocab_size):
+        raise ValueError(f"token ids from {int(ids.min())} to {int(ids.max())}, vocabulary of {cfg.vocab_size}")
+
+
 def _gather(cache: torch.Tensor, table: torch.Tensor, n: int, bs: int) -> torch.Tensor:
     """Positions [0, n) of one layer's paged cache [blocks, nkv, bs, D] -> [nkv, n, D]."""
     pos = torch.arange(n, device=cache.device)
@@ -133,7 +140,10 @@ def prefill(eng, prompt: torch.Tensor, chunk: int = 2048, gemm: str = "q4", attn
         raise ValueError(f"attn must be 'sdpa' or 'paged', not {attn!r}")
     cfg, w = eng.cfg, eng.w
     dev = eng.device
-    prompt = torch.as_tensor(prompt, dtype=torch.int64).to(dev)
+    prompt = torch.as_tensor(prompt, dtype=torch.int64)
+    if not prompt.is_cuda:
+        _check_ids(prompt, cfg)
+    prompt = prompt.to(dev)
     P = prompt.numel()
     if P == 0 or P > eng.max_seq_len:
         raise ValueError(f"prompt of {P} tokens (max_seq_len {eng.max_seq_len})")
@@ -235,6 +245,8 @@ def prefill_packed(eng, prompts, block_tables: torch.Tensor, chunk: int = 8192, 
     R, lens = len(prompts), [p.numel() for p in prompts]
     if R == 0 or min(lens) == 0 or max(lens) > eng.max_seq_len:
         raise ValueError(f"prompts of {lens} tokens (1 to max_seq_len {eng.max_seq_len} each)")
+    for p in prompts:
+        _check_ids(p, cfg)
     if chunk < 1 or block_tables.shape[0] != R:
         raise ValueError("chunk must be positive and block_tables hold a row per prompt")
     q4, mats = _projections(eng, gemm)
