@@ -202,7 +202,7 @@ class BatchDecodeEngine:
         if packed:
             self.logits.copy_(prefill_packed(self, prompts, self.block_tables, chunk * self.batch))
             self.token.copy_(torch.argmax(self.logits.float(), dim=-1))
-            self.pos.copy_(torch.tensor([len(p) for p in prompts], dtype=torch.int64))
+            self.pos.copy_(torch.tensor([torch.as_tensor(p).numel() for p in prompts], dtype=torch.int64))
             self.step_idx.zero_()
             self.key.zero_()
             return self.token.clone()
