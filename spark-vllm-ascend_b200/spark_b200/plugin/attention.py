@@ -31,6 +31,7 @@ from __future__ import annotations
 
 import math
 import os
+import weakref
 from dataclasses import dataclass, field
 from typing import ClassVar
 
@@ -77,11 +78,47 @@ class SparkAttentionMetadata:
     max_split_tokens: int
     prefix_len: torch.Tensor | None = None  # int32 [1]: positions all requests share (cascade)
     plans: dict = field(default_factory=dict)  # this step's attention work lists, per head layout and window
-    plan_pool: dict = field(default_factory=dict)  # their buffers, kept by the builder from step to step
 
     @property
     def is_decode(self) -> bool:
         return self.max_query_len == 1
+
+
+class PlanPool:
+    """Attention plans (``ops.AttnPlan``) kept from step to step.
+
+    A plan holds one work list at a time, and every layer of a step reads it.  So metadata
+    objects that are alive together (micro-batches whose layers take turns, cache groups of
+    one layout) get a plan each: one is free again when the metadata object that took it is
+    gone.  Work that is still queued then stays in front of the next list's on the plan's
+    stream; a plan is not handed to another stream."""
+
+    def __init__(self):
+        self._plans: dict = {}  # (head layout, window, device) -> [[plan, its metadata, its stream]]
+
+    @staticmethod
+    def _stream(device):
+        return torch.cuda.current_stream(device) if torch.device(device).type == "cuda" else None
+
+    def take(self, layout, device, tokens: int, reqs: int, owner):
+        """A plan for up to ``tokens`` tokens and ``reqs`` requests that ``owner`` alone uses."""
+        entries = self._plans.setdefault((*layout, str(device)), [])
+        stream = self._stream(device)
+        free = [e for e in entries if e[1]() is None and e[2] == stream]
+        for e in free:
+            if e[0].max_tokens >= tokens and e[0].max_reqs >= reqs:
+                e[1] = weakref.ref(owner)
+                return e[0]
+        if free:  # too small: a larger one in its place
+            tokens, reqs = max(tokens, free[0][0].max_tokens), max(reqs, free[0][0].max_reqs)
+            entries.remove(free[0])
+        room = lambda n: 1 << max(n - 1, 63).bit_length()  # noqa: E731
+        plan = ops.AttnPlan(room(tokens), room(reqs), *layout[:3], device, layout[3])
+        entries.append([plan, weakref.ref(owner), stream])
+        return plan
+
+
+_pool = PlanPool()
 
 
 class SparkAttentionMetadataBuilder(AttentionMetadataBuilder[SparkAttentionMetadata]):
@@ -92,7 +129,6 @@ class SparkAttentionMetadataBuilder(AttentionMetadataBuilder[SparkAttentionMetad
         max_len = vllm_config.model_config.max_model_len if vllm_config is not None else 4096
         self.splits = choose_splits(max_len)
         self.max_split_tokens = split_tokens(max_len, self.splits)
-        self.plan_pool: dict = {}
 
     def use_cascade_attention(self, common_prefix_len: int, query_lens, num_query_heads: int, num_kv_heads: int,
                               use_alibi: bool, use_sliding_window: bool, use_local_attention: bool, num_sms: int,
@@ -110,7 +146,7 @@ class SparkAttentionMetadataBuilder(AttentionMetadataBuilder[SparkAttentionMetad
         if common_prefix_len > 0:
             prefix = torch.full((1,), common_prefix_len, dtype=torch.int32, device=cm.seq_lens.device)
         return SparkAttentionMetadata(
-            prefix_len=prefix, plan_pool=self.plan_pool if hasattr(self, "plan_pool") else {},
+            prefix_len=prefix,
             num_actual_tokens=cm.num_actual_tokens, num_reqs=cm.num_reqs, max_query_len=cm.max_query_len,
             max_seq_len=cm.max_seq_len, query_start_loc=cm.query_start_loc, query_start_loc_cpu=cm.query_start_loc_cpu,
             seq_lens=cm.seq_lens, block_table=cm.block_table_tensor, slot_mapping=cm.slot_mapping,
@@ -191,11 +227,8 @@ class SparkAttentionImpl(AttentionImpl[SparkAttentionMetadata]):
         key = (self.num_heads, self.num_kv_heads, self.head_size, self.window)
         plan = md.plans.get(key)
         if plan is None:
-            tokens, reqs = max(md.num_actual_tokens, md.num_reqs), md.num_reqs
-            plan = md.plan_pool.get(key)
-            if plan is None or plan.max_tokens < tokens or plan.max_reqs < reqs:
-                room = lambda n: 1 << max(n - 1, 63).bit_length()  # noqa: E731
-                plan = md.plan_pool[key] = ops.AttnPlan(room(tokens), room(reqs), *key[:3], device, self.window)
+            reqs = md.num_reqs
+            plan = _pool.take(key, device, max(md.num_actual_tokens, reqs), reqs, md)
             if md.is_decode and md.prefix_len is not None and not self.window:
                 plan.update_prefix(md.seq_lens[:reqs], md.prefix_len)
             else:

@@ -1,0 +1,119 @@
+"""CPU checks of the vLLM backend's paged path: which plan a step's layers use, what happens to
+status words, what the profiling run sets aside.  Plans are stood in for by objects that keep
+what they were given; no kernel is launched."""
+from __future__ import annotations
+
+import gc
+
+import pytest
+
+pytest.importorskip("vllm")
+
+
+class FakePlan:
+    made: list = []
+
+    def __init__(self, max_tokens, max_reqs, nq, nkv, head_dim, device, window=0):
+        import torch
+        self.max_tokens, self.max_reqs, self.nq, self.nkv = max_tokens, max_reqs, nq, nkv
+        self.head_dim, self.device, self.window = head_dim, device, window
+        self.error, self.kind, self.list = torch.zeros(1, dtype=torch.int32), None, None
+        FakePlan.made.append(self)
+
+    def update(self, query_start, seq_lens):
+        self.kind, self.list = "prompt", seq_lens.tolist()
+        return self
+
+    def update_prefix(self, seq_lens, prefix_len):
+        self.kind, self.list = "prefix", [int(prefix_len), *seq_lens.tolist()]
+        return self
+
+
+@pytest.fixture
+def attention(monkeypatch):
+    """The backend's module with fake plans, a pool of its own and the paged path switched on;
+    ``seen`` holds the work list of each attention call at the time of the call."""
+    from spark_b200.plugin import attention as A
+    monkeypatch.setenv(A.PAGED_ENV, "1")
+    monkeypatch.setattr(FakePlan, "made", [])
+    monkeypatch.setattr(A, "_pool", A.PlanPool())
+    monkeypatch.setattr(A.ops, "AttnPlan", FakePlan)
+    monkeypatch.setattr(A.ops, "kv_store_", lambda *a: None)
+    A.seen = []
+    call = lambda q, k, v, table, plan, scale, out, err: A.seen.append((plan.kind, plan.list))  # noqa: E731
+    monkeypatch.setattr(A.ops, "attn_prompt_out", call)
+    monkeypatch.setattr(A.ops, "attn_shared_prefix_out", call)
+    yield A
+    del A.seen
+
+
+def _metadata(A, seq_lens, query_lens, builder=None, prefix=0):
+    import torch
+    from vllm.v1.attention.backend import CommonAttentionMetadata
+    start = torch.tensor([0, *torch.tensor(query_lens).cumsum(0).tolist()], dtype=torch.int32)
+    builder = builder or _builder(A)
+    return builder.build(prefix, CommonAttentionMetadata(
+        query_start_loc=start, query_start_loc_cpu=start, seq_lens=torch.tensor(seq_lens, dtype=torch.int32),
+        num_reqs=len(seq_lens), num_actual_tokens=int(start[-1]), max_query_len=max(query_lens),
+        max_seq_len=max(seq_lens), block_table_tensor=torch.zeros((len(seq_lens), 8), dtype=torch.int32),
+        slot_mapping=torch.zeros(int(start[-1]), dtype=torch.int64)))
+
+
+def _builder(A, layers=0):
+    """A builder without vLLM's configuration, for ``layers`` layers."""
+    b = A.SparkAttentionMetadataBuilder.__new__(A.SparkAttentionMetadataBuilder)
+    b.splits, b.max_split_tokens, b.layer_names = 16, 128, [f"layer{i}" for i in range(layers)]
+    return b
+
+
+def _layer(impl, md, nq=8, nkv=2, d=128):
+    import torch
+    t = md.num_actual_tokens
+    x = lambda h: torch.zeros((t, h * d), dtype=torch.bfloat16)  # noqa: E731
+    return impl.forward(None, x(nq), x(nkv), x(nkv), torch.zeros((2, 1, nkv, 128, d), dtype=torch.bfloat16), md, x(nq))
+
+
+def test_metadata_alive_together_has_a_plan_each(attention):
+    """Two micro-batches whose layers take turns: every call has its own batch's work list."""
+    A = attention
+    impl = A.SparkAttentionImpl(8, 128, 0.1, 2)
+    builder = _builder(A)
+    one, two = _metadata(A, [70, 9], [60, 9], builder), _metadata(A, [5, 300], [5, 1], builder)
+    for _ in range(2):
+        _layer(impl, one)
+        _layer(impl, two)
+    assert A.seen == [("prompt", [70, 9]), ("prompt", [5, 300])] * 2
+    assert len(FakePlan.made) == 2
+
+
+def test_plans_are_used_again_by_later_steps(attention):
+    A = attention
+    impl = A.SparkAttentionImpl(8, 128, 0.1, 2)
+    for n in (70, 64, 3, 2):
+        md = _metadata(A, [n, 9], [n, 9])
+        _layer(impl, md)
+        _layer(impl, md)
+        del md
+        gc.collect()
+    assert [p.max_tokens for p in FakePlan.made] == [128]
+
+
+def test_a_larger_step_replaces_the_plan(attention):
+    A = attention
+    impl = A.SparkAttentionImpl(8, 128, 0.1, 2)
+    for n, reqs in ((2, 80), (500, 1), (20, 3), (2, 80)):
+        md = _metadata(A, [n] * reqs, [n] * reqs)
+        _layer(impl, md)
+        del md
+        gc.collect()
+    assert [(p.max_tokens, p.max_reqs) for p in FakePlan.made] == [(256, 128), (512, 128)]
+    assert sum(len(e) for e in A._pool._plans.values()) == 1
+
+
+def test_layouts_and_windows_have_plans_of_their_own(attention):
+    A = attention
+    md = _metadata(A, [30], [30])
+    full, slide = A.SparkAttentionImpl(16, 256, 0.1, 4), A.SparkAttentionImpl(16, 256, 0.1, 4, sliding_window=16)
+    for impl in (full, slide, full):
+        _layer(impl, md, 16, 4, 256)
+    assert [p.window for p in FakePlan.made] == [0, 17] and len(md.plans) == 2
