@@ -78,10 +78,65 @@ class SparkAttentionMetadata:
     max_split_tokens: int
     prefix_len: torch.Tensor | None = None  # int32 [1]: positions all requests share (cascade)
     plans: dict = field(default_factory=dict)  # this step's attention work lists, per head layout and window
+    layers_left: int = 0  # paged attention calls until the step's last (0: not known)
 
     @property
     def is_decode(self) -> bool:
         return self.max_query_len == 1
+
+
+class StepStatus:
+    """The status word of a device's paged steps (ERR_* bits of plans and attention calls) and its
+    way to the host: copied to pinned memory behind a step's last layer, looked at when a later
+    step is built, so that nothing waits.  A copy that is under way is looked at before the next
+    one is made, whose event would take its place."""
+
+    def __init__(self, device):
+        self.word = torch.zeros(1, dtype=torch.int32, device=device)
+        cuda = self.word.is_cuda
+        self._host = torch.zeros(1, dtype=torch.int32, pin_memory=cuda)
+        self._event = torch.cuda.Event() if cuda else None
+        self._stream = None
+        self._used = self._posted = False
+
+    def used(self) -> None:
+        """A call that may set bits was queued on the current stream."""
+        self._used = True
+        if self._event is not None:
+            self._stream = torch.cuda.current_stream(self.word.device)
+
+    def post(self) -> None:
+        if not self._used or self._posted:
+            return
+        if self._event is None:
+            self._host.copy_(self.word)
+        else:
+            with torch.cuda.stream(self._stream):
+                if torch.cuda.is_current_stream_capturing():
+                    return
+                self._host.copy_(self.word, non_blocking=True)
+                self._event.record()
+        self._used, self._posted = False, True
+
+    def check(self, wait: bool = False) -> None:
+        """Raise if a copy that has arrived (``wait``: the one under way, too) holds bits."""
+        if not self._posted:
+            return
+        if self._event is not None:
+            if wait:
+                self._event.synchronize()
+            elif not self._event.query():
+                return
+        self._posted = False
+        bits = int(self._host)
+        if bits:
+            if self._stream is not None:
+                with torch.cuda.stream(self._stream):
+                    self.word.zero_()
+            else:
+                self.word.zero_()
+            raise RuntimeError(f"paged attention: a step reported status {bits} (spark_b200.ops.ERR_* bits): "
+                               "its outputs are not valid")
 
 
 class PlanPool:
@@ -95,6 +150,21 @@ class PlanPool:
 
     def __init__(self):
         self._plans: dict = {}  # (head layout, window, device) -> [[plan, its metadata, its stream]]
+        self._status: dict = {}
+
+    def status(self, device) -> StepStatus:
+        st = self._status.get(str(device))
+        if st is None:
+            st = self._status[str(device)] = StepStatus(device)
+        return st
+
+    def check(self, wait: bool = False) -> None:
+        """Raise what earlier steps reported, and send for what has been used since."""
+        for st in self._status.values():
+            st.check(wait)
+            st.post()
+            if wait:
+                st.check(wait)
 
     @staticmethod
     def _stream(device):
@@ -114,11 +184,18 @@ class PlanPool:
             entries.remove(free[0])
         room = lambda n: 1 << max(n - 1, 63).bit_length()  # noqa: E731
         plan = ops.AttnPlan(room(tokens), room(reqs), *layout[:3], device, layout[3])
+        plan.error = self.status(device).word
         entries.append([plan, weakref.ref(owner), stream])
         return plan
 
 
 _pool = PlanPool()
+
+
+def raise_on_error() -> None:
+    """Wait for the paged steps that are queued and raise if one reported an error.  (Without a
+    call, a step's error is raised when a later step is built.)"""
+    _pool.check(wait=True)
 
 
 class SparkAttentionMetadataBuilder(AttentionMetadataBuilder[SparkAttentionMetadata]):
@@ -142,11 +219,12 @@ class SparkAttentionMetadataBuilder(AttentionMetadataBuilder[SparkAttentionMetad
     def build(self, common_prefix_len: int, common_attn_metadata: CommonAttentionMetadata,
               fast_build: bool = False) -> SparkAttentionMetadata:
         cm = common_attn_metadata
+        _pool.check()
         prefix = None
         if common_prefix_len > 0:
             prefix = torch.full((1,), common_prefix_len, dtype=torch.int32, device=cm.seq_lens.device)
         return SparkAttentionMetadata(
-            prefix_len=prefix,
+            prefix_len=prefix, layers_left=len(getattr(self, "layer_names", ())),
             num_actual_tokens=cm.num_actual_tokens, num_reqs=cm.num_reqs, max_query_len=cm.max_query_len,
             max_seq_len=cm.max_seq_len, query_start_loc=cm.query_start_loc, query_start_loc_cpu=cm.query_start_loc_cpu,
             seq_lens=cm.seq_lens, block_table=cm.block_table_tensor, slot_mapping=cm.slot_mapping,
@@ -237,12 +315,15 @@ class SparkAttentionImpl(AttentionImpl[SparkAttentionMetadata]):
         return plan
 
     def _paged_attention(self, q, k_cache, v_cache, md, out, output):
-        err = self._error.get(q.device)
-        if err is None:
-            err = self._error[q.device] = torch.zeros(1, dtype=torch.int32, device=q.device)
+        status = _pool.status(q.device)
+        self._error[q.device] = status.word
         plan = self._plan(md, q.device)
+        status.used()
         attend = ops.attn_prompt_out if plan.kind == "prompt" else ops.attn_shared_prefix_out
-        attend(q, k_cache, v_cache, md.block_table, plan, self.scale, out, err)
+        attend(q, k_cache, v_cache, md.block_table, plan, self.scale, out, status.word)
+        md.layers_left -= 1
+        if md.layers_left == 0:
+            status.post()
         return output
 
     def _step_state(self, md, device):

@@ -117,3 +117,62 @@ def test_layouts_and_windows_have_plans_of_their_own(attention):
     for impl in (full, slide, full):
         _layer(impl, md, 16, 4, 256)
     assert [p.window for p in FakePlan.made] == [0, 17] and len(md.plans) == 2
+
+
+def _failing(A, monkeypatch, bits):
+    """Attention calls set ``bits`` in the word that they are given."""
+    monkeypatch.setattr(A.ops, "attn_prompt_out", lambda q, k, v, t, plan, s, out, err: err.bitwise_or_(bits))
+
+
+@pytest.mark.parametrize("layers", [2, 0])  # (0: a builder that does not know its layers)
+def test_status_of_a_step_is_raised_when_a_later_one_is_built(attention, monkeypatch, layers):
+    A = attention
+    impl, builder = A.SparkAttentionImpl(8, 128, 0.1, 2), _builder(A, layers)
+    _failing(A, monkeypatch, 64)
+    md = _metadata(A, [30], [30], builder)
+    _layer(impl, md)
+    _layer(impl, md)
+    if not layers:  # (its copy is sent for by the next step's metadata)
+        md = _metadata(A, [30], [30], builder)
+    with pytest.raises(RuntimeError, match="status 64"):
+        _metadata(A, [30], [30], builder)
+    _metadata(A, [30], [30], builder)  # raised once; the word starts again from 0
+    _failing(A, monkeypatch, 0)
+    _layer(impl, md)
+    A.raise_on_error()
+
+
+def test_status_of_the_work_list_is_raised_too(attention):
+    A = attention
+    impl, builder = A.SparkAttentionImpl(8, 128, 0.1, 2), _builder(A, 1)
+    md = _metadata(A, [30], [30], builder)
+    _layer(impl, md)
+    next(iter(md.plans.values())).error.bitwise_or_(4)  # (what AttnPlan.update reports into)
+    _layer(impl, md)
+    with pytest.raises(RuntimeError, match="status 4"):
+        A.raise_on_error()
+    A.raise_on_error()
+
+
+def test_a_copy_that_is_under_way_is_not_overtaken(attention):
+    """Steps built before the last one's copy has arrived: it is raised by the first step that
+    finds it there."""
+    A = attention
+
+    class Event:
+        done = False
+        query = lambda self: Event.done  # noqa: E731
+        record = synchronize = lambda self: None  # noqa: E731
+
+    status = A._pool.status("cpu")
+    status.word.fill_(64)
+    status.used()
+    status.post()
+    status._event = Event()  # (the copy under way)
+    for _ in range(3):
+        status._used = True
+        A._pool.check()
+        assert status._posted and status._used
+    Event.done = True
+    with pytest.raises(RuntimeError):
+        A._pool.check()

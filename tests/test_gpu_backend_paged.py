@@ -159,3 +159,28 @@ def test_backend_micro_batches_take_turns(cuda, monkeypatch):
         want = _oracle(q.cpu().view(-1, nq, D), kv.cpu(), table.cpu(), lens, new, nq, nkv, D, 0)
         for out in outs:
             assert _within(out.view(-1, nq, D), *want)
+
+
+def test_backend_raises_a_bad_page_when_the_next_step_is_built(cuda, monkeypatch):
+    """A table entry outside the cache: no step is waited for, the next one's metadata raises;
+    afterwards the backend goes on, and right."""
+    import torch
+    from spark_b200.plugin import attention as A
+    monkeypatch.setenv(A.PAGED_ENV, "1")
+    A.raise_on_error()  # (nothing is left from before)
+    nq, nkv, D, lens, new = 8, 2, 128, [200, 90], [200, 30]
+    impl, builder = A.SparkAttentionImpl(nq, D, 1 / math.sqrt(D), nkv), _builder(1)
+    q, k, v, kv, table, slots = _mixed(lens, new, nq, nkv, D, seed=9)
+    bad = table.clone()
+    bad[1, 0] = 1 << 20
+    impl.forward(None, q, k, v, kv, _build(builder, lens, new, bad, slots), torch.zeros_like(q))
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="status 64"):
+        _build(builder, lens, new, table, slots)
+    out = torch.zeros_like(q)
+    impl.forward(None, q, k, v, kv, _build(builder, lens, new, table, slots), out)
+    A.raise_on_error()
+    assert _within(out.view(-1, nq, D), *_oracle(q.cpu().view(-1, nq, D), kv.cpu(), table.cpu(), lens, new, nq, nkv, D, 0))
+    impl.forward(None, q, k, v, kv, _build(builder, lens, new, bad, slots), out)
+    with pytest.raises(RuntimeError, match="status 64"):
+        A.raise_on_error()
