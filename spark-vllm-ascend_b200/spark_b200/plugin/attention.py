@@ -38,6 +38,7 @@ from typing import ClassVar
 import ctypes
 
 import torch
+from vllm.config import get_current_vllm_config_or_none
 from vllm.v1.attention.backend import (AttentionBackend, AttentionCGSupport, AttentionImpl, AttentionMetadataBuilder,
                                        AttentionType, CommonAttentionMetadata)
 
@@ -146,7 +147,7 @@ class PlanPool:
     objects that are alive together (micro-batches whose layers take turns, cache groups of
     one layout) get a plan each: one is free again when the metadata object that took it is
     gone.  Work that is still queued then stays in front of the next list's on the plan's
-    stream; a plan is not handed to another stream."""
+    stream; a plan that was used is not handed to another stream."""
 
     def __init__(self):
         self._plans: dict = {}  # (head layout, window, device) -> [[plan, its metadata, its stream]]
@@ -170,20 +171,36 @@ class PlanPool:
     def _stream(device):
         return torch.cuda.current_stream(device) if torch.device(device).type == "cuda" else None
 
+    @staticmethod
+    def _make(layout, device, tokens: int, reqs: int):
+        room = lambda n: 1 << max(n - 1, 63).bit_length()  # noqa: E731
+        return ops.AttnPlan(room(tokens), room(reqs), *layout[:3], device, layout[3])
+
+    def reserve(self, layout, device, tokens: int, reqs: int) -> None:
+        """Have a plan of this layout before the first step, bound to no stream yet (vLLM's
+        profiling run counts the memory that is taken then)."""
+        entries = self._plans.setdefault((*layout, str(device)), [])
+        if not entries:
+            plan = self._make(layout, device, tokens, reqs)
+            plan.error = self.status(device).word
+            entries.append([plan, lambda: None, None])
+
     def take(self, layout, device, tokens: int, reqs: int, owner):
         """A plan for up to ``tokens`` tokens and ``reqs`` requests that ``owner`` alone uses."""
         entries = self._plans.setdefault((*layout, str(device)), [])
         stream = self._stream(device)
-        free = [e for e in entries if e[1]() is None and e[2] == stream]
+        free = [e for e in entries if e[1]() is None and e[2] in (None, stream)]
         for e in free:
             if e[0].max_tokens >= tokens and e[0].max_reqs >= reqs:
-                e[1] = weakref.ref(owner)
+                if e[2] is None and stream is not None:  # (its memory may be another stream's)
+                    for t in (e[0].buf, e[0].part_o, e[0].part_ml):
+                        t.record_stream(stream)
+                e[1], e[2] = weakref.ref(owner), stream
                 return e[0]
         if free:  # too small: a larger one in its place
             tokens, reqs = max(tokens, free[0][0].max_tokens), max(reqs, free[0][0].max_reqs)
             entries.remove(free[0])
-        room = lambda n: 1 << max(n - 1, 63).bit_length()  # noqa: E731
-        plan = ops.AttnPlan(room(tokens), room(reqs), *layout[:3], device, layout[3])
+        plan = self._make(layout, device, tokens, reqs)
         plan.error = self.status(device).word
         entries.append([plan, weakref.ref(owner), stream])
         return plan
@@ -260,6 +277,9 @@ class SparkAttentionImpl(AttentionImpl[SparkAttentionMetadata]):
         self._step = None
         self._paged = paged_attention()
         self._error: dict = {}
+        self._layout = (num_heads, self.num_kv_heads, head_size, self.window)
+        config = get_current_vllm_config_or_none()
+        self._max_reqs = config.scheduler_config.max_num_seqs if config is not None else 1
 
     def _workspace(self, splits: int, device) -> tuple:
         key = (splits, device)
@@ -277,6 +297,8 @@ class SparkAttentionImpl(AttentionImpl[SparkAttentionMetadata]):
                 attn_metadata: SparkAttentionMetadata, output: torch.Tensor, output_scale: torch.Tensor | None = None,
                 output_block_scale: torch.Tensor | None = None) -> torch.Tensor:
         if attn_metadata is None:  # profiling run
+            if self._paged and not (query.is_cuda and torch.cuda.is_current_stream_capturing()):
+                _pool.reserve(self._layout, query.device, query.shape[0], self._max_reqs)
             return output.fill_(0)
         md = attn_metadata
         nq, nkv, d = self.num_heads, self.num_kv_heads, self.head_size
@@ -302,7 +324,7 @@ class SparkAttentionImpl(AttentionImpl[SparkAttentionMetadata]):
     def _plan(self, md, device):
         """This step's work list: made by the first layer of a head layout and window, used
         by the others."""
-        key = (self.num_heads, self.num_kv_heads, self.head_size, self.window)
+        key = self._layout
         plan = md.plans.get(key)
         if plan is None:
             reqs = md.num_reqs

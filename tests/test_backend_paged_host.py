@@ -176,3 +176,35 @@ def test_a_copy_that_is_under_way_is_not_overtaken(attention):
     Event.done = True
     with pytest.raises(RuntimeError):
         A._pool.check()
+
+
+def test_the_profiling_run_sets_the_workspace_aside(attention, monkeypatch):
+    """A run without metadata (vLLM measures its memory) makes a plan per layout for the tokens
+    that it carries and the scheduler's requests; the steps use it."""
+    import types
+    import torch
+    A = attention
+    config = types.SimpleNamespace(scheduler_config=types.SimpleNamespace(max_num_seqs=200))
+    monkeypatch.setattr(A, "get_current_vllm_config_or_none", lambda: config)
+    impls = [A.SparkAttentionImpl(16, 256, 0.1, 4, sliding_window=w) for w in (None, 16, 16)]
+    x = torch.ones((5000, 16 * 256), dtype=torch.bfloat16)
+    for impl in impls:
+        assert not impl.forward(None, x, None, None, None, None, x.clone()).any()
+    assert [(p.max_tokens, p.max_reqs, p.window) for p in FakePlan.made] == [(8192, 256, 0), (8192, 256, 17)]
+    for n in (30, 4000):
+        md = _metadata(A, [n] * 3, [n // 3] * 3)
+        for impl in impls:
+            _layer(impl, md, 16, 4, 256)
+        del md
+        gc.collect()
+    assert len(FakePlan.made) == 2
+    assert all(p.error is A._pool.status("cpu").word for p in FakePlan.made)
+
+
+def test_the_profiling_run_takes_nothing_with_the_switch_off(attention, monkeypatch):
+    import torch
+    A = attention
+    monkeypatch.delenv(A.PAGED_ENV)
+    x = torch.ones((50, 8 * 128), dtype=torch.bfloat16)
+    A.SparkAttentionImpl(8, 128, 0.1, 2).forward(None, x, None, None, None, None, x)
+    assert not FakePlan.made

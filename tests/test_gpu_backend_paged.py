@@ -184,3 +184,27 @@ def test_backend_raises_a_bad_page_when_the_next_step_is_built(cuda, monkeypatch
     impl.forward(None, q, k, v, kv, _build(builder, lens, new, bad, slots), out)
     with pytest.raises(RuntimeError, match="status 64"):
         A.raise_on_error()
+
+
+def test_backend_profiling_run_counts_the_workspace(cuda, monkeypatch):
+    """The plan of the profiling run is the steps' one: no memory of its size is taken later, also
+    when they run on another stream."""
+    import torch
+    from spark_b200.plugin import attention as A
+    monkeypatch.setenv(A.PAGED_ENV, "1")
+    monkeypatch.setattr(A, "_pool", A.PlanPool())
+    nq, nkv, D, lens, new = 32, 8, 128, [200, 90], [200, 30]
+    impl, builder = A.SparkAttentionImpl(nq, D, 1 / math.sqrt(D), nkv), _builder(1)
+    q, k, v, kv, table, slots = _mixed(lens, new, nq, nkv, D, seed=10)
+    md, out, side = _build(builder, lens, new, table, slots), torch.zeros_like(q), torch.cuda.Stream()
+    before = torch.cuda.memory_allocated()  # (with the step's own output, 230 x 4096 x 2 bytes)
+    impl.forward(None, torch.zeros((1024, nq * D), dtype=torch.bfloat16, device="cuda"), None, None, None, None,
+                 torch.empty_like(q))
+    held = torch.cuda.memory_allocated() - before
+    assert held > 100 << 20
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        impl.forward(None, q, k, v, kv, md, out)
+        A.raise_on_error()
+    assert torch.cuda.memory_allocated() - before < held + (1 << 20)
+    assert _within(out.view(-1, nq, D), *_oracle(q.cpu().view(-1, nq, D), kv.cpu(), table.cpu(), lens, new, nq, nkv, D, 0))
