@@ -31,6 +31,7 @@ from __future__ import annotations
 
 import math
 import os
+import threading
 import weakref
 from dataclasses import dataclass, field
 from typing import ClassVar
@@ -86,6 +87,12 @@ class SparkAttentionMetadata:
         return self.max_query_len == 1
 
 
+def _settle(device) -> None:
+    """What was just zeroed on the current stream may be another stream's from now on."""
+    if torch.device(device).type == "cuda" and not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(device).synchronize()
+
+
 class StepStatus:
     """The status word of a device's paged steps (ERR_* bits of plans and attention calls) and its
     way to the host: copied to pinned memory behind a step's last layer, looked at when a later
@@ -99,6 +106,7 @@ class StepStatus:
         self._event = torch.cuda.Event() if cuda else None
         self._stream = None
         self._used = self._posted = False
+        _settle(device)
 
     def used(self) -> None:
         """A call that may set bits was queued on the current stream."""
@@ -152,11 +160,13 @@ class PlanPool:
     def __init__(self):
         self._plans: dict = {}  # (head layout, window, device) -> [[plan, its metadata, its stream]]
         self._status: dict = {}
+        self._lock = threading.RLock()  # (micro-batches may run in threads of their own)
 
     def status(self, device) -> StepStatus:
         st = self._status.get(str(device))
         if st is None:
-            st = self._status[str(device)] = StepStatus(device)
+            with self._lock:
+                st = self._status.get(str(device)) or self._status.setdefault(str(device), StepStatus(device))
         return st
 
     def check(self, wait: bool = False) -> None:
@@ -171,39 +181,41 @@ class PlanPool:
     def _stream(device):
         return torch.cuda.current_stream(device) if torch.device(device).type == "cuda" else None
 
-    @staticmethod
-    def _make(layout, device, tokens: int, reqs: int):
+    def _make(self, layout, device, tokens: int, reqs: int):
         room = lambda n: 1 << max(n - 1, 63).bit_length()  # noqa: E731
-        return ops.AttnPlan(room(tokens), room(reqs), *layout[:3], device, layout[3])
+        plan = ops.AttnPlan(room(tokens), room(reqs), *layout[:3], device, layout[3])
+        plan.error = self.status(device).word
+        return plan
 
     def reserve(self, layout, device, tokens: int, reqs: int) -> None:
         """Have a plan of this layout before the first step, bound to no stream yet (vLLM's
         profiling run counts the memory that is taken then)."""
-        entries = self._plans.setdefault((*layout, str(device)), [])
-        if not entries:
-            plan = self._make(layout, device, tokens, reqs)
-            plan.error = self.status(device).word
-            entries.append([plan, lambda: None, None])
+        with self._lock:
+            entries = self._plans.setdefault((*layout, str(device)), [])
+            if not entries:
+                plan = self._make(layout, device, tokens, reqs)
+                _settle(device)
+                entries.append([plan, lambda: None, None])
 
     def take(self, layout, device, tokens: int, reqs: int, owner):
         """A plan for up to ``tokens`` tokens and ``reqs`` requests that ``owner`` alone uses."""
-        entries = self._plans.setdefault((*layout, str(device)), [])
-        stream = self._stream(device)
-        free = [e for e in entries if e[1]() is None and e[2] in (None, stream)]
-        for e in free:
-            if e[0].max_tokens >= tokens and e[0].max_reqs >= reqs:
-                if e[2] is None and stream is not None:  # (its memory may be another stream's)
-                    for t in (e[0].buf, e[0].part_o, e[0].part_ml):
-                        t.record_stream(stream)
-                e[1], e[2] = weakref.ref(owner), stream
-                return e[0]
-        if free:  # too small: a larger one in its place
-            tokens, reqs = max(tokens, free[0][0].max_tokens), max(reqs, free[0][0].max_reqs)
-            entries.remove(free[0])
-        plan = self._make(layout, device, tokens, reqs)
-        plan.error = self.status(device).word
-        entries.append([plan, weakref.ref(owner), stream])
-        return plan
+        with self._lock:
+            entries = self._plans.setdefault((*layout, str(device)), [])
+            stream = self._stream(device)
+            free = [e for e in entries if e[1]() is None and e[2] in (None, stream)]
+            for e in free:
+                if e[0].max_tokens >= tokens and e[0].max_reqs >= reqs:
+                    if e[2] is None and stream is not None:  # (its memory may be another stream's)
+                        for t in (e[0].buf, e[0].part_o, e[0].part_ml):
+                            t.record_stream(stream)
+                    e[1], e[2] = weakref.ref(owner), stream
+                    return e[0]
+            if free:  # too small: a larger one in its place
+                tokens, reqs = max(tokens, free[0][0].max_tokens), max(reqs, free[0][0].max_reqs)
+                entries.remove(free[0])
+            plan = self._make(layout, device, tokens, reqs)
+            entries.append([plan, weakref.ref(owner), stream])
+            return plan
 
 
 _pool = PlanPool()

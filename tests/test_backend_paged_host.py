@@ -208,3 +208,29 @@ def test_the_profiling_run_takes_nothing_with_the_switch_off(attention, monkeypa
     x = torch.ones((50, 8 * 128), dtype=torch.bfloat16)
     A.SparkAttentionImpl(8, 128, 0.1, 2).forward(None, x, None, None, None, None, x)
     assert not FakePlan.made
+
+
+def test_threads_that_ask_at_once_get_a_plan_each(attention, monkeypatch):
+    """Micro-batches may run in threads of their own: a switch between the look at a free plan
+    and taking it (here while its size is read) hands it out once."""
+    import threading
+    import time
+    A = attention
+
+    class Slow(FakePlan):
+        max_tokens = property(lambda self: (time.sleep(0.05), self._n)[1],
+                              lambda self, n: setattr(self, "_n", n))
+
+    monkeypatch.setattr(A.ops, "AttnPlan", Slow)
+    layout, mds, got = (8, 2, 128, 0), [_metadata(A, [30], [30]) for _ in range(2)], [None, None]
+    A._pool.reserve(layout, "cpu", 64, 4)
+
+    def ask(i):
+        got[i] = A._pool.take(layout, "cpu", 30, 1, mds[i])
+
+    threads = [threading.Thread(target=ask, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert got[0] is not got[1] and None not in got
