@@ -184,7 +184,8 @@ class PlanPool:
     def _make(self, layout, device, tokens: int, reqs: int):
         room = lambda n: 1 << max(n - 1, 63).bit_length()  # noqa: E731
         plan = ops.AttnPlan(room(tokens), room(reqs), *layout[:3], device, layout[3])
-        plan.error = self.status(device).word
+        plan.status = self.status(device)
+        plan.error = plan.status.word
         return plan
 
     def reserve(self, layout, device, tokens: int, reqs: int) -> None:
@@ -349,9 +350,9 @@ class SparkAttentionImpl(AttentionImpl[SparkAttentionMetadata]):
         return plan
 
     def _paged_attention(self, q, k_cache, v_cache, md, out, output):
-        status = _pool.status(q.device)
-        self._error[q.device] = status.word
         plan = self._plan(md, q.device)
+        status = plan.status
+        self._error[q.device] = status.word
         status.used()
         attend = ops.attn_prompt_out if plan.kind == "prompt" else ops.attn_shared_prefix_out
         attend(q, k_cache, v_cache, md.block_table, plan, self.scale, out, status.word)
