@@ -294,9 +294,13 @@ int spark_attn_plan(const int32_t* query_start, const int32_t* seq_lens, const i
 /* Attention of the planned batch over the paged caches (bf16
  * [num_blocks][nkv][block_size][head_dim], block_size a multiple of 16): for query token
  * t (q + t * q_tok_stride + head * q_head_stride, bf16) out = softmax(scale * q.k) v over
- * the keys its plan gives it, fp32 statistics; a token without keys is zero.  Rows of out
- * behind the last planned token are left alone.  K and V of positions at or past a
- * request's length may hold anything (NaN included).  head_dim 128 or 256, nq / nkv any
+ * the keys its plan gives it; scores, exponentials, sums and joins are fp32, the probabilities
+ * are rounded to bf16 as an operand of the product with V, the output once.  A token without
+ * keys is zero; rows of out behind the last planned token are left alone.  K and V of
+ * positions at or past a request's length may hold anything (NaN included), and so may a K that
+ * no row sees; V of the positions it holds must be finite (a weight of 0 still multiplies it).
+ * A row that sees a NaN score or one of +inf is NaN, a score of -inf has no weight.  out may not
+ * overlap the inputs or the workspace.  head_dim 128 or 256, nq / nkv any
  * integer up to 128, scale > 0; strides in elements, multiples of 8.  The maxima, head
  * layout and window must be the plan's (else bit 512 and nothing is written), and block_table
  * has a row for each of its requests (spark_attn_paged_bounded checks that on the device).  part_o fp32 [spark_attn_part_rows][nkv][head_dim] and part_ml fp32

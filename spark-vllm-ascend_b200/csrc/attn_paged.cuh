@@ -44,16 +44,17 @@
 // when every warp of the half has rescaled its columns of it, or read them out for the last
 // item.
 //
-// Measured (32 query and 8 kv heads of 128): a causal prompt of 16384 1.97 ms = 1118 TFLOP/s (1044 when
-// repeated until the power cap takes the clock to 1.63 GHz), of 2048 47 us; 8 tokens behind 32768
-// keys each 136 us = 6.1 TB/s.  A unit of 256 rows x 128 keys takes 1.93 us (head_dim 256, 128 rows:
-// 1.68 us) where its products alone take 1.15: a half's scores, maximum, probabilities and sums
-// follow one another, two halves fill each other's gaps, and a third set of scores has no room in
-// tensor memory.  Around an item 3-4 us, around a call (with the join) 9-10 us.
+// Measured (32 query and 8 kv heads of 128): a causal prompt of 16384 1.88 ms = 1170 TFLOP/s in a burst
+// (2.13 ms when repeated until the power cap takes the clock down), of 2048 47 us; 8 tokens behind
+// 17.9k to 32.8k keys (836 MB) 137-143 us = 5.8-6.1 TB/s.  A unit of 256 rows x 128 keys takes 1.95 us
+// (head_dim 256, 128 rows: 1.6-1.7 us) where its products alone take 1.15: a half's scores, maximum,
+// probabilities and sums follow one another, two halves fill each other's gaps, and a third set of
+// scores has no room in tensor memory.  Around an item 3-4 us, around a call (with the join) 9-10 us.
 //
 // Stale memory: a K / V row at or past the request's length (or before the window) may hold
 // anything.  Scores are masked by selection, and V rows outside [klo, len) are zeroed in
-// shared memory before their product, since 0 * NaN is NaN.
+// shared memory before their product, since 0 * NaN is NaN.  (V at positions in between has to be
+// finite: one that is not reaches that column of every row of the tile.)
 //
 // Every mbarrier wait is bounded by %globaltimer; one that runs out sets bit 1 of *error
 // and an abort flag that every other wait checks.  Before the CTA gives up shared or

@@ -363,7 +363,8 @@ def paged_plan_out(ctx_lens, new_lens, block_table, block_size, query_start, seq
     pages' ids into ``block_table`` and the advanced head into ``free_head_out`` (default:
     ``free_head`` itself).  All or nothing: a batch that does not fit comes out empty, with
     the reason in ``error`` (ERR_* bits).  ``counter`` int32 [1], zero before the first call
-    and left zero; calls that may overlap on the device need one each."""
+    and left zero; calls that may overlap on the device need one each.  No output may overlap
+    an input or another output."""
     i32 = torch.int32
     dev = _home(ctx_lens, "ctx_lens", i32)
     R, rows = ctx_lens.numel(), positions.numel()
@@ -536,17 +537,19 @@ def attn_prompt_out(q, k_cache, v_cache, block_table, plan: AttnPlan, scale, out
     multiples of 8), caches bf16 [blocks, nkv, block_size, D], block_table int32 [R, pages].
     Whole prompts, chunks on top of cached context and single tokens alike; tokens without
     keys give zero, rows of ``out`` behind the last planned token are left as they were.
-    Keys and values at positions a request does hold must be finite; what its pages carry
-    past its length does not matter.  ``error`` (int32 [1], required): nonzero, out is not
-    valid (ERR_* bits)."""
+    Scores and sums are fp32, the probabilities are rounded to bf16 as an operand of the product
+    with V.  Values at positions a request does hold must be finite; what its pages carry past
+    its length does not matter.  A row that sees a NaN or +inf score is NaN.  ``error`` (int32
+    [1], required): nonzero, out is not valid (ERR_* bits)."""
     return _attn_paged("prompt", q, k_cache, v_cache, block_table, plan, scale, out, error, wait_ns)
 
 
 def attn_shared_prefix_out(q, k_cache, v_cache, block_table, plan: AttnPlan, scale, out, error, wait_ns: int = -1):
     """Attention of one query token per request (q / out bf16 [R, nq, D]) where all requests
     share their first positions (``plan.update_prefix``): the prefix's pages are read once
-    for the whole batch, through the first request's table, each request's own keys through
-    its own; the parts join by log-sum-exp.  Otherwise as ``attn_prompt_out``."""
+    for the whole batch, through the first request's table (which must hold as much of it as
+    the longest request has), each request's own keys through its own; the parts join by
+    log-sum-exp.  Otherwise as ``attn_prompt_out``."""
     _check(q.shape[0] >= plan.reqs, "q must have a row per request")
     return _attn_paged("prefix", q, k_cache, v_cache, block_table, plan, scale, out, error, wait_ns)
 

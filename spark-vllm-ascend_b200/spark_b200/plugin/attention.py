@@ -24,8 +24,10 @@ metadata to the sm_100a kernels:
   chunks, mixed batches) runs the paged attention kernel instead (``ops.attn_prompt_out``:
   one launch for all requests, reading the pages in place, no host copy of the lengths), and
   the backend asks vLLM for cascade attention, so that decode batches with a common prefix
-  read it once (``ops.attn_shared_prefix_out``).  Off by default: its outputs differ from
-  the torch path's in the last bf16 bit.
+  read it once (``ops.attn_shared_prefix_out``).  Off by default: its probabilities are
+  rounded to bf16 where the torch path's are fp32, so its outputs differ by up to 2^-8 of
+  sum p |v| (several bf16 steps where the sum cancels).  What a step's kernels report is
+  raised when a later step is built (``raise_on_error`` waits for it).
 """
 from __future__ import annotations
 
